@@ -41,7 +41,7 @@ __device__ __forceinline__ void cora_gelu_both(float a, float& g, float& gp) {
   gp = __builtin_fmaf(a * s_ * r, du, s_);
 }
 
-// two values per call on the packed fp32 pipe (v_pk_mul_f32 / v_pk_fma_f32); exp2 / rcp stay scalar
+// two values per call (the build keeps packed fp32 arithmetic off, so this compiles to scalar operations)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void cora_gelu_both2(f32x2 a, f32x2& g, f32x2& gp) {
   const f32x2 a2 = a * a;
