@@ -10,6 +10,7 @@ from .inference import calculate_psnr, extract_features_from_batch, make_mask, u
 from .loops import eval_pretext_metrics, train
 from .optim import (Optim, adamw, chain, clip_by_global_norm, create_learning_rate_schedule,
                     make_optimizers, sgd)
+from .ops import attention, attention_backward, orthogonalize, rotary, rotary_backward
 from .serialisation import load_params, save_params
 
 __all__ = [
@@ -18,5 +19,5 @@ __all__ = [
     "VodeParam", "energy", "forward", "layer_energies", "step", "step_energies", "train_on_batch",
     "Optim", "adamw", "chain", "clip_by_global_norm", "create_learning_rate_schedule",
     "make_optimizers", "sgd", "load_params", "save_params", "calculate_psnr", "extract_features_from_batch",
-    "make_mask", "unmask_on_batch_enhanced", "eval_pretext_metrics", "train",
+    "attention", "attention_backward", "orthogonalize", "rotary", "rotary_backward", "make_mask", "unmask_on_batch_enhanced", "eval_pretext_metrics", "train",
 ]

@@ -28,6 +28,24 @@ class CoraStepOut(C.Structure):
                 ("train_mse", C.c_double), ("infer_ms", C.c_float), ("learn_ms", C.c_float)]
 
 
+def _struct(name: str, *fields):
+    """ctypes structure from (type, "name name ..") groups"""
+    return type(name, (C.Structure,), {"_fields_": [(n, t) for t, names in fields for n in names.split()]})
+
+
+CoraRotaryArgs = _struct(
+    "CoraRotaryArgs", (C.c_int32, "dtype heads head_dim n_axes"), (C.c_int32 * 4, "axes_dim"),
+    (C.c_int32, "interleaved backward"), (C.c_double, "theta"), (C.c_int64, "rows pos_rows"), (C.c_void_p, "pos x y"),
+    (C.c_int64, "x_row x_head y_row y_head"))
+CoraAttentionArgs = _struct(
+    "CoraAttentionArgs", (C.c_int32, "dtype heads kv_heads head_dim n_seq seq_len causal_block"), (C.c_float, "scale"),
+    (C.c_int64, "rows"), (C.c_void_p, "cu_seqlens q k v out lse dout dq dk dv"),
+    (C.c_int64, "q_row q_head k_row k_head v_row v_head out_row out_head"),
+    (C.c_int64, "dout_row dout_head dq_row dq_head dk_row dk_head dv_row dv_head"),
+    (C.c_void_p, "workspace"), (C.c_size_t, "workspace_bytes"))
+CoraMatrices = _struct(
+    "CoraMatrices", (C.c_void_p, "x y"), (C.c_int64, "x_mat x_row y_mat y_row"), (C.c_int32, "count rows cols"))
+
 # name -> (restype, argtypes); every symbol include/cora_hip.h declares
 _P = C.c_void_p
 _FP = C.POINTER(C.c_float)
@@ -83,6 +101,12 @@ SIGNATURES = {
     "cora_profile_step": (C.c_int, [_P, C.c_int, _P, _P, _P, _P, _P, C.POINTER(C.c_int)]),
     "cora_sync": (C.c_int, [_P]),
     "cora_kernel_path": (C.c_int, [_P]),
+    "cora_rotary": (C.c_int, [C.POINTER(CoraRotaryArgs), C.c_int, _P]),
+    "cora_attention": (C.c_int, [C.POINTER(CoraAttentionArgs), C.c_int, _P]),
+    "cora_attention_backward": (C.c_int, [C.POINTER(CoraAttentionArgs), C.c_int, _P]),
+    "cora_attention_workspace": (_SZ, [C.POINTER(CoraAttentionArgs)]),
+    "cora_orthogonalize_workspace": (_SZ, [C.c_int, C.POINTER(CoraMatrices), C.c_int]),
+    "cora_orthogonalize": (C.c_int, [C.c_int, C.POINTER(CoraMatrices), C.c_int, C.c_int, _P, C.c_float, _P, _SZ, C.c_int, _P]),
 }
 
 _lib: Optional[C.CDLL] = None

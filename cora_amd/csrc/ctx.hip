@@ -57,6 +57,11 @@ const char* rccl_load() {   // nullptr on success, else what failed
 
 }  // namespace
 
+// message of the last call without a ctx on this thread (cora_last_error(NULL)); also set by op_api.hip
+void cora_note_error(const char* msg) noexcept {
+  try { g_create_err = msg; } catch (...) {}
+}
+
 // ---- allocation-free entry point (cora_forward_static): its scratch lives in the code object ---------
 // 16 MiB per GPU, held from module load until the process ends.  In HOST code the array's name is only
 // a stand-in for the symbol, not a device address: the per-device address comes from

@@ -1,0 +1,110 @@
+// op_rotary.hip -- rotary positions over several axes (time, height, width), forward and backward (gfx950).
+//
+// Axis a owns n_a consecutive channels of every head; its pair i (of n_a / 2) turns by the angle pos_a theta^(-2 i / n_a):
+//   (u, v) -> (u cos - v sin, u sin + v cos)
+// with u, v neighbours (interleaved) or n_a / 2 channels apart.  The map is orthogonal, so the backward pass is the same
+// kernel with the opposite sign.  Channels behind the last axis pass through.
+//
+// The angle of a far position loses its fraction in 32 bits (position 1e6 times a frequency near 1 is off by 0.06), so
+// turns = pos * (theta^(-2 i / n) / 2 pi) and the reduction to a quarter turn are done in 64 bits; sine and cosine of what
+// is left, in [-pi/4, pi/4], are taken in 32.  A thread does this once for its channels of a row and then walks the heads,
+// which share the angles: the kernel is bound by reading and writing x.
+#include "ops.h"
+
+namespace {
+
+// cos, sin of 2 pi turns
+__device__ __forceinline__ void turn_cs(double turns, float sign, float& c, float& s) {
+  const double t4 = 4.0 * turns, q = rint(t4);
+  const float f = 0.5f * (float)(t4 - q);               // [-1/4, 1/4] half turns
+  const int k = (int)(q - 4.0 * floor(0.25 * q));       // quarter turns mod 4, exact for any position
+  float fs, fc;
+  sincospif(f, &fs, &fc);
+  const float a = (k & 1) ? fs : fc, b = (k & 1) ? fc : fs;
+  c = (k == 1 || k == 2) ? -a : a;
+  s = ((k >= 2) ? -b : b) * sign;
+}
+
+template <typename T, int V> struct VecOf { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct VecOf<T, 1> { struct type { T v; __device__ T& operator[](int) { return v; } }; };
+
+// MODE 0: one pair (or one passed channel) a thread, any layout; 1: 16 bytes of neighbouring pairs; 2: two 16-byte pieces,
+// the first and second channels of V pairs
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const int units, const int hchunk) {
+  constexpr int V = MODE == 0 ? 1 : 16 / (int)sizeof(T), NPAIR = MODE == 1 ? V / 2 : V;
+  typedef typename VecOf<T, V>::type vec;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / units;
+  if (row >= p.rows) return;
+  const int u = (int)(id - row * units);
+  const int h0 = blockIdx.y * hchunk, h1 = min(p.heads, h0 + hchunk);
+  const int turning = MODE == 1 ? 2 * p.pairs / V : p.pairs / V;
+  const T* x = (const T*)p.x + row * p.xr + h0 * p.xh;
+  T* y = (T*)p.y + row * p.yr + h0 * p.yh;
+  if (u >= turning) {                                    // channels that pass through
+    const int c = 2 * p.pairs + (u - turning) * V;
+    for (int h = h0; h < h1; ++h, x += p.xh, y += p.yh) *reinterpret_cast<vec*>(y + c) = *reinterpret_cast<const vec*>(x + c);
+    return;
+  }
+  const int* pos = p.pos + (row % p.pos_rows) * p.n_axes;
+  float cs[NPAIR], sn[NPAIR];
+#pragma unroll
+  for (int i = 0; i < NPAIR; ++i) {
+    const int pr = u * NPAIR + i;
+    turn_cs((double)pos[p.axis[pr]] * p.turn[pr], p.sign, cs[i], sn[i]);
+  }
+  const int ca = MODE == 1 ? u * V : p.c0[u * NPAIR], cb = MODE == 1 ? 0 : p.c1[u * NPAIR];
+#pragma unroll 4
+  for (int h = h0; h < h1; ++h, x += p.xh, y += p.yh) {
+    if (MODE == 1) {
+      vec a = *reinterpret_cast<const vec*>(x + ca);
+#pragma unroll
+      for (int i = 0; i < NPAIR; ++i) {
+        const float ua = (float)a[2 * i], ub = (float)a[(2 * i + 1) % V];
+        a[2 * i] = (T)(ua * cs[i] - ub * sn[i]);
+        a[(2 * i + 1) % V] = (T)(ua * sn[i] + ub * cs[i]);
+      }
+      *reinterpret_cast<vec*>(y + ca) = a;
+    } else {
+      vec a = *reinterpret_cast<const vec*>(x + ca), b = *reinterpret_cast<const vec*>(x + cb);
+#pragma unroll
+      for (int i = 0; i < NPAIR; ++i) {
+        const float ua = (float)a[i], ub = (float)b[i];
+        a[i] = (T)(ua * cs[i] - ub * sn[i]);
+        b[i] = (T)(ua * sn[i] + ub * cs[i]);
+      }
+      *reinterpret_cast<vec*>(y + ca) = a;
+      *reinterpret_cast<vec*>(y + cb) = b;
+    }
+  }
+}
+
+template <typename T> int run(const RotaryP& p, hipStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  // 16-byte pieces where every address is a multiple of 16 and no piece crosses the border between turning and passing
+  // channels (halves: between an axis' halves)
+  bool vec = p.d % V == 0 && 2 * p.pairs % V == 0 && ((uintptr_t)p.x | (uintptr_t)p.y) % 16 == 0 &&
+             p.xr % V == 0 && p.xh % V == 0 && p.yr % V == 0 && p.yh % V == 0;
+  if (!p.interleaved)
+    for (int i = 0; i < p.pairs && vec; i += V)
+      vec = p.pairs % V == 0 && p.c0[i] % V == 0 && p.c1[i] % V == 0 && p.c0[i + V - 1] == p.c0[i] + V - 1 && p.axis[i + V - 1] == p.axis[i];
+  const int mode = !vec ? 0 : p.interleaved ? 1 : 2;
+  const int rest = p.copy ? p.d - 2 * p.pairs : 0;
+  const int units = mode == 0 ? p.pairs + rest : mode == 1 ? (2 * p.pairs + rest) / V : (p.pairs + rest) / V;
+  const long long threads = p.rows * units, blocks = (threads + 255) / 256;
+  // few rows: the heads are split over the grid until there are about four workgroups per compute unit
+  int split = 1;
+  while (split < p.heads && blocks * split < 1024) split *= 2;
+  const int hchunk = (p.heads + split - 1) / split;
+  const dim3 grid((unsigned)blocks, (unsigned)((p.heads + hchunk - 1) / hchunk));
+  if (mode == 0) rotary_kernel<T, 0><<<grid, 256, 0, st>>>(p, units, hchunk);
+  else if (mode == 1) rotary_kernel<T, 1><<<grid, 256, 0, st>>>(p, units, hchunk);
+  else rotary_kernel<T, 2><<<grid, 256, 0, st>>>(p, units, hchunk);
+  return hipGetLastError() != hipSuccess;
+}
+
+}  // namespace
+
+int launch_rotary(const RotaryP& p, int dtype, hipStream_t st) {
+  return dtype == OP_F32 ? run<float>(p, st) : dtype == OP_BF16 ? run<__bf16>(p, st) : run<_Float16>(p, st);
+}

@@ -1,0 +1,54 @@
+// ops.h -- parameter blocks of the stand-alone operators (op_rotary.hip, op_attention.hip, op_ortho.hip); the C entry
+// points that check the caller's arguments and fill them are in op_api.hip.
+#pragma once
+#include "common.h"
+
+enum OpType { OP_F32 = 0, OP_BF16 = 1, OP_F16 = 2 };
+inline int op_bytes(int dtype) { return dtype == OP_F32 ? 4 : 2; }
+
+// ---- rotary positions ----------------------------------------------------------------------------
+struct RotaryP {
+  const void* x; void* y;
+  const int* pos;               // [pos_rows, n_axes]
+  long long rows, pos_rows;     // row r turns by pos[r % pos_rows]
+  long long xr, xh, yr, yh;     // strides of x and y in elements: row, head
+  int heads, d, n_axes, pairs;  // pairs: half the channels that turn
+  int interleaved, copy;        // copy: the channels past the last axis are copied (y is not x)
+  float sign;                   // +1 forward, -1 backward
+  double turn[64];              // pair -> turns per unit of position, theta^(-2 i / n) / (2 pi)
+  unsigned char axis[64], c0[64], c1[64];   // pair -> axis, its two channels
+};
+int launch_rotary(const RotaryP& p, int dtype, hipStream_t st);
+
+// ---- attention over packed sequences -------------------------------------------------------------
+struct AttnP {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float* lse;                   // [heads, rows]
+  float* delta;                 // backward workspace: [2, heads, rows] (rowsum(dout out), then log2 of the row's scale)
+  const int* cu;                // [nseq + 1] first rows, or null: nseq sequences of seqlen rows each
+  long long rows;
+  long long qr, qh, kr, kh, vr, vh, orow, oh, dor, doh, dqr, dqh, dkr, dkh, dvr, dvh;   // element strides
+  int nseq, seqlen, heads, kv_heads, d, block;   // block: causal block, 0 = bidirectional
+  float scale;
+};
+int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st);
+int launch_attention_bwd(const AttnP& p, int dtype, hipStream_t st);
+
+// ---- orthogonalisation of updates ----------------------------------------------------------------
+constexpr int ORTHO_GROUPS = 16, ORTHO_STEPS = 32, ORTHO_PARTS = 64;
+struct OrthoG {                 // a stack of equal matrices; m = min(rows, cols), n = max
+  const void* x; void* y;
+  long long xm, xr, ym, yr;     // strides in elements: matrix, row
+  int count, rows, cols, m, n, ldn, ldm, first;   // ldn, ldm: n, m rounded up to 64; first: matrices of the groups before
+  long long ws;                 // first 16-bit element of its matrices in the workspace
+};
+struct OrthoP {
+  OrthoG g[ORTHO_GROUPS];
+  int ngroups, matrices;
+  unsigned short* ws;           // planes of 16-bit halves (op_ortho.hip)
+  double* parts;                // [matrices, ORTHO_PARTS] partial sums of squares
+  float eps;
+};
+size_t ortho_ws_bytes(OrthoP& p);   // sets the groups' ws offsets
+int launch_ortho(const OrthoP& p, int dtype, int steps, const float* coef, hipStream_t st);

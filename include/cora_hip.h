@@ -239,6 +239,74 @@ size_t cora_forward_static_floats(const cora_config* cfg);
 int cora_forward_static(const cora_config* cfg, int device, const float* W_dev, size_t n_weights,
                         const float* pos_dev, const float* h0_dev, float* xhat_dev, void* hip_stream);
 
+/* --- stand-alone operators -------------------------------------------------------------------
+ * No ctx: device pointers in, kernel launches on `hip_stream` (a hipStream_t of `device`, NULL = the null stream), no
+ * allocation, no copy, no synchronisation, so they may be called under stream capture.  The caller's current device is
+ * left as it was.  Thread-safe; errors: cora_last_error(NULL).  Strides count elements; the innermost dimension is
+ * contiguous.  Inputs may have any strides >= 0 (0 repeats a row or head); rows and heads of an output must not overlap.
+ * No counterpart in the reference, whose blocks have additive positions and bidirectional attention
+ * (pcx/nn/_layer.py:405-447) and whose weights are stepped by AdamW. */
+enum { CORA_F32 = 0, CORA_BF16 = 1, CORA_F16 = 2 };
+
+/* Rotary positions over up to four axes (time, height, width, ..).  Axis a owns axes_dim[a] consecutive channels of every
+ * head; its pair i turns by the angle pos_a * theta^(-2 i / axes_dim[a]): (u, v) -> (u cos - v sin, u sin + v cos), with
+ * u, v neighbouring channels (interleaved) or axes_dim[a] / 2 apart.  Channels behind the last axis are copied.
+ * backward != 0 turns the other way: the gradient with respect to x of a gradient given for y.
+ * x [rows, heads, head_dim] -> y, which may be x itself (same strides).  Row r takes positions pos[r % pos_rows]. */
+typedef struct cora_rotary_args {
+  int32_t dtype, heads, head_dim, n_axes;
+  int32_t axes_dim[4];          /* positive, even, together at most head_dim and at most 128 */
+  int32_t interleaved, backward;
+  double  theta;
+  int64_t rows, pos_rows;
+  const int32_t* pos;           /* [pos_rows, n_axes] */
+  const void* x; void* y;
+  int64_t x_row, x_head, y_row, y_head;
+} cora_rotary_args;
+int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream);
+
+/* Attention over packed sequences.  q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim] (heads a multiple of
+ * kv_heads; query head h reads key head h / (heads / kv_heads)).  Sequence s owns rows cu_seqlens[s] .. cu_seqlens[s+1] - 1
+ * (int32, on the device, non-decreasing, at most rows; bounds outside are cut), or, with cu_seqlens NULL, n_seq sequences
+ * of seq_len rows each.  Sequences may be empty; rows of no sequence are neither read nor written.
+ * causal_block 0: a token sees its whole sequence; b >= 1: the tokens of its own and of earlier blocks of b tokens of the
+ * sequence (1: causal; tokens per frame: frame-causal).
+ *   out_i = sum_j softmax_j(scale q_i k_j) v_j,  lse [heads, rows] = log sum_j exp(scale q_i k_j)  (float32)
+ * head_dim: up to 128, a multiple of 8 (float32: 4); pointers 16-byte aligned, strides multiples of 16 bytes.  Sums and
+ * softmax statistics are float32; the probabilities are rounded to a 16-bit dtype before they meet v.
+ * Backward: dout and the forward's out and lse -> dq, dk, dv (sums over the query heads of a key head).  workspace:
+ * cora_attention_workspace(a) bytes, 16-byte aligned, not shared by calls that may overlap.  Results repeat bit for bit. */
+typedef struct cora_attention_args {
+  int32_t dtype, heads, kv_heads, head_dim, n_seq, seq_len, causal_block;
+  float   scale;                /* > 0 */
+  int64_t rows;                 /* < 2^31 */
+  const int32_t* cu_seqlens;    /* [n_seq + 1] */
+  const void *q, *k, *v;
+  void* out; float* lse;        /* written by the forward, read by the backward call */
+  const void* dout; void *dq, *dk, *dv;   /* backward call only */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  int64_t dout_row, dout_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  void* workspace; size_t workspace_bytes;   /* backward call only */
+} cora_attention_args;
+int cora_attention(const cora_attention_args* a, int device, void* hip_stream);
+int cora_attention_backward(const cora_attention_args* a, int device, void* hip_stream);
+size_t cora_attention_workspace(const cora_attention_args* a);
+
+/* Orthogonalise weight updates by Newton-Schulz products: X = G / (|G|_F + eps), then per step, with coefficients
+ * (a, b, c) of coef [steps, 3] (host), X <- a X + (b A + c A^2) X with A = X X^T (tall matrices: of the transpose).
+ * All stacks (each `count` equal matrices) are worked on together; y may be x (same strides).  Products are float32-grade
+ * (bfloat16: of an error below the result's rounding).  Refused: coefficients under which a singular value of [0, 1]
+ * leaves [0, 8] or |a + b s^2 + c s^4| exceeds 1000.
+ * workspace: cora_orthogonalize_workspace(..) bytes, 256-byte aligned, not shared by calls that may overlap. */
+typedef struct cora_matrices {
+  const void* x; void* y;
+  int64_t x_mat, x_row, y_mat, y_row;
+  int32_t count, rows, cols;    /* count <= 65535; rows, cols <= 32768 */
+} cora_matrices;
+size_t cora_orthogonalize_workspace(int dtype, const cora_matrices* stacks, int n_stacks);
+int cora_orthogonalize(int dtype, const cora_matrices* stacks, int n_stacks, int steps, const float* coef, float eps,
+                       void* workspace, size_t workspace_bytes, int device, void* hip_stream);
+
 /* `unmask_on_batch_enhanced` (/root/reference/src/decoder_transformer.py:833-1046): the inference-only /
  * inpainting loop.  x_true, x_init, mask: host [B,C,H,W] (mask already broadcast over channels,
  * 1 = masked; ignored unless use_corruption).  The sensory vode starts from x_init (:896-901); with
