@@ -35,18 +35,36 @@ __device__ __forceinline__ half* plane_a(const OrthoP& p, const OrthoG& g, int m
 
 __device__ __forceinline__ void split2(float v, half& hi, half& lo) { hi = (half)v; lo = (half)(v - (float)hi); }
 
-// partial sums of squares in 64 bits: part z of a matrix takes every ORTHO_PARTS-th row
+// partial sums of squares in 64 bits: part z of a matrix takes every ORTHO_PARTS-th strip of 2048 elements of its rows
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_sumsq(const OrthoP p) {
+  constexpr int V = 16 / (int)sizeof(T);
   __shared__ double sh[4];
   const int id = blockIdx.x, part = blockIdx.y;
   int gi = 0;
   while (gi + 1 < p.ngroups && id >= p.g[gi + 1].first) ++gi;
   const OrthoG& g = p.g[gi];
   const T* x = (const T*)g.x + (long long)(id - g.first) * g.xm;
+  const bool vec = (uintptr_t)x % 16 == 0 && g.xr % V == 0;
+  const int strips = (g.cols + 2047) / 2048;
   double s = 0.0;
-  for (int r = part; r < g.rows; r += ORTHO_PARTS)
-    for (int c = threadIdx.x; c < g.cols; c += 256) { const double v = (double)(float)x[(long long)r * g.xr + c]; s += v * v; }
+  for (long long t = part; t < (long long)g.rows * strips; t += ORTHO_PARTS) {
+    const long long r = t / strips;
+    const int c0 = (int)(t - r * strips) * 2048, c1 = min(g.cols, c0 + 2048);
+    const T* row = x + r * g.xr;
+    if (vec) {
+      for (int c = c0 + (int)threadIdx.x * V; c < c1; c += 256 * V) {
+        typedef T vecT __attribute__((ext_vector_type(V)));
+        if (c + V <= c1) {
+          const vecT v = *reinterpret_cast<const vecT*>(row + c);
+#pragma unroll
+          for (int i = 0; i < V; ++i) s += (double)(float)v[i] * (double)(float)v[i];
+        } else
+          for (int i = c; i < c1; ++i) s += (double)(float)row[i] * (double)(float)row[i];
+      }
+    } else
+      for (int c = c0 + (int)threadIdx.x; c < c1; c += 256) s += (double)(float)row[c] * (double)(float)row[c];
+  }
   s = block_sum_256(s, sh);
   if (threadIdx.x == 0) p.parts[(long long)id * ORTHO_PARTS + part] = s;
 }
@@ -62,12 +80,13 @@ __global__ __launch_bounds__(256) void ortho_load(const OrthoP p) {
   const int mat = id - g.first, tn = g.ldn / 64, tm = g.ldm / 64;
   if ((int)blockIdx.x >= tn * tm) return;
   const int i0 = blockIdx.x / tn * 64, j0 = blockIdx.x % tn * 64;
-  double s = 0.0;
-  for (int k = 0; k < ORTHO_PARTS; ++k) s += p.parts[(long long)id * ORTHO_PARTS + k];
+  static_assert(ORTHO_PARTS == 64, "one part per lane");
+  const double s = wave_sum_d(p.parts[(long long)id * ORTHO_PARTS + (threadIdx.x & 63)]);
   const double f = (double)SX / (sqrt(s) + (double)p.eps);
   const bool tall = g.rows > g.cols;
   const T* x = (const T*)g.x + (long long)mat * g.xm;
   const int a = threadIdx.x & 63, b = threadIdx.x >> 6;
+#pragma unroll 4
   for (int k = b; k < 64; k += 4) {                       // source rows along b
     const int r = (tall ? j0 : i0) + k, c = (tall ? i0 : j0) + a;
     const float v = r < g.rows && c < g.cols ? (float)((double)(float)x[(long long)r * g.xr + c] * f) : 0.f;
@@ -75,25 +94,210 @@ __global__ __launch_bounds__(256) void ortho_load(const OrthoP p) {
   }
   __syncthreads();
   half* hi = plane_x(p, g, mat, 0); half* lo = plane_x(p, g, mat, 1);
-  for (int k = b; k < 64; k += 4)
+#pragma unroll
+  for (int k = threadIdx.x >> 4; k < 64; k += 16)
     if (i0 + k < g.m) {
-      half vh, vl;
-      split2(t[k][a], vh, vl);
-      const long long o = (long long)(i0 + k) * g.ldn + j0 + a;
-      hi[o] = vh; lo[o] = vl;
+      h16x4 vh, vl;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { half u, v; split2(t[k][4 * (threadIdx.x & 15) + e], u, v); vh[e] = u; vl[e] = v; }
+      const long long o = (long long)(i0 + k) * g.ldn + j0 + 4 * (threadIdx.x & 15);
+      *reinterpret_cast<h16x4*>(hi + o) = vh;
+      *reinterpret_cast<h16x4*>(lo + o) = vl;
     }
+}
+
+// ---- matrices that fit one compute unit's LDS ----------------------------------------------------
+// All steps of one matrix in one workgroup of 16 waves: X, then A and P in A's place, as two fp16 planes each in LDS; 16 x 16
+// tiles (v_mfma_f32_16x16x32_f16), three instructions a product for every type.  A wave keeps whole columns of X, so
+// X <- P X happens in place.  Bound by the chain of 3 products and 4 barriers a step, about 1.5 us; against the tiled path
+// this saves its 2 + 3 * steps launches.
+// Rows are padded to a stride of 80 bytes mod 256 (the 16 rows of a row read start 16 bytes apart mod 256, the 4 rows of a
+// transposing read 80 apart) or, where that does not fit, to 16 mod 256.
+constexpr int SMALL_LDS = 160 * 1024 - 256;
+struct SmallDim { int mp, np, sx, sa, bytes; };           // padded sizes, row strides in halves, LDS bytes
+__host__ __device__ inline SmallDim small_dim(int m, int n) {
+  SmallDim d;
+  d.mp = (m + 31) / 32 * 32; d.np = (n + 31) / 32 * 32;
+  for (int want = 80; want >= 16; want -= 64) {
+    d.sx = d.np + ((want - 2 * d.np) & 255) / 2; d.sa = d.mp + ((want - 2 * d.mp) & 255) / 2;
+    d.bytes = 4 * d.mp * (d.sx + d.sa);
+    if (d.bytes <= SMALL_LDS) break;
+  }
+  return d;
+}
+
+// the steps, for matrices of MT row tiles
+template <typename T, int MT>
+__device__ __forceinline__ void small_steps(half* lds, const OrthoG& g, const SmallDim d, T* y, const OrthoCoef& co) {
+  constexpr int MP = 16 * MT, NZ = (MT * MT + 15) / 16;    // tiles of A per wave
+  const int m = g.m, n = g.n, np = d.np, sx = d.sx, sa = d.sa;
+  const long long yr = g.yr;
+  const bool tall = g.rows > g.cols;
+  half *xh = lds, *xl = xh + MP * sx, *ah = xl + MP * sx, *al = ah + MP * sa;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g16 = lane >> 4;
+  // 16 x 32 operand pieces: lane holds index l & 15, contraction 8 (l >> 4) + 0 .. 7
+  auto row = [&](const half* t, int stride, int i0, int k0) {
+    return *reinterpret_cast<const h16x8*>(t + (i0 + r16) * stride + k0 + 8 * g16);
+  };
+  auto col = [&](const half* t, int stride, int k0, int j0) {
+    const half* q = t + (k0 + 8 * g16 + (r16 >> 2)) * stride + j0 + 4 * (r16 & 3);
+    s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS3 s16x4*)q);
+    s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS3 s16x4*)(q + 4 * stride));
+    s16x8 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    return __builtin_bit_cast(h16x8, v);
+  };
+  auto mma = [](h16x8 a, h16x8 b, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0); };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // four neighbouring columns of a lane's row, split
+  auto put = [&](half* hi, half* lo, int o, f32x4 v) {
+    h16x4 vh, vl;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { half a, b; split2(v[e], a, b); vh[e] = a; vl[e] = b; }
+    *reinterpret_cast<h16x4*>(hi + o) = vh;
+    *reinterpret_cast<h16x4*>(lo + o) = vl;
+  };
+  for (int step = 0; step < co.steps; ++step) {
+    const float ca = co.c[3 * step], cb = co.c[3 * step + 1], cc = co.c[3 * step + 2];
+    f32x4 pt[NZ];
+    __syncthreads();
+#pragma unroll
+    for (int z = 0; z < NZ; ++z) {                         // A = X X^T
+      const int t = w + 16 * z;
+      if (MT * MT % 16 && t >= MT * MT) continue;
+      const int i = 16 * (t / MT), j = 16 * (t % MT);
+      f32x4 hh = zero, hl = zero, lh = zero;
+      for (int k = 0; k < np; k += 32) {
+        const h16x8 a0 = row(xh, sx, j, k), a1 = row(xl, sx, j, k), b0 = row(xh, sx, i, k), b1 = row(xl, sx, i, k);
+        hh = mma(a0, b0, hh); hl = mma(a0, b1, hl); lh = mma(a1, b0, lh);
+      }
+      put(ah, al, (i + r16) * sa + j + 4 * g16, (hh + (hl + lh)) * (SA / (SX * SX)));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int z = 0; z < NZ; ++z) {                         // P = a I + b A + c A A
+      const int t = w + 16 * z;
+      if (MT * MT % 16 && t >= MT * MT) continue;
+      const int i = 16 * (t / MT), j = 16 * (t % MT), r = i + r16, c = j + 4 * g16;
+      f32x4 hh = zero, hl = zero, lh = zero;
+#pragma unroll
+      for (int k = 0; k < MP; k += 32) {
+        const h16x8 a0 = row(ah, sa, j, k), a1 = row(al, sa, j, k), b0 = row(ah, sa, i, k), b1 = row(al, sa, i, k);
+        hh = mma(a0, b0, hh); hl = mma(a0, b1, hl); lh = mma(a1, b0, lh);
+      }
+      const h16x4 vh = *reinterpret_cast<const h16x4*>(ah + r * sa + c), vl = *reinterpret_cast<const h16x4*>(al + r * sa + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        pt[z][e] = __builtin_fmaf(cc / SA, hh[e] + (hl[e] + lh[e]), cb * ((float)vh[e] + (float)vl[e])) + (r == c + e ? ca * SA : 0.f);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int z = 0; z < NZ; ++z) {
+      const int t = w + 16 * z;
+      if (MT * MT % 16 && t >= MT * MT) continue;
+      put(ah, al, (16 * (t / MT) + r16) * sa + 16 * (t % MT) + 4 * g16, pt[z]);
+    }
+    __syncthreads();
+    for (int j = 16 * w; j < np; j += 256) {               // X <- P X, 16 columns at a time
+      f32x4 hh[MT], lo[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) { hh[i] = zero; lo[i] = zero; }
+#pragma unroll
+      for (int k = 0; k < MP; k += 32) {
+        const h16x8 a0 = col(xh, sx, k, j), a1 = col(xl, sx, k, j);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const h16x8 b0 = row(ah, sa, 16 * i, k), b1 = row(al, sa, 16 * i, k);
+          hh[i] = mma(a0, b0, hh[i]); lo[i] = mma(a1, b0, lo[i]); lo[i] = mma(a0, b1, lo[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int r = 16 * i + r16, c = j + 4 * g16;
+        const f32x4 v = hh[i] + lo[i];
+        if (step == co.steps - 1) {
+          if (r < m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < n) y[tall ? (c + e) * yr + r : r * yr + c + e] = (T)(v[e] * (1.f / (SA * SX)));
+        } else put(xh, xl, r * sx + c, v * (1.f / SA));
+      }
+    }
+  }
+}
+
+template <typename T, int MT>
+__global__ __launch_bounds__(1024) void ortho_small(const OrthoP p, const OrthoCoef co) {
+  extern __shared__ __attribute__((aligned(16))) half lds[];
+  __shared__ double red[16];
+  const int id = blockIdx.x;
+  int gi = 0;
+  while (gi + 1 < p.ngroups && id >= p.g[gi + 1].first) ++gi;
+  const OrthoG& g = p.g[gi];
+  const SmallDim d = small_dim(g.m, g.n);
+  const int rows = g.rows, cols = g.cols, sx = d.sx, tid = threadIdx.x;
+  const bool tall = rows > cols;
+  const T* x = (const T*)g.x + (long long)(id - g.first) * g.xm;
+  const long long xr = g.xr;
+  unsigned short *xh = (unsigned short*)lds, *xl = xh + d.mp * sx;
+
+  // The matrix goes to its place with its bits halved between the planes and is scaled and split there once its norm is
+  // known.  Loops are kept short: a workgroup lives for some 10 us and fetches its code cold.
+  for (int i = tid; i < d.mp * sx / 4; i += 1024) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0u, 0u, 0u, 0u);   // both planes
+  __syncthreads();
+  double s = 0.0;
+  const int dr = 1024 / cols, dc = 1024 - dr * cols;       // element tid + 1024 i: its row and column step by these
+  int r = tid / cols, c = tid - r * cols;
+  while (r < rows) {
+    float v[8]; int o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = r < rows ? (float)x[r * xr + c] : 0.f;
+      o[i] = r < rows ? (tall ? c * sx + r : r * sx + c) : -1;
+      r += dr; c += dc;
+      if (c >= cols) { c -= cols; ++r; }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s += (double)v[i] * (double)v[i];
+      if (o[i] >= 0) { const unsigned u = __float_as_uint(v[i]); xh[o[i]] = (unsigned short)(u >> 16); xl[o[i]] = (unsigned short)u; }
+    }
+  }
+  s = wave_sum_d(s);
+  if ((tid & 63) == 0) red[tid >> 6] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += red[i];
+  const double f = (double)SX / (sqrt(s) + (double)p.eps);
+  for (int i = tid; i < d.mp * sx / 4; i += 1024) {
+    const ushort4 uh = reinterpret_cast<ushort4*>(xh)[i], ul = reinterpret_cast<ushort4*>(xl)[i];
+    const unsigned u[4] = {(unsigned)uh.x << 16 | ul.x, (unsigned)uh.y << 16 | ul.y, (unsigned)uh.z << 16 | ul.z, (unsigned)uh.w << 16 | ul.w};
+    h16x4 vh, vl;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { half a, b; split2((float)((double)__uint_as_float(u[e]) * f), a, b); vh[e] = a; vl[e] = b; }
+    reinterpret_cast<h16x4*>(xh)[i] = vh; reinterpret_cast<h16x4*>(xl)[i] = vl;
+  }
+  T* y = (T*)g.y + (long long)(id - g.first) * g.ym;
+  small_steps<T, MT>(lds, g, d, y, co);
 }
 
 // One product for all matrices.  STEP 0: A = X X^T; 1: P = a I + b A + c A A; 2: X' = P X (last: to the caller's matrix).
 // Tile 128 x 128, four waves of 64 x 64, slabs of 32: the first operand gives the output's columns, the second its rows
-// (op_tile.h), so a lane holds four neighbouring columns of one output row.
+// (op_tile.h), so a lane holds four neighbouring columns of one output row.  Slabs go from global memory straight into one
+// of two LDS buffers while the other is worked on; a lane fetches the 16-byte piece that belongs at its place of the
+// swizzled tile.  Rows and columns outside a matrix are read from its last one; what they give is not stored, and along
+// the contraction they meet zeros (columns up to ldn and ldm are stored as zeros).
 template <typename T, int STEP, bool FULL>
 __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const int cur, const int last, const float ca, const float cb, const float cc) {
   constexpr int TK = 32;
+  constexpr bool BLO = FULL || STEP == 1, ALO = FULL || STEP != 0;
+  constexpr int NPL = 2 + BLO + ALO, PB1 = 1, PA0 = BLO ? 2 : 1, PA1 = PA0 + 1;   // planes: B hi, (B lo,) A hi, (A lo)
   typedef Tile<half, TK> LR; typedef Tile<half, 128> LC;
   typedef Op<half> O;
-  __shared__ __attribute__((aligned(16))) half Bs[2][128 * TK];   // rows of the output (second operand): hi, lo
-  __shared__ __attribute__((aligned(16))) half As[2][128 * TK];   // columns of the output (first operand)
+  __shared__ __attribute__((aligned(16))) half buf0[NPL][128 * TK];
+  __shared__ __attribute__((aligned(16))) half buf1[NPL][128 * TK];
   int gi = 0, id = blockIdx.x, per = 0;
   for (;; ++gi) {                                          // group of this tile
     if (gi == p.ngroups) return;
@@ -103,60 +307,57 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
     id -= per * p.g[gi].count;
   }
   const OrthoG& g = p.g[gi];
+  const int m = g.m, ldn = g.ldn, ldm = g.ldm;
   const int mat = id / per, tl = id % per;
   int ti, tj;
-  if (STEP == 2) { const int tm = (g.m + 127) / 128; ti = tl % tm; tj = tl / tm; }
+  if (STEP == 2) { const int tm = (m + 127) / 128; ti = tl % tm; tj = tl / tm; }
   else {
     ti = (int)((sqrtf(8.f * tl + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > tl) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= tl) ++ti;
     tj = tl - ti * (ti + 1) / 2;
   }
-  const int ld = STEP == 0 ? g.ldn : g.ldm;                // contraction length
+  const int ld = STEP == 0 ? ldn : ldm;                    // contraction length
   const half* bh = STEP == 0 ? plane_x(p, g, mat, cur) : plane_a(p, g, mat, STEP == 1 ? 0 : 2);
   const half* bl = STEP == 0 ? plane_x(p, g, mat, cur + 1) : plane_a(p, g, mat, STEP == 1 ? 1 : 3);
   const half* ah = STEP == 2 ? plane_x(p, g, mat, cur) : bh;
   const half* al = STEP == 2 ? plane_x(p, g, mat, cur + 1) : bl;
-  constexpr bool BLO = FULL || STEP == 1, ALO = FULL || STEP != 0;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int r0 = ti * 128, c0 = tj * 128;
 
-  uint4 vb[2][2], va[2][2];
-  auto load = [&](int k0) {
+  // wave w fills chunks w and w + 4 (64 pieces each) of every plane
+  const half* src[NPL][2];
+#pragma unroll
+  for (int pl = 0; pl < NPL; ++pl)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int q = i * 256 + (int)threadIdx.x;
-      const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-      { const int r = r0 + q / 4, c = k0 + 8 * (q & 3);
-        const long long o = (long long)r * ld + c;
-        vb[0][i] = r < g.m ? *reinterpret_cast<const uint4*>(bh + o) : z;
-        if (BLO) vb[1][i] = r < g.m ? *reinterpret_cast<const uint4*>(bl + o) : z; }
-      if (STEP != 2) {
-        const int r = c0 + q / 4, c = k0 + 8 * (q & 3);
-        const long long o = (long long)r * ld + c;
-        va[0][i] = r < g.m ? *reinterpret_cast<const uint4*>(ah + o) : z;
-        if (ALO) va[1][i] = r < g.m ? *reinterpret_cast<const uint4*>(al + o) : z;
+      const int q = (4 * i + w) * 64 + lane;
+      const bool a = pl >= PA0;
+      const half* base = pl == 0 ? bh : (BLO && pl == PB1) ? bl : pl == PA0 ? ah : al;
+      if (STEP == 2 && a) {
+        const int r = q / 16, c = min(c0 + 8 * ((q & 15) ^ LC::swz(r)), ldn - 8);
+        src[pl][i] = base + (long long)r * ldn + c;       // r < 32: rows behind m are met at the last slab only (below)
       } else {
-        const int r = k0 + q / 16, c = c0 + 8 * (q & 15);
-        const long long o = (long long)r * g.ldn + c;
-        const bool ok = r < g.m && c < g.ldn;
-        va[0][i] = ok ? *reinterpret_cast<const uint4*>(ah + o) : z;
-        if (ALO) va[1][i] = ok ? *reinterpret_cast<const uint4*>(al + o) : z;
+        const int r = q / 4, c = (q & 3) ^ LR::swz(r);
+        src[pl][i] = base + (long long)min((a ? c0 : r0) + r, m - 1) * ld + 8 * c;
       }
     }
-  };
-  auto store = [&]() {
+  auto fetch = [&](half (&dst)[NPL][128 * TK], int k0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = i * 256 + (int)threadIdx.x;
-      *reinterpret_cast<uint4*>(Bs[0] + LR::at(q / 4, q & 3)) = vb[0][i];
-      if (BLO) *reinterpret_cast<uint4*>(Bs[1] + LR::at(q / 4, q & 3)) = vb[1][i];
-      const int o = STEP != 2 ? LR::at(q / 4, q & 3) : LC::at(q / 16, q & 15);
-      *reinterpret_cast<uint4*>(As[0] + o) = va[0][i];
-      if (ALO) *reinterpret_cast<uint4*>(As[1] + o) = va[1][i];
-    }
+    for (int pl = 0; pl < NPL; ++pl)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const half* s;
+        if (STEP == 2 && pl >= PA0) {
+          const int r = ((4 * i + w) * 64 + lane) / 16;
+          s = src[pl][i] + (long long)(min(k0 + r, m - 1) - r) * ldn;
+        } else s = src[pl][i] + k0;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s,
+                                         (LDS3 void*)(dst[pl] + (4 * i + w) * 512), 16, 0, 0);
+      }
+    __builtin_amdgcn_sched_barrier(0);                     // the requests leave before the work on the other buffer starts
   };
-  // second operand in contraction order 16 s + 8 h + 0 .. 7, as row_frag gives it
+  // first operand from a tile of contraction rows x columns, in contraction order 16 s + 8 h + 0 .. 7 as row_frag gives it
   auto col = [&](const half* t, int s, int ct) {
     const int i = lane & 15, row = 16 * s + 8 * h + (i >> 2), ch = ct + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
     s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS3 s16x4*)(t + LC::at(row, ch / 8) + (ch & 7)));
@@ -174,21 +375,16 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  load(0);
-  for (int k0 = 0; k0 < ld; k0 += TK) {
-    __syncthreads();
-    store();
-    __syncthreads();
-    if (k0 + TK < ld) load(k0 + TK);
+  auto work = [&](half (&t)[NPL][128 * TK]) {
 #pragma unroll
     for (int s = 0; s < TK / 16; ++s) {
       h16x8 b0[2], b1[2], a0[2], a1[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        b0[i] = LR::row_frag(Bs[0], wr + 32 * i, s, lane);
-        if (BLO) b1[i] = LR::row_frag(Bs[1], wr + 32 * i, s, lane);
-        a0[i] = STEP != 2 ? LR::row_frag(As[0], wc + 32 * i, s, lane) : col(As[0], s, wc + 32 * i);
-        if (ALO) a1[i] = STEP != 2 ? LR::row_frag(As[1], wc + 32 * i, s, lane) : col(As[1], s, wc + 32 * i);
+        b0[i] = LR::row_frag(t[0], wr + 32 * i, s, lane);
+        if (BLO) b1[i] = LR::row_frag(t[PB1], wr + 32 * i, s, lane);
+        a0[i] = STEP != 2 ? LR::row_frag(t[PA0], wc + 32 * i, s, lane) : col(t[PA0], s, wc + 32 * i);
+        if (ALO) a1[i] = STEP != 2 ? LR::row_frag(t[PA1 < NPL ? PA1 : 0], wc + 32 * i, s, lane) : col(t[PA1 < NPL ? PA1 : 0], s, wc + 32 * i);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -199,13 +395,22 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
           if (BLO) acc[i][j] = O::mma(a0[j], b1[i], acc[i][j]);
         }
     }
+  };
+  fetch(buf0, 0);
+  for (int k0 = 0; k0 < ld; k0 += 2 * TK) {                // ld is a multiple of 64
+    __syncthreads();                                       // buf0 has arrived, buf1 is no longer read
+    fetch(buf1, k0 + TK);
+    work(buf0);
+    __syncthreads();
+    if (k0 + 2 * TK < ld) fetch(buf0, k0 + 2 * TK);
+    work(buf1);
   }
   const bool mirror = STEP != 2 && ti != tj;
   half *oh, *ol;
   if (STEP == 0) { oh = plane_a(p, g, mat, 0); ol = plane_a(p, g, mat, 1); }
   else if (STEP == 1) { oh = plane_a(p, g, mat, 2); ol = plane_a(p, g, mat, 3); }
   else { oh = plane_x(p, g, mat, 2 - cur); ol = plane_x(p, g, mat, 3 - cur); }
-  const int lo_out = STEP == 2 ? g.ldn : g.ldm;
+  const int lo_out = STEP == 2 ? ldn : ldm;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -213,18 +418,18 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int r = r0 + wr + 32 * i + (lane & 31), c = c0 + wc + 32 * j + 8 * q + 4 * h;
-        // rows behind the matrix are zero: their mirror images fill the columns up to ldm
-        if (r >= (STEP == 2 ? g.m : g.ldm) || c >= lo_out) continue;
-        const bool in = r < g.m;
+        // A and P: rows behind the matrix are zero, their mirror images fill the columns up to ldm
+        if (r >= (STEP == 2 ? m : ldm) || c >= lo_out) continue;
+        const bool in = r < m;
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+        for (int e = 0; e < 4; ++e) v[e] = in && (STEP == 2 || c + e < m) ? acc[i][j][4 * q + e] : 0.f;
         if (STEP == 0) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= SA / (SX * SX);
         } else if (STEP == 1 && in) {
-          const h16x4 xh = *reinterpret_cast<const h16x4*>(bh + (long long)r * g.ldm + c);
-          const h16x4 xl = *reinterpret_cast<const h16x4*>(bl + (long long)r * g.ldm + c);
+          const h16x4 xh = *reinterpret_cast<const h16x4*>(bh + (long long)r * ldm + c);
+          const h16x4 xl = *reinterpret_cast<const h16x4*>(bl + (long long)r * ldm + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             v[e] = __builtin_fmaf(cc / SA, v[e], cb * ((float)xh[e] + (float)xl[e])) + (FULL && r == c + e ? ca * SA : 0.f);
@@ -232,8 +437,8 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= 1.f / SA;
           if (!FULL) {
-            const h16x4 xh = *reinterpret_cast<const h16x4*>(ah + (long long)r * g.ldn + c);
-            const h16x4 xl = *reinterpret_cast<const h16x4*>(al + (long long)r * g.ldn + c);
+            const h16x4 xh = *reinterpret_cast<const h16x4*>(ah + (long long)r * ldn + c);
+            const h16x4 xl = *reinterpret_cast<const h16x4*>(al + (long long)r * ldn + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ca, (float)xh[e] + (float)xl[e], v[e]);
           }
@@ -256,12 +461,12 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
         if (mirror) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c + e < g.m) { oh[(long long)(c + e) * lo_out + r] = vh[e]; ol[(long long)(c + e) * lo_out + r] = vl[e]; }
+            if (c + e < m) { oh[(long long)(c + e) * lo_out + r] = vh[e]; ol[(long long)(c + e) * lo_out + r] = vl[e]; }
         }
       }
 }
 
-template <typename T, bool FULL> int run(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
+template <typename T, bool FULL> int run_tiled(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
   int load_tiles = 0;
   long long sym = 0, full = 0;
   for (int i = 0; i < p.ngroups; ++i) {
@@ -283,13 +488,52 @@ template <typename T, bool FULL> int run(const OrthoP& p, int steps, const float
   return hipGetLastError() != hipSuccess;
 }
 
+template <typename T, int MT> int run_small(const OrthoP& p, const OrthoCoef& co, hipStream_t st) {
+  static bool seen[64];
+  if (first_use_on_device(seen) &&
+      hipFuncSetAttribute((const void*)ortho_small<T, MT>, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS) != hipSuccess) return 1;
+  int bytes = 0;
+  for (int i = 0; i < p.ngroups; ++i) { const int b = small_dim(p.g[i].m, p.g[i].n).bytes; if (b > bytes) bytes = b; }
+  ortho_small<T, MT><<<dim3(p.matrices), 1024, bytes, st>>>(p, co);
+  return hipGetLastError() != hipSuccess;
+}
+
+// the stacks of p in one class: small with mt row tiles, or (0) too large for one workgroup
+OrthoP only(const OrthoP& p, int mt) {
+  OrthoP q = p;
+  q.ngroups = 0; q.matrices = 0;
+  for (int i = 0; i < p.ngroups; ++i)
+    if ((ortho_is_small(p.g[i]) ? (p.g[i].m + 31) / 32 * 2 : 0) == mt) {
+      q.g[q.ngroups] = p.g[i];
+      q.g[q.ngroups++].first = q.matrices;
+      q.matrices += p.g[i].count;
+    }
+  return q;
+}
+
+template <typename T, bool FULL> int run(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
+  OrthoCoef co;
+  co.steps = steps;
+  for (int i = 0; i < 3 * steps; ++i) co.c[i] = coef[i];
+  for (int mt = 0; mt <= 8; mt += 2) {
+    const OrthoP q = only(p, mt);
+    if (!q.ngroups) continue;
+    const int rc = mt == 0 ? run_tiled<T, FULL>(q, steps, coef, st) : mt == 2 ? run_small<T, 2>(q, co, st) :
+                   mt == 4 ? run_small<T, 4>(q, co, st) : mt == 6 ? run_small<T, 6>(q, co, st) : run_small<T, 8>(q, co, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
 }  // namespace
+
+bool ortho_is_small(const OrthoG& g) { return g.m <= 128 && small_dim(g.m, g.n).bytes <= SMALL_LDS; }
 
 size_t ortho_ws_bytes(OrthoP& p) {
   long long at = 0;
   for (int i = 0; i < p.ngroups; ++i) {
     p.g[i].ws = at;
-    at += (long long)p.g[i].count * (4LL * p.g[i].m * p.g[i].ldn + 4LL * p.g[i].m * p.g[i].ldm);
+    if (!ortho_is_small(p.g[i])) at += (long long)p.g[i].count * (4LL * p.g[i].m * p.g[i].ldn + 4LL * p.g[i].m * p.g[i].ldm);
   }
   return (size_t)at * 2 + (size_t)p.matrices * ORTHO_PARTS * sizeof(double) + 256;
 }

@@ -50,5 +50,7 @@ struct OrthoP {
   double* parts;                // [matrices, ORTHO_PARTS] partial sums of squares
   float eps;
 };
+struct OrthoCoef { int steps; float c[3 * ORTHO_STEPS]; };
+bool ortho_is_small(const OrthoG& g);   // worked on by one workgroup, in LDS
 size_t ortho_ws_bytes(OrthoP& p);   // sets the groups' ws offsets
 int launch_ortho(const OrthoP& p, int dtype, int steps, const float* coef, hipStream_t st);
