@@ -70,6 +70,7 @@ int check_attention(const cora_attention_args* a, AttnP* p, const char* who, boo
     if (!r.ptr) return refuse("%s: %s is NULL", who, r.name);
     if ((uintptr_t)r.ptr % 16 || r.row % v || r.head % v || r.row < 0 || r.head < 0)
       return refuse("%s: %s must be 16-byte aligned with non-negative strides that are multiples of 16 bytes", who, r.name);
+    if (r.row >= (1LL << 24)) return refuse("%s: the row stride of %s must be below 2^24 elements", who, r.name);
     if (r.out && !disjoint(a->rows, r.heads, a->head_dim, r.row, r.head)) return refuse("%s: rows or heads of %s overlap", who, r.name);
   }
   if (!a->lse || (uintptr_t)a->lse % 4 || (a->cu_seqlens && (uintptr_t)a->cu_seqlens % 4))
@@ -177,7 +178,7 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream) {
 
 size_t cora_attention_workspace(const cora_attention_args* a) {
   if (!a || a->heads < 1 || a->rows < 1) return 16;
-  return (size_t)a->heads * (size_t)a->rows * 2 * sizeof(float);
+  return (size_t)a->heads * (size_t)a->rows * 3 * sizeof(float);
 }
 
 int cora_attention(const cora_attention_args* a, int device, void* hip_stream) {

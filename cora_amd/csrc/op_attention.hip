@@ -23,27 +23,34 @@
 
 namespace {
 
-// Staging of R rows x D channels through registers: load() issues the global reads of the next tile, store() puts them
-// into LDS after the current one has been used.  Rows >= nvalid and channels >= d are zero.
-template <typename T, int D, int R, int NT>
-struct Stage {
-  static constexpr int NP = D / Op<T>::E, N = R * NP, NI = (N + NT - 1) / NT;
-  uint4 v[NI];
-  __device__ __forceinline__ void load(const T* base, long long stride, int nvalid, int d) {
+// Direct requests of 16 or 4 bytes a lane: the lane's bytes at base + at go to lds + 16 (4) * lane, zeros where at is behind
+// `bytes`.  (The host pass has no buffer descriptor type and silently drops kernels that name one.)
+#ifdef __HIP_DEVICE_COMPILE__
+#define REQUEST(base, bytes, lds, n, at) \
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)(base), 0, bytes, 0x00020000), (LDS3 void*)(lds), n, at, 0, 0, 0)
+#else
+#define REQUEST(base, bytes, lds, n, at) (void)0
+#endif
+
+// Staging of R rows x D channels straight from global memory into an LDS tile by NW waves.  A wave's request fills 64
+// consecutive 16-byte places; each lane asks for the piece that belongs there (Tile::swz).  The buffer descriptor ends
+// with the last valid row, and the pieces of channels >= d ask for an address past any end: both arrive as zeros.
+template <typename T, int D, int R, int NW>
+struct Fetch {
+  static constexpr int NP = D / Op<T>::E, NI = R * NP / 64 / NW;
+  static_assert(R * NP % (64 * NW) == 0, "whole requests");
+  int at[NI], stride, width;
+  __device__ __forceinline__ Fetch(long long row_stride, int d, int w, int lane) : stride((int)row_stride * (int)sizeof(T)), width(d * (int)sizeof(T)) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int id = i * NT + (int)threadIdx.x, r = id / NP, c = id % NP;
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if ((N % NT == 0 || id < N) && r < nvalid && c * Op<T>::E < d)
-        v[i] = *reinterpret_cast<const uint4*>(base + r * stride + c * Op<T>::E);
+      const int id = (i * NW + w) * 64 + lane, r = id / NP, c = (id % NP) ^ Tile<T, D>::swz(r);
+      at[i] = c * 16 < width ? r * stride + c * 16 : (int)0x80000000;
     }
   }
-  __device__ __forceinline__ void store(T* lds) const {
+  __device__ __forceinline__ void operator()(const T* rows, int nvalid, T* lds, int w) const {
+    [[maybe_unused]] const int bytes = nvalid > 0 ? (min(nvalid, R) - 1) * stride + width : 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int id = i * NT + (int)threadIdx.x, r = id / NP, c = id % NP;
-      if (N % NT == 0 || id < N) *reinterpret_cast<uint4*>(lds + Tile<T, D>::at(r, c)) = v[i];
-    }
+    for (int i = 0; i < NI; ++i) REQUEST(rows, bytes, lds + (i * NW + w) * 64 * Op<T>::E, 16, at[i]);
   }
 };
 
@@ -96,28 +103,54 @@ template <typename T, int D> __device__ __forceinline__ void store_own(T* row, c
 // query heads of one key head next to each other in the block order (they read the same keys and values)
 __device__ __forceinline__ int head_of(int i, int heads, int kv) { return (i % kv) * (heads / kv) + i / kv; }
 
+// the keys a sequence's token i sees end here
+__device__ __forceinline__ int limit(int i, int n, int block) {
+  return block ? (int)min((long long)n, ((long long)(i / block) + 1) * block) : n;
+}
+
+// The tiles a workgroup walks pass through two LDS buffers, each an object of its own so that the compiler sees that the
+// requests for one do not touch what is read from the other.  Between two barriers the next tile is under way while the
+// current one is worked on.
+#define WALK(COUNT, FETCH, WORK)                                                   \
+  FETCH(0, 0);                                                                     \
+  for (int it_ = 0; it_ < (COUNT); it_ += 2) {                                     \
+    arrive_barrier();                                                              \
+    if (it_ + 1 < (COUNT)) FETCH(it_ + 1, 1);                                      \
+    __builtin_amdgcn_sched_barrier(0);                                             \
+    WORK(it_, 0);                                                                  \
+    if (it_ + 1 >= (COUNT)) break;                                                 \
+    arrive_barrier();                                                              \
+    if (it_ + 2 < (COUNT)) FETCH(it_ + 2, 0);                                      \
+    __builtin_amdgcn_sched_barrier(0);                                             \
+    WORK(it_ + 1, 1);                                                              \
+  }
+
 // ---- forward -------------------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attn_fwd(const AttnP p) {
+// NW waves of 32 queries each.  The running maximum m only has to keep exp2 in range, so it is raised (and the sums
+// scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_fwd(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 128, NC = D / O::CH, NS = KT / O::CH;
-  __shared__ __attribute__((aligned(16))) T Ks[2][KT * D];
-  __shared__ __attribute__((aligned(16))) T Vs[2][KT * D];
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 32 * NW, NC = D / O::CH, NS = KT / O::CH;
+  __shared__ __attribute__((aligned(16))) T ks0[KT * D];
+  __shared__ __attribute__((aligned(16))) T vs0[KT * D];
+  __shared__ __attribute__((aligned(16))) T ks1[KT * D];
+  __shared__ __attribute__((aligned(16))) T vs1[KT * D];
   long long b; int n, tile;
   if (!locate(p, blockIdx.x / p.heads, QT, b, n, tile)) return;
   tile = (n + QT - 1) / QT - 1 - tile;                      // causal: the tiles with most keys start first
   const int head = head_of(blockIdx.x % p.heads, p.heads, p.kv_heads), kv = head / (p.heads / p.kv_heads);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int qw = tile * QT + 32 * w, qi = qw + (lane & 31);  // the wave's first query, the lane's
   const bool own = qi < n;
-  auto limit = [&](int i) { return p.block ? (int)min((long long)n, ((long long)(i / p.block) + 1) * p.block) : n; };
-  const int lim = own ? limit(qi) : 0;
-  const int wave_end = qw < n ? limit(min(qw + 31, n - 1)) : 0;      // keys the wave needs
-  const int wave_min = limit(min(qw, n - 1));                        // keys every query of it sees
-  const int end = limit(min(tile * QT + QT, n) - 1);                 // keys the workgroup needs
+  const int lim = own ? limit(qi, n, p.block) : 0;
+  const int wave_end = qw < n ? limit(min(qw + 31, n - 1), n, p.block) : 0;      // keys the wave needs
+  const int wave_min = limit(min(qw, n - 1), n, p.block);                        // keys every query of it sees
+  const int end = limit(min(tile * QT + QT, n) - 1, n, p.block);                 // keys the workgroup needs
 
   const T* kb = (const T*)p.k + b * p.kr + (long long)kv * p.kh;
   const T* vb = (const T*)p.v + b * p.vr + (long long)kv * p.vh;
+  const Fetch<T, D, KT, NW> fk(p.kr, p.d, w, lane), fv(p.vr, p.d, w, lane);
   const T* qrow = (const T*)p.q + (b + qi) * p.qr + (long long)head * p.qh;
   frag qf[NC];
 #pragma unroll
@@ -131,68 +164,66 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attn_fwd(const At
   float m = -INFINITY, l = 0.f;                             // running maximum (log2 units) and sum
   const float sl2 = p.scale * CORA_LOG2E;
 
-  Stage<T, D, KT, 256> sk, sv;
-  sk.load(kb, p.kr, end, p.d); sv.load(vb, p.vr, end, p.d);
-  sk.store(Ks[0]); sv.store(Vs[0]);
-  __syncthreads();
-  for (int j0 = 0, cur = 0; j0 < end; j0 += KT, cur ^= 1) {
-    const bool more = j0 + KT < end;
-    if (more) {
-      sk.load(kb + (long long)(j0 + KT) * p.kr, p.kr, end - j0 - KT, p.d);
-      sv.load(vb + (long long)(j0 + KT) * p.vr, p.vr, end - j0 - KT, p.d);
+  auto fetch = [&](int it, T* k, T* v) {
+    const int j0 = it * KT;
+    fk(kb + j0 * p.kr, end - j0, k, w);
+    fv(vb + j0 * p.vr, end - j0, v, w);
+  };
+  auto work = [&](int it, const T* k, const T* v) {
+    const int j0 = it * KT;
+    if (j0 >= wave_end) return;
+    f32x16 s[KT / 32];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[t] = O::mma(L::row_frag(k, 32 * t, c, lane), qf[c], s[t]);
     }
-    if (j0 < wave_end) {
-      f32x16 s[KT / 32];
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < KT / 32; ++t) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s[t] = O::mma(L::row_frag(Ks[cur], 32 * t, c, lane), qf[c], s[t]);
-      }
-      if (j0 + KT > wave_min) {
-#pragma unroll
-        for (int t = 0; t < KT / 32; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (j0 + 32 * t + acc_row(r, h) >= lim) s[t][r] = -INFINITY;
-      }
+    if (j0 + KT > wave_min) {
 #pragma unroll
       for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-      mx = half_max(mx) * sl2;
-      const float mn = fmaxf(m, mx);
-      if (__any(mn > m)) {
-        const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= al;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][r] *= al;
-        m = mn;
-      }
-      const float mb = m == -INFINITY ? 0.f : m;            // a row that has seen nothing yet
-      float sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < KT / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], sl2, -mb));
-          sum += s[t][r];
-        }
-      l += sum;
-#pragma unroll
-      for (int k = 0; k < NS; ++k) {
-        const frag pf = O::pack(s[k * O::CH / 32], k % (32 / O::CH));
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] = O::mma(L::col_frag(Vs[cur], k, i, lane), pf, acc[i]);
-      }
+        for (int r = 0; r < 16; ++r)
+          if (j0 + 32 * t + acc_row(r, h) >= lim) s[t][r] = -INFINITY;
     }
-    if (more) { sk.store(Ks[cur ^ 1]); sv.store(Vs[cur ^ 1]); }
-    __syncthreads();
-  }
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+    mx = half_max(mx) * sl2;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= al;
+      m = mn;
+    }
+    const float mb = m == -INFINITY ? 0.f : m;              // a row that has seen nothing yet
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], sl2, -mb));
+        sum += s[t][r];
+      }
+    l += sum;
+#pragma unroll
+    for (int c = 0; c < NS; ++c) {
+      const frag pf = O::pack(s[c * O::CH / 32], c % (32 / O::CH));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] = O::mma(L::col_frag(v, c, i, lane), pf, acc[i]);
+    }
+  };
+#define FETCH(it, buf) fetch(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
+#define WORK(it, buf) work(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
+  WALK((end + KT - 1) / KT, FETCH, WORK)
+#undef FETCH
+#undef WORK
   l = half_sum(l);
   if (own) {
     store_own<T, D>((T*)p.out + (b + qi) * p.orow + (long long)head * p.oh, acc, 1.f / l, p.d, h);
@@ -202,33 +233,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attn_fwd(const At
 
 // ---- backward: dq (and the row constants the dk/dv kernel reads) ---------------------------------
 // fp16 holds nothing below 2^-24, and ds ~ p do / sqrt(n) of an unscaled loss lies there.  Every query row of do therefore
-// enters with a power of two 2^-e that brings its largest element to [1, 2); e is kept beside delta for the other kernel.
-template <typename T, int D>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(const AttnP p) {
+// enters with a power of two 2^-e that brings its largest element to [1, 2); e is kept for the other kernel, beside
+// delta and -lse / scale.  Both products start from these constants instead of zero: s - lse / scale, do v - delta.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
-  constexpr bool F16 = sizeof(T) == 2 && O::CH == 16 && __is_same(T, _Float16);
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 128, NC = D / O::CH;
-  __shared__ __attribute__((aligned(16))) T Ks[2][KT * D];
-  __shared__ __attribute__((aligned(16))) T Vs[2][KT * D];
+  constexpr bool F16 = __is_same(T, _Float16);
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 32 * NW, NC = D / O::CH;
+  __shared__ __attribute__((aligned(16))) T ks0[KT * D];
+  __shared__ __attribute__((aligned(16))) T vs0[KT * D];
+  __shared__ __attribute__((aligned(16))) T ks1[KT * D];
+  __shared__ __attribute__((aligned(16))) T vs1[KT * D];
   long long b; int n, tile;
   if (!locate(p, blockIdx.x / p.heads, QT, b, n, tile)) return;
   tile = (n + QT - 1) / QT - 1 - tile;
   const int head = head_of(blockIdx.x % p.heads, p.heads, p.kv_heads), kv = head / (p.heads / p.kv_heads);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int qw = tile * QT + 32 * w, qi = qw + (lane & 31);
   const bool own = qi < n;
-  auto limit = [&](int i) { return p.block ? (int)min((long long)n, ((long long)(i / p.block) + 1) * p.block) : n; };
-  const int lim = own ? limit(qi) : 0;
-  const int wave_end = qw < n ? limit(min(qw + 31, n - 1)) : 0;
-  const int wave_min = limit(min(qw, n - 1));
-  const int end = limit(min(tile * QT + QT, n) - 1);
+  const int lim = own ? limit(qi, n, p.block) : 0;
+  const int wave_end = qw < n ? limit(min(qw + 31, n - 1), n, p.block) : 0;
+  const int wave_min = limit(min(qw, n - 1), n, p.block);
+  const int end = limit(min(tile * QT + QT, n) - 1, n, p.block);
 
   const T* kb = (const T*)p.k + b * p.kr + (long long)kv * p.kh;
   const T* vb = (const T*)p.v + b * p.vr + (long long)kv * p.vh;
-  Stage<T, D, KT, 256> sk, sv;
-  sk.load(kb, p.kr, end, p.d); sv.load(vb, p.vr, end, p.d);
-
-  const long long row = b + qi;
+  const Fetch<T, D, KT, NW> fk(p.kr, p.d, w, lane), fv(p.vr, p.d, w, lane);
+  const long long row = b + qi, at = (long long)head * p.rows + row, plane = (long long)p.heads * p.rows;
   frag qf[NC], df[NC];
   float delta = 0.f, big = 0.f;
 #pragma unroll
@@ -245,10 +276,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(const 
     big = half_max(big);
     const int e = big > 0.f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
     dscale = __builtin_amdgcn_ldexpf(1.f, -e); back = __builtin_amdgcn_ldexpf(p.scale, e);
-    if (own && h == 0) p.delta[((long long)p.heads + head) * p.rows + row] = big > 0.f ? (float)e : NO_EXP;
+    if (own && h == 0) p.delta[2 * plane + at] = big > 0.f ? (float)e : NO_EXP;
   }
-  const float lse2 = own ? p.lse[(long long)head * p.rows + row] * CORA_LOG2E : 0.f;
-  if (own && h == 0) p.delta[(long long)head * p.rows + row] = delta;
+  const float lse = own ? -p.lse[at] / p.scale : 0.f;
+  if (own && h == 0) { p.delta[at] = -delta; p.delta[plane + at] = lse; }
   const float sl2 = p.scale * CORA_LOG2E;
 
   f32x16 acc[D / 32];
@@ -256,66 +287,74 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(const 
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-  sk.store(Ks[0]); sv.store(Vs[0]);
-  __syncthreads();
-  for (int j0 = 0, cur = 0; j0 < end; j0 += KT, cur ^= 1) {
-    const bool more = j0 + KT < end;
-    if (more) {
-      sk.load(kb + (long long)(j0 + KT) * p.kr, p.kr, end - j0 - KT, p.d);
-      sv.load(vb + (long long)(j0 + KT) * p.vr, p.vr, end - j0 - KT, p.d);
-    }
-    if (j0 < wave_end) {
+
+  auto fetch = [&](int it, T* k, T* v) {
+    const int j0 = it * KT;
+    fk(kb + j0 * p.kr, end - j0, k, w);
+    fv(vb + j0 * p.vr, end - j0, v, w);
+  };
+  auto work = [&](int it, const T* k, const T* v) {
+    const int j0 = it * KT;
+    if (j0 >= wave_end) return;
 #pragma unroll
-      for (int t = 0; t < KT / 32; ++t) {
-        f32x16 s, dp;
+    for (int t = 0; t < KT / 32; ++t) {
+      f32x16 s, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+      for (int r = 0; r < 16; ++r) { s[r] = lse; dp[r] = -delta; }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          s = O::mma(L::row_frag(Ks[cur], 32 * t, c, lane), qf[c], s);
-          dp = O::mma(L::row_frag(Vs[cur], 32 * t, c, lane), df[c], dp);
-        }
-        const bool edge = j0 + 32 * t + 32 > wave_min;
+      for (int c = 0; c < NC; ++c) {
+        s = O::mma(L::row_frag(k, 32 * t, c, lane), qf[c], s);
+        dp = O::mma(L::row_frag(v, 32 * t, c, lane), df[c], dp);
+      }
+      const bool edge = j0 + 32 * t + 32 > wave_min;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)) * (dp[r] - delta);
-          if (F16) pr *= dscale;
-          s[r] = edge && j0 + 32 * t + acc_row(r, h) >= lim ? 0.f : pr;
-        }
+      for (int r = 0; r < 16; ++r) {
+        float pr = __builtin_amdgcn_exp2f(s[r] * sl2) * dp[r];
+        if (F16) pr *= dscale;
+        s[r] = edge && j0 + 32 * t + acc_row(r, h) >= lim ? 0.f : pr;
+      }
 #pragma unroll
-        for (int k = 0; k < 32 / O::CH; ++k) {
-          const frag pf = O::pack(s, k);
+      for (int c = 0; c < 32 / O::CH; ++c) {
+        const frag pf = O::pack(s, c);
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) acc[i] = O::mma(L::col_frag(Ks[cur], t * (32 / O::CH) + k, i, lane), pf, acc[i]);
-        }
+        for (int i = 0; i < D / 32; ++i) acc[i] = O::mma(L::col_frag(k, t * (32 / O::CH) + c, i, lane), pf, acc[i]);
       }
     }
-    if (more) { sk.store(Ks[cur ^ 1]); sv.store(Vs[cur ^ 1]); }
-    __syncthreads();
-  }
+  };
+#define FETCH(it, buf) fetch(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
+#define WORK(it, buf) work(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
+  WALK((end + KT - 1) / KT, FETCH, WORK)
+#undef FETCH
+#undef WORK
   if (own) store_own<T, D>((T*)p.dq + row * p.dqr + (long long)head * p.dqh, acc, back, p.d, h);
 }
 
 // ---- backward: dk and dv -------------------------------------------------------------------------
-// A workgroup owns 128 keys of one key head and walks the queries that see any of them, head after head of its group.
-template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void attn_bwd_kv(const AttnP p) {
+// A workgroup owns 32 NW keys of one key head and walks the queries that see any of them, head after head of its group.
+// Staged rows behind the sequence are zeros, and so are their constants: their p is 1, but do and ds are zero.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void attn_bwd_kv(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
-  constexpr bool F16 = sizeof(T) == 2 && O::CH == 16 && __is_same(T, _Float16);
-  constexpr int QT = sizeof(T) == 4 ? 32 : 64, KB = 128, NC = D / O::CH;
-  __shared__ __attribute__((aligned(16))) T Qs[2][QT * D];
-  __shared__ __attribute__((aligned(16))) T Ds[2][QT * D];
-  __shared__ float cl[2][QT], cd[2][QT], ce[2][QT];     // per staged query: lse (log2), delta, exponent of its do scale
-  __shared__ int lm[2][QT];                             // and the keys it sees
+  constexpr bool F16 = __is_same(T, _Float16);
+  constexpr int QT = sizeof(T) == 4 ? 32 : 64, KB = 32 * NW, NC = D / O::CH;
+  __shared__ __attribute__((aligned(16))) T qs0[QT * D];
+  __shared__ __attribute__((aligned(16))) T ds0[QT * D];
+  __shared__ __attribute__((aligned(16))) T qs1[QT * D];
+  __shared__ __attribute__((aligned(16))) T ds1[QT * D];
+  __shared__ __attribute__((aligned(16))) float cs0[3][64];   // per staged query: -delta, -lse / scale, exponent of its do scale
+  __shared__ __attribute__((aligned(16))) float cs1[3][64];
   long long b; int n, tile;
   if (!locate(p, blockIdx.x / p.kv_heads, KB, b, n, tile)) return;
   const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int k0 = tile * KB, kw = k0 + 32 * w, ki = kw + (lane & 31);
   const bool own = ki < n;
-  const int qbeg = p.block ? k0 / p.block * p.block / QT * QT : 0;    // the first staged query that sees key k0 is behind it
-  const int ntile = (n - qbeg + QT - 1) / QT, total = ntile * group;
+  const int qmin = p.block ? ki / p.block * p.block : 0;              // the first query that sees the lane's key
+  const int wave_max = p.block ? (kw + 31) / p.block * p.block : 0;   // the first that sees all keys of the wave
+  const int qbeg = p.block ? k0 / p.block * p.block / QT * QT : 0;    // the first tile with a query that sees key k0
+  const int ntile = (n - qbeg + QT - 1) / QT;
 
+  const Fetch<T, D, QT, NW> fq(p.qr, p.d, w, lane), fd(p.dor, p.d, w, lane);
   frag kf[NC], vf[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -329,84 +368,74 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_kv(const AttnP p) {
     for (int r = 0; r < 16; ++r) { ak[i][r] = 0.f; av[i][r] = 0.f; }
   const float sl2 = p.scale * CORA_LOG2E;
   float ecur = NO_EXP;                                  // F16: exponent ak is scaled by
+  [[maybe_unused]] const long long plane = (long long)p.heads * p.rows;
 
-  Stage<T, D, QT, 256> sq, sd;
-  float rl = 0.f, rd = 0.f, re = 0.f; int rm = 0;
-  auto load = [&](int it) {
-    const int head = kv * group + it / ntile, q0 = qbeg + (it % ntile) * QT;
-    sq.load((const T*)p.q + (b + q0) * p.qr + (long long)head * p.qh, p.qr, n - q0, p.d);
-    sd.load((const T*)p.dout + (b + q0) * p.dor + (long long)head * p.doh, p.dor, n - q0, p.d);
-    const int i = q0 + (int)threadIdx.x;
-    if (threadIdx.x < QT) {
-      const bool ok = i < n;
-      const long long at = (long long)head * p.rows + b + i;
-      rl = ok ? p.lse[at] * CORA_LOG2E : INFINITY;      // exp2(. - inf) = 0: rows behind the sequence add nothing
-      rd = ok ? p.delta[at] : 0.f;
-      rm = ok ? (p.block ? (int)min((long long)n, ((long long)(i / p.block) + 1) * p.block) : n) : 0;
-      if (F16) re = ok ? p.delta[(long long)p.heads * p.rows + at] : NO_EXP;
-    }
+  auto fetch = [&](int it, T* q, T* d, float (&cs)[3][64]) {
+    const int g = it / ntile, q0 = qbeg + (it - g * ntile) * QT, head = kv * group + g;
+    fq((const T*)p.q + (b + q0) * p.qr + (long long)head * p.qh, n - q0, q, w);
+    fd((const T*)p.dout + (b + q0) * p.dor + (long long)head * p.doh, n - q0, d, w);
+    // constants: one request of 64 floats each (fp32 stages 32 queries and asks for 32 more than it needs)
+#pragma unroll
+    for (int k = 0; k < (F16 ? 3 : 2); ++k)
+      if (w == k % NW) REQUEST(p.delta + k * plane + (long long)head * p.rows + b + q0, 4 * min(n - q0, 64), cs[k], 4, 4 * lane);
   };
-  auto store = [&](int s) {
-    sq.store(Qs[s]); sd.store(Ds[s]);
-    if (threadIdx.x < QT) { cl[s][threadIdx.x] = rl; cd[s][threadIdx.x] = rd; lm[s][threadIdx.x] = rm; if (F16) ce[s][threadIdx.x] = re; }
-  };
-  load(0); store(0);
-  __syncthreads();
-  for (int it = 0, cur = 0; it < total; ++it, cur ^= 1) {
-    const bool more = it + 1 < total;
-    if (more) load(it + 1);
+  auto work = [&](int it, const T* qt, const T* dt_, const float (&cs)[3][64]) {
     const int q0 = qbeg + (it % ntile) * QT;
-    if (kw < n) {
-      if (F16) {
-        float e = ce[cur][lane & (QT - 1)];
+    if (kw >= n) return;
+    if (F16) {
+      float e = q0 + lane < n ? cs[2][lane] : NO_EXP;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) e = fmaxf(e, __shfl_xor(e, o, 64));
-        if (e > ecur) {                                 // larger gradients than before: bring the sum to their scale
-          const float f = ecur == NO_EXP ? 0.f : __builtin_amdgcn_exp2f(ecur - e);
+      for (int o = 32; o > 0; o >>= 1) e = fmaxf(e, __shfl_xor(e, o, 64));
+      if (e > ecur) {                                   // larger gradients than before: bring the sum to their scale
+        const float f = ecur == NO_EXP ? 0.f : __builtin_amdgcn_exp2f(ecur - e);
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i)
+        for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ak[i][r] *= f;
-          ecur = e;
-        }
+          for (int r = 0; r < 16; ++r) ak[i][r] *= f;
+        ecur = e;
       }
-      const float ds = F16 && ecur != NO_EXP ? __builtin_amdgcn_exp2f(-ecur) : 1.f;
+    }
+    const float dscale = F16 && ecur != NO_EXP ? __builtin_amdgcn_exp2f(-ecur) : 1.f;
 #pragma unroll
-      for (int t = 0; t < QT / 32; ++t) {
-        if (q0 + 32 * t >= n) break;
-        f32x16 s, dp;
+    for (int t = 0; t < QT / 32; ++t) {
+      f32x16 s, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 c0 = *reinterpret_cast<const f32x4*>(&cs[1][32 * t + 8 * g + 4 * h]);
+        const f32x4 c1 = *reinterpret_cast<const f32x4*>(&cs[0][32 * t + 8 * g + 4 * h]);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          s = O::mma(L::row_frag(Qs[cur], 32 * t, c, lane), kf[c], s);
-          dp = O::mma(L::row_frag(Ds[cur], 32 * t, c, lane), vf[c], dp);
-        }
-        const bool edge = p.block && lm[cur][32 * t] < kw + 32;
+        for (int i = 0; i < 4; ++i) { s[4 * g + i] = c0[i]; dp[4 * g + i] = c1[i]; }
+      }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int q = 32 * t + acc_row(r, h);
-          float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -cl[cur][q]));
-          float g = pr * (dp[r] - cd[cur][q]);
-          if (F16) g *= ds;
-          const bool hide = edge && ki >= lm[cur][q];
-          s[r] = hide ? 0.f : pr;
-          dp[r] = hide ? 0.f : g;
-        }
+      for (int c = 0; c < NC; ++c) {
+        s = O::mma(L::row_frag(qt, 32 * t, c, lane), kf[c], s);
+        dp = O::mma(L::row_frag(dt_, 32 * t, c, lane), vf[c], dp);
+      }
+      const bool edge = q0 + 32 * t < wave_max;
 #pragma unroll
-        for (int k = 0; k < 32 / O::CH; ++k) {
-          const frag pf = O::pack(s, k), gf = O::pack(dp, k);
+      for (int r = 0; r < 16; ++r) {
+        float pr = __builtin_amdgcn_exp2f(s[r] * sl2), g = pr * dp[r];
+        if (F16) g *= dscale;
+        const bool hide = edge && q0 + 32 * t + acc_row(r, h) < qmin;
+        s[r] = hide ? 0.f : pr;
+        dp[r] = hide ? 0.f : g;
+      }
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            av[i] = O::mma(L::col_frag(Ds[cur], t * (32 / O::CH) + k, i, lane), pf, av[i]);
-            ak[i] = O::mma(L::col_frag(Qs[cur], t * (32 / O::CH) + k, i, lane), gf, ak[i]);
-          }
+      for (int c = 0; c < 32 / O::CH; ++c) {
+        const frag pf = O::pack(s, c), gf = O::pack(dp, c);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          av[i] = O::mma(L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), pf, av[i]);
+          ak[i] = O::mma(L::col_frag(qt, t * (32 / O::CH) + c, i, lane), gf, ak[i]);
         }
       }
     }
-    if (more) store(cur ^ 1);
-    __syncthreads();
-  }
+  };
+#define FETCH(it, buf) fetch(it, buf ? qs1 : qs0, buf ? ds1 : ds0, buf ? cs1 : cs0)
+#define WORK(it, buf) work(it, buf ? qs1 : qs0, buf ? ds1 : ds0, buf ? cs1 : cs0)
+  WALK(ntile * group, FETCH, WORK)
+#undef FETCH
+#undef WORK
   if (own) {
     const float f = F16 && ecur != NO_EXP ? p.scale * __builtin_amdgcn_exp2f(ecur) : p.scale;
     store_own<T, D>((T*)p.dk + (b + ki) * p.dkr + (long long)kv * p.dkh, ak, f, p.d, h);
@@ -418,13 +447,13 @@ long long slots(const AttnP& p, int tr) {
   return p.cu ? p.rows / tr + p.nseq : (long long)p.nseq * ((p.seqlen + tr - 1) / tr);
 }
 template <typename T, int D> int fwd(const AttnP& p, hipStream_t st) {
-  attn_fwd<T, D><<<dim3((unsigned)(slots(p, 128) * p.heads)), 256, 0, st>>>(p);
+  attn_fwd<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.heads)), 256, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
 template <typename T, int D> int bwd(const AttnP& p, hipStream_t st) {
-  attn_bwd_q<T, D><<<dim3((unsigned)(slots(p, 128) * p.heads)), 256, 0, st>>>(p);
+  attn_bwd_q<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.heads)), 256, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return 1;
-  attn_bwd_kv<T, D><<<dim3((unsigned)(slots(p, 128) * p.kv_heads)), 256, 0, st>>>(p);
+  attn_bwd_kv<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.kv_heads)), 256, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
 template <typename T> int fwd_d(const AttnP& p, hipStream_t st) {

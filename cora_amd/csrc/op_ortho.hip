@@ -398,10 +398,10 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
   };
   fetch(buf0, 0);
   for (int k0 = 0; k0 < ld; k0 += 2 * TK) {                // ld is a multiple of 64
-    __syncthreads();                                       // buf0 has arrived, buf1 is no longer read
+    arrive_barrier();                                      // buf0 has arrived, buf1 is no longer read
     fetch(buf1, k0 + TK);
     work(buf0);
-    __syncthreads();
+    arrive_barrier();
     if (k0 + 2 * TK < ld) fetch(buf0, k0 + 2 * TK);
     work(buf1);
   }

@@ -104,3 +104,10 @@ template <typename T, int D> struct Tile {
     return f;
   }
 };
+
+// Barrier behind which the direct requests into LDS of every wave of the workgroup have arrived.  The wait is explicit: a
+// workgroup barrier alone orders LDS and global accesses of the waves, but does not wait for requests still under way.
+__device__ __forceinline__ void arrive_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}

@@ -25,7 +25,7 @@ struct AttnP {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
   float* lse;                   // [heads, rows]
-  float* delta;                 // backward workspace: [2, heads, rows] (rowsum(dout out), then log2 of the row's scale)
+  float* delta;                 // backward workspace [3, heads, rows]: -rowsum(dout out), -lse / scale, exponent of the row's scale (fp16)
   const int* cu;                // [nseq + 1] first rows, or null: nseq sequences of seqlen rows each
   long long rows;
   long long qr, qh, kr, kh, vr, vh, orow, oh, dor, doh, dqr, dqh, dkr, dkh, dvr, dvh;   // element strides

@@ -272,7 +272,8 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream);
  * causal_block 0: a token sees its whole sequence; b >= 1: the tokens of its own and of earlier blocks of b tokens of the
  * sequence (1: causal; tokens per frame: frame-causal).
  *   out_i = sum_j softmax_j(scale q_i k_j) v_j,  lse [heads, rows] = log sum_j exp(scale q_i k_j)  (float32)
- * head_dim: up to 128, a multiple of 8 (float32: 4); pointers 16-byte aligned, strides multiples of 16 bytes.  Sums and
+ * head_dim: up to 128, a multiple of 8 (float32: 4); pointers 16-byte aligned, strides multiples of 16 bytes,
+ * row strides below 2^24 elements.  Sums and
  * softmax statistics are float32; the probabilities are rounded to a 16-bit dtype before they meet v.
  * Backward: dout and the forward's out and lse -> dq, dk, dv (sums over the query heads of a key head).  workspace:
  * cora_attention_workspace(a) bytes, 16-byte aligned, not shared by calls that may overlap.  Results repeat bit for bit. */

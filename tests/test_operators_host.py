@@ -60,7 +60,7 @@ def attn_args(**kw):
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(cu_seqlens=None, seq_len=51), "seq_len"), (dict(cu_seqlens=None, seq_len=0), "seq_len"), (dict(q=None), "q is NULL"),
     (dict(k=FAKE + 8), "k must be 16-byte"), (dict(v_row=130), "v must be"), (dict(q_head=-64), "q must be"),
-    (dict(out_row=128), "overlap"), (dict(out_head=0), "overlap"), (dict(lse=None), "lse"), (dict(cu_seqlens=FAKE + 2), "aligned"),
+    (dict(k_row=1 << 24), "row stride"), (dict(out_row=128), "overlap"), (dict(out_head=0), "overlap"), (dict(lse=None), "lse"), (dict(cu_seqlens=FAKE + 2), "aligned"),
 ])
 def test_attention_refuses(kw, word):
     lib = _lib.load()
@@ -71,7 +71,7 @@ def test_attention_refuses(kw, word):
 
 @pytest.mark.parametrize("kw,word", [
     (dict(dout=None), "dout is NULL"), (dict(dq=None), "dq is NULL"), (dict(dk_row=64), "overlap"), (dict(dv_head=32), "overlap"),
-    (dict(workspace=None), "workspace"), (dict(workspace=FAKE + 4), "workspace"), (dict(workspace_bytes=4 * 100 * 2 * 4 - 1), "workspace"),
+    (dict(workspace=None), "workspace"), (dict(workspace=FAKE + 4), "workspace"), (dict(workspace_bytes=4 * 100 * 3 * 4 - 1), "workspace"),
 ])
 def test_attention_backward_refuses(kw, word):
     assert _lib.load().cora_attention_backward(C.byref(attn_args(**kw)), 0, None) == -1 and word in _err()
