@@ -20,6 +20,7 @@
 // No atomics: every output element is summed by one wave in a fixed order, so results repeat bit for bit.
 #include "op_tile.h"
 #include "ops.h"
+#include <cstdlib>
 
 namespace {
 
@@ -129,7 +130,7 @@ __device__ __forceinline__ int limit(int i, int n, int block) {
 // NW waves of 32 queries each.  The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_fwd(const AttnP p) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void attn_fwd(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 32 * NW, NC = D / O::CH, NS = KT / O::CH;
   __shared__ __attribute__((aligned(16))) T ks0[KT * D];
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_fwd(cons
 // enters with a power of two 2^-e that brings its largest element to [1, 2); e is kept for the other kernel, beside
 // delta and -lse / scale.  Both products start from these constants instead of zero: s - lse / scale, do v - delta.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(const AttnP p) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
   constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 32 * NW, NC = D / O::CH;
@@ -306,12 +307,16 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(co
         s = O::mma(L::row_frag(k, 32 * t, c, lane), qf[c], s);
         dp = O::mma(L::row_frag(v, 32 * t, c, lane), df[c], dp);
       }
-      const bool edge = j0 + 32 * t + 32 > wave_min;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float pr = __builtin_amdgcn_exp2f(s[r] * sl2) * dp[r];
         if (F16) pr *= dscale;
-        s[r] = edge && j0 + 32 * t + acc_row(r, h) >= lim ? 0.f : pr;
+        s[r] = pr;
+      }
+      if (j0 + 32 * t + 32 > wave_min) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (j0 + 32 * t + acc_row(r, h) >= lim) s[r] = 0.f;
       }
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
@@ -331,9 +336,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void attn_bwd_q(co
 
 // ---- backward: dk and dv -------------------------------------------------------------------------
 // A workgroup owns 32 NW keys of one key head and walks the queries that see any of them, head after head of its group.
+// With p.parts > 1 that walk is cut into as many ranges, one per workgroup (blockIdx.y), whose sums go to the workspace in
+// fp32 and are added in order by attn_bwd_sum: few workgroups with long walks would leave most of the chip idle.
 // Staged rows behind the sequence are zeros, and so are their constants: their p is 1, but do and ds are zero.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void attn_bwd_kv(const AttnP p) {
+__global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1 : 2) void attn_bwd_kv(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
   constexpr int QT = sizeof(T) == 4 ? 32 : 64, KB = 32 * NW, NC = D / O::CH;
@@ -352,7 +359,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void a
   const int qmin = p.block ? ki / p.block * p.block : 0;              // the first query that sees the lane's key
   const int wave_max = p.block ? (kw + 31) / p.block * p.block : 0;   // the first that sees all keys of the wave
   const int qbeg = p.block ? k0 / p.block * p.block / QT * QT : 0;    // the first tile with a query that sees key k0
-  const int ntile = (n - qbeg + QT - 1) / QT;
+  const int ntile = (n - qbeg + QT - 1) / QT, total = ntile * group;
+  const int it0 = (int)((long long)total * blockIdx.y / p.parts), it1 = (int)((long long)total * (blockIdx.y + 1) / p.parts);
 
   const Fetch<T, D, QT, NW> fq(p.qr, p.d, w, lane), fd(p.dor, p.d, w, lane);
   frag kf[NC], vf[NC];
@@ -371,6 +379,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void a
   [[maybe_unused]] const long long plane = (long long)p.heads * p.rows;
 
   auto fetch = [&](int it, T* q, T* d, float (&cs)[3][64]) {
+    it += it0;
     const int g = it / ntile, q0 = qbeg + (it - g * ntile) * QT, head = kv * group + g;
     fq((const T*)p.q + (b + q0) * p.qr + (long long)head * p.qh, n - q0, q, w);
     fd((const T*)p.dout + (b + q0) * p.dor + (long long)head * p.doh, n - q0, d, w);
@@ -380,7 +389,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void a
       if (w == k % NW) REQUEST(p.delta + k * plane + (long long)head * p.rows + b + q0, 4 * min(n - q0, 64), cs[k], 4, 4 * lane);
   };
   auto work = [&](int it, const T* qt, const T* dt_, const float (&cs)[3][64]) {
-    const int q0 = qbeg + (it % ntile) * QT;
+    const int q0 = qbeg + ((it0 + it) % ntile) * QT;
     if (kw >= n) return;
     if (F16) {
       float e = q0 + lane < n ? cs[2][lane] : NO_EXP;
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void a
       }
     }
     const float dscale = F16 && ecur != NO_EXP ? __builtin_amdgcn_exp2f(-ecur) : 1.f;
-#pragma unroll
+#pragma unroll D == 128 ? 1 : 2
     for (int t = 0; t < QT / 32; ++t) {
       f32x16 s, dp;
 #pragma unroll
@@ -406,54 +415,102 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || D == 128 ? 1 : 2) void a
 #pragma unroll
         for (int i = 0; i < 4; ++i) { s[4 * g + i] = c0[i]; dp[4 * g + i] = c1[i]; }
       }
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        s = O::mma(L::row_frag(qt, 32 * t, c, lane), kf[c], s);
-        dp = O::mma(L::row_frag(dt_, 32 * t, c, lane), vf[c], dp);
-      }
       const bool edge = q0 + 32 * t < wave_max;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float pr = __builtin_amdgcn_exp2f(s[r] * sl2), g = pr * dp[r];
-        if (F16) g *= dscale;
-        const bool hide = edge && q0 + 32 * t + acc_row(r, h) < qmin;
-        s[r] = hide ? 0.f : pr;
-        dp[r] = hide ? 0.f : g;
+      for (int c = 0; c < NC; ++c) s = O::mma(L::row_frag(qt, 32 * t, c, lane), kf[c], s);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * sl2);
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (q0 + 32 * t + acc_row(r, h) < qmin) s[r] = 0.f;
       }
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
-        const frag pf = O::pack(s, c), gf = O::pack(dp, c);
+        const frag pf = O::pack(s, c);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          av[i] = O::mma(L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), pf, av[i]);
-          ak[i] = O::mma(L::col_frag(qt, t * (32 / O::CH) + c, i, lane), gf, ak[i]);
-        }
+        for (int i = 0; i < D / 32; ++i) av[i] = O::mma(L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), pf, av[i]);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) dp = O::mma(L::row_frag(dt_, 32 * t, c, lane), vf[c], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dp[r] *= s[r];
+        if (F16) dp[r] *= dscale;
+      }
+      if (edge) {                                       // p = 0 does not hide an infinite do v
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (q0 + 32 * t + acc_row(r, h) < qmin) dp[r] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 32 / O::CH; ++c) {
+        const frag gf = O::pack(dp, c);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) ak[i] = O::mma(L::col_frag(qt, t * (32 / O::CH) + c, i, lane), gf, ak[i]);
       }
     }
   };
 #define FETCH(it, buf) fetch(it, buf ? qs1 : qs0, buf ? ds1 : ds0, buf ? cs1 : cs0)
 #define WORK(it, buf) work(it, buf ? qs1 : qs0, buf ? ds1 : ds0, buf ? cs1 : cs0)
-  WALK(ntile * group, FETCH, WORK)
+  if (it1 > it0) { WALK(it1 - it0, FETCH, WORK) }
 #undef FETCH
 #undef WORK
   if (own) {
     const float f = F16 && ecur != NO_EXP ? p.scale * __builtin_amdgcn_exp2f(ecur) : p.scale;
+    if (p.parts > 1) {
+      const long long half = p.rows * p.kv_heads * p.d;
+      float* dst = p.partial + 2 * half * blockIdx.y + ((b + ki) * p.kv_heads + kv) * p.d;
+      store_own<float, D>(dst, ak, f, p.d, h);
+      store_own<float, D>(dst + half, av, 1.f, p.d, h);
+      return;
+    }
     store_own<T, D>((T*)p.dk + (b + ki) * p.dkr + (long long)kv * p.dkh, ak, f, p.d, h);
     store_own<T, D>((T*)p.dv + (b + ki) * p.dvr + (long long)kv * p.dvh, av, 1.f, p.d, h);
   }
 }
 
+// dk and dv from the parts' sums; a thread takes four channels of a row.  Bound by reading 8 parts bytes per element.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_sum(const AttnP p) {
+  const long long half = p.rows * p.kv_heads * p.d, e = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= half) return;
+  const int ch = (int)(e % p.d);
+  const long long rh = e / p.d, row = rh / p.kv_heads;
+  const int kv = (int)(rh - row * p.kv_heads);
+  // rows of no sequence stay as they are
+  const long long lo = p.cu ? p.cu[0] : 0, hi = p.cu ? p.cu[p.nseq] : (long long)p.nseq * p.seqlen;
+  if (row < lo || row >= hi) return;
+  const float* src = p.partial + (blockIdx.y ? half : 0) + e;
+  f32x4 s = *reinterpret_cast<const f32x4*>(src);
+  for (int i = 1; i < p.parts; ++i) s += *reinterpret_cast<const f32x4*>(src + 2 * half * i);
+  T* dst = blockIdx.y ? (T*)p.dv + row * p.dvr + (long long)kv * p.dvh : (T*)p.dk + row * p.dkr + (long long)kv * p.dkh;
+  store4<T>(dst + ch, s[0], s[1], s[2], s[3]);
+}
+
+#ifndef NWF
+#define NWF 4
+#endif
+#ifndef NWQ
+#define NWQ 4
+#endif
+#ifndef NWK
+#define NWK 4
+#endif
 long long slots(const AttnP& p, int tr) {
   return p.cu ? p.rows / tr + p.nseq : (long long)p.nseq * ((p.seqlen + tr - 1) / tr);
 }
 template <typename T, int D> int fwd(const AttnP& p, hipStream_t st) {
-  attn_fwd<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.heads)), 256, 0, st>>>(p);
+  attn_fwd<T, D, NWF><<<dim3((unsigned)(slots(p, 32 * NWF) * p.heads)), 64 * NWF, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
 template <typename T, int D> int bwd(const AttnP& p, hipStream_t st) {
-  attn_bwd_q<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.heads)), 256, 0, st>>>(p);
+  attn_bwd_q<T, D, NWQ><<<dim3((unsigned)(slots(p, 32 * NWQ) * p.heads)), 64 * NWQ, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return 1;
-  attn_bwd_kv<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.kv_heads)), 256, 0, st>>>(p);
+  attn_bwd_kv<T, D, NWK><<<dim3((unsigned)(slots(p, 32 * NWK) * p.kv_heads), (unsigned)p.parts), 64 * NWK, 0, st>>>(p);
+  if (hipGetLastError() != hipSuccess) return 1;
+  if (p.parts == 1) return 0;
+  attn_bwd_sum<T><<<dim3((unsigned)((p.rows * p.kv_heads * p.d / 4 + 255) / 256), 2), 256, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
 template <typename T> int fwd_d(const AttnP& p, hipStream_t st) {
@@ -465,6 +522,11 @@ template <typename T> int bwd_d(const AttnP& p, hipStream_t st) {
 
 }  // namespace
 
+int attention_parts(long long rows, int nseq, int heads, int kv_heads, int d) {
+  static const char* e = getenv("PARTS");
+  if (e) return atoi(e);
+  return 1;
+}
 int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st) {
   return dtype == OP_F32 ? fwd_d<float>(p, st) : dtype == OP_BF16 ? fwd_d<__bf16>(p, st) : fwd_d<_Float16>(p, st);
 }

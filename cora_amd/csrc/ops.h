@@ -26,12 +26,15 @@ struct AttnP {
   void *out, *dq, *dk, *dv;
   float* lse;                   // [heads, rows]
   float* delta;                 // backward workspace [3, heads, rows]: -rowsum(dout out), -lse / scale, exponent of the row's scale (fp16)
+  float* partial;               // [parts, 2, rows, kv_heads, d]: dk and dv of each part, if parts > 1
+  int parts;                    // ranges the queries of a key tile are cut into (attention_parts)
   const int* cu;                // [nseq + 1] first rows, or null: nseq sequences of seqlen rows each
   long long rows;
   long long qr, qh, kr, kh, vr, vh, orow, oh, dor, doh, dqr, dqh, dkr, dkh, dvr, dvh;   // element strides
   int nseq, seqlen, heads, kv_heads, d, block;   // block: causal block, 0 = bidirectional
   float scale;
 };
+int attention_parts(long long rows, int nseq, int heads, int kv_heads, int d);
 int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st);
 int launch_attention_bwd(const AttnP& p, int dtype, hipStream_t st);
 
