@@ -86,7 +86,7 @@ int check_attention(const cora_attention_args* a, AttnP* p, const char* who, boo
   memset(p, 0, sizeof *p);
   p->q = a->q; p->k = a->k; p->v = a->v; p->out = a->out; p->o = a->out; p->lse = a->lse;
   p->dout = a->dout; p->dq = a->dq; p->dk = a->dk; p->dv = a->dv; p->delta = (float*)a->workspace; p->cu = a->cu_seqlens;
-  p->parts = backward ? attention_parts(a->rows, a->n_seq, a->heads, a->kv_heads, a->head_dim) : 1;
+  p->parts = backward ? attention_parts(a->dtype, a->rows, a->n_seq, a->heads, a->kv_heads, a->causal_block) : 1;
   p->partial = (float*)((char*)a->workspace + ((size_t)a->heads * (size_t)a->rows * 3 * sizeof(float) + 15) / 16 * 16);
   p->rows = a->rows;
   p->qr = a->q_row; p->qh = a->q_head; p->kr = a->k_row; p->kh = a->k_head; p->vr = a->v_row; p->vh = a->v_head;
@@ -179,9 +179,9 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream) {
 }
 
 size_t cora_attention_workspace(const cora_attention_args* a) {
-  if (!a || a->heads < 1 || a->kv_heads < 1 || a->head_dim < 1 || a->rows < 1) return 16;
+  if (!a || a->heads < 1 || a->kv_heads < 1 || a->head_dim < 1 || a->rows < 1 || a->n_seq < 0) return 16;
   const size_t constants = ((size_t)a->heads * (size_t)a->rows * 3 * sizeof(float) + 15) / 16 * 16;
-  const int parts = attention_parts(a->rows, a->n_seq, a->heads, a->kv_heads, a->head_dim);
+  const int parts = attention_parts(a->dtype, a->rows, a->n_seq, a->heads, a->kv_heads, a->causal_block);
   return constants + (parts > 1 ? (size_t)parts * 2 * sizeof(float) * (size_t)a->rows * (size_t)a->kv_heads * (size_t)a->head_dim : 0);
 }
 

@@ -20,7 +20,6 @@
 // No atomics: every output element is summed by one wave in a fixed order, so results repeat bit for bit.
 #include "op_tile.h"
 #include "ops.h"
-#include <cstdlib>
 
 namespace {
 
@@ -126,23 +125,59 @@ __device__ __forceinline__ int limit(int i, int n, int block) {
     WORK(it_ + 1, 1);                                                              \
   }
 
+// Queries of a workgroup and its walk over keys.  SPLIT = false: NW waves of 32 queries each share every staged tile of KT
+// keys.  SPLIT = true, for few rows: NW waves share the same 32 queries, wave w walks the key tiles w, w + NW, .. through
+// buffers of its own, and the waves' results are joined in LDS at the end (join_own).
+template <typename T, int D, int NW, bool SPLIT> struct Walk {
+  static constexpr int KT = sizeof(T) == 4 || SPLIT ? 32 : 64, QT = SPLIT ? 32 : 32 * NW;
+  static constexpr int TILE = KT * D, BUF = SPLIT ? NW * TILE : TILE, FW = SPLIT ? 1 : NW;    // elements; waves that fetch a tile
+};
+
+// Sum over the waves of a workgroup of their accumulators, into wave 0, in halving steps.  lds: NW / 2 * D * 32 floats,
+// no longer used for anything else.
+template <int D, int NW>
+__device__ __forceinline__ void join_own(f32x16 (&acc)[D / 32], float* lds, int w, int lane) {
+#pragma unroll
+  for (int o = NW / 2; o >= 1; o /= 2) {
+    float* at = lds + (w % o) * (D * 32) + lane * 4;
+    __syncthreads();
+    if (w >= o && w < 2 * o)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(at + (4 * i + g) * 256) = f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+    __syncthreads();
+    if (w < o)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(at + (4 * i + g) * 256);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][4 * g + e] += v[e];
+        }
+  }
+}
+
 // ---- forward -------------------------------------------------------------------------------------
-// NW waves of 32 queries each.  The running maximum m only has to keep exp2 in range, so it is raised (and the sums
+// The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void attn_fwd(const AttnP p) {
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_fwd(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 32 * NW, NC = D / O::CH, NS = KT / O::CH;
-  __shared__ __attribute__((aligned(16))) T ks0[KT * D];
-  __shared__ __attribute__((aligned(16))) T vs0[KT * D];
-  __shared__ __attribute__((aligned(16))) T ks1[KT * D];
-  __shared__ __attribute__((aligned(16))) T vs1[KT * D];
+  typedef Walk<T, D, NW, SPLIT> W;
+  constexpr int KT = W::KT, QT = W::QT, NC = D / O::CH, NS = KT / O::CH;
+  __shared__ __attribute__((aligned(16))) T ks0[W::BUF];
+  __shared__ __attribute__((aligned(16))) T vs0[W::BUF];
+  __shared__ __attribute__((aligned(16))) T ks1[W::BUF];
+  __shared__ __attribute__((aligned(16))) T vs1[W::BUF];
   long long b; int n, tile;
   if (!locate(p, blockIdx.x / p.heads, QT, b, n, tile)) return;
   tile = (n + QT - 1) / QT - 1 - tile;                      // causal: the tiles with most keys start first
   const int head = head_of(blockIdx.x % p.heads, p.heads, p.kv_heads), kv = head / (p.heads / p.kv_heads);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int qw = tile * QT + 32 * w, qi = qw + (lane & 31);  // the wave's first query, the lane's
+  const int qw = tile * QT + (SPLIT ? 0 : 32 * w), qi = qw + (lane & 31);  // the wave's first query, the lane's
   const bool own = qi < n;
   const int lim = own ? limit(qi, n, p.block) : 0;
   const int wave_end = qw < n ? limit(min(qw + 31, n - 1), n, p.block) : 0;      // keys the wave needs
@@ -151,7 +186,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
 
   const T* kb = (const T*)p.k + b * p.kr + (long long)kv * p.kh;
   const T* vb = (const T*)p.v + b * p.vr + (long long)kv * p.vh;
-  const Fetch<T, D, KT, NW> fk(p.kr, p.d, w, lane), fv(p.vr, p.d, w, lane);
+  const int fw = SPLIT ? 0 : w, mine = SPLIT ? w * W::TILE : 0;    // the wave's share of the requests, its place in a buffer
+  const Fetch<T, D, KT, W::FW> fk(p.kr, p.d, fw, lane), fv(p.vr, p.d, fw, lane);
   const T* qrow = (const T*)p.q + (b + qi) * p.qr + (long long)head * p.qh;
   frag qf[NC];
 #pragma unroll
@@ -166,13 +202,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
   const float sl2 = p.scale * CORA_LOG2E;
 
   auto fetch = [&](int it, T* k, T* v) {
-    const int j0 = it * KT;
-    fk(kb + j0 * p.kr, end - j0, k, w);
-    fv(vb + j0 * p.vr, end - j0, v, w);
+    const int j0 = (SPLIT ? it * NW + w : it) * KT;
+    fk(kb + j0 * p.kr, end - j0, k + mine, fw);
+    fv(vb + j0 * p.vr, end - j0, v + mine, fw);
   };
   auto work = [&](int it, const T* k, const T* v) {
-    const int j0 = it * KT;
+    const int j0 = (SPLIT ? it * NW + w : it) * KT;
     if (j0 >= wave_end) return;
+    k += mine; v += mine;
     f32x16 s[KT / 32];
     float mx = -INFINITY;
 #pragma unroll
@@ -222,35 +259,58 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
   };
 #define FETCH(it, buf) fetch(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
 #define WORK(it, buf) work(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
-  WALK((end + KT - 1) / KT, FETCH, WORK)
+  WALK(SPLIT ? (end + NW * KT - 1) / (NW * KT) : (end + KT - 1) / KT, FETCH, WORK)
 #undef FETCH
 #undef WORK
   l = half_sum(l);
-  if (own) {
-    store_own<T, D>((T*)p.out + (b + qi) * p.orow + (long long)head * p.oh, acc, 1.f / l, p.d, h);
-    if (h == 0) p.lse[(long long)head * p.rows + b + qi] = (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  if constexpr (SPLIT) {                                    // one maximum for all waves, then their sums add up
+    __shared__ float ml[2][NW][32];
+    if (h == 0) { ml[0][w][lane & 31] = m; ml[1][w][lane & 31] = l; }
+    __syncthreads();
+    float mt = ml[0][0][lane & 31];
+#pragma unroll
+    for (int o = 1; o < NW; ++o) mt = fmaxf(mt, ml[0][o][lane & 31]);
+    l = 0.f;
+#pragma unroll
+    for (int o = 0; o < NW; ++o) {
+      const float mo = ml[0][o][lane & 31];
+      if (mo != -INFINITY) l += ml[1][o][lane & 31] * __builtin_amdgcn_exp2f(mo - mt);
+    }
+    const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= al;
+    join_own<D, NW>(acc, reinterpret_cast<float*>(ks0), w, lane);
+    if (w) return;
+    m = mt;
   }
+  if (!own) return;
+  store_own<T, D>((T*)p.out + (b + qi) * p.orow + (long long)head * p.oh, acc, 1.f / l, p.d, h);
+  if (h == 0) p.lse[(long long)head * p.rows + b + qi] = (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 // ---- backward: dq (and the row constants the dk/dv kernel reads) ---------------------------------
 // fp16 holds nothing below 2^-24, and ds ~ p do / sqrt(n) of an unscaled loss lies there.  Every query row of do therefore
 // enters with a power of two 2^-e that brings its largest element to [1, 2); e is kept for the other kernel, beside
-// delta and -lse / scale.  Both products start from these constants instead of zero: s - lse / scale, do v - delta.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void attn_bwd_q(const AttnP p) {
+// -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves nothing and
+// triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
+template <typename T, int D, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64, QT = 32 * NW, NC = D / O::CH;
-  __shared__ __attribute__((aligned(16))) T ks0[KT * D];
-  __shared__ __attribute__((aligned(16))) T vs0[KT * D];
-  __shared__ __attribute__((aligned(16))) T ks1[KT * D];
-  __shared__ __attribute__((aligned(16))) T vs1[KT * D];
+  typedef Walk<T, D, NW, SPLIT> W;
+  constexpr int KT = W::KT, QT = W::QT, NC = D / O::CH;
+  __shared__ __attribute__((aligned(16))) T ks0[W::BUF];
+  __shared__ __attribute__((aligned(16))) T vs0[W::BUF];
+  __shared__ __attribute__((aligned(16))) T ks1[W::BUF];
+  __shared__ __attribute__((aligned(16))) T vs1[W::BUF];
   long long b; int n, tile;
   if (!locate(p, blockIdx.x / p.heads, QT, b, n, tile)) return;
   tile = (n + QT - 1) / QT - 1 - tile;
   const int head = head_of(blockIdx.x % p.heads, p.heads, p.kv_heads), kv = head / (p.heads / p.kv_heads);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int qw = tile * QT + 32 * w, qi = qw + (lane & 31);
+  const int qw = tile * QT + (SPLIT ? 0 : 32 * w), qi = qw + (lane & 31);
   const bool own = qi < n;
   const int lim = own ? limit(qi, n, p.block) : 0;
   const int wave_end = qw < n ? limit(min(qw + 31, n - 1), n, p.block) : 0;
@@ -259,7 +319,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
 
   const T* kb = (const T*)p.k + b * p.kr + (long long)kv * p.kh;
   const T* vb = (const T*)p.v + b * p.vr + (long long)kv * p.vh;
-  const Fetch<T, D, KT, NW> fk(p.kr, p.d, w, lane), fv(p.vr, p.d, w, lane);
+  const int fw = SPLIT ? 0 : w, mine = SPLIT ? w * W::TILE : 0;    // the wave's share of the requests, its place in a buffer
+  const Fetch<T, D, KT, W::FW> fk(p.kr, p.d, fw, lane), fv(p.vr, p.d, fw, lane);
   const long long row = b + qi, at = (long long)head * p.rows + row, plane = (long long)p.heads * p.rows;
   frag qf[NC], df[NC];
   float delta = 0.f, big = 0.f;
@@ -279,9 +340,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
     dscale = __builtin_amdgcn_ldexpf(1.f, -e); back = __builtin_amdgcn_ldexpf(p.scale, e);
     if (own && h == 0) p.delta[2 * plane + at] = big > 0.f ? (float)e : NO_EXP;
   }
-  const float lse = own ? -p.lse[at] / p.scale : 0.f;
-  if (own && h == 0) { p.delta[at] = -delta; p.delta[plane + at] = lse; }
-  const float sl2 = p.scale * CORA_LOG2E;
+  const float lse2 = own ? p.lse[at] * CORA_LOG2E : 0.f, sl2 = p.scale * CORA_LOG2E;
+  if (own && h == 0) { p.delta[at] = -delta; p.delta[plane + at] = -lse2; }
 
   f32x16 acc[D / 32];
 #pragma unroll
@@ -290,18 +350,19 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
 
   auto fetch = [&](int it, T* k, T* v) {
-    const int j0 = it * KT;
-    fk(kb + j0 * p.kr, end - j0, k, w);
-    fv(vb + j0 * p.vr, end - j0, v, w);
+    const int j0 = (SPLIT ? it * NW + w : it) * KT;
+    fk(kb + j0 * p.kr, end - j0, k + mine, fw);
+    fv(vb + j0 * p.vr, end - j0, v + mine, fw);
   };
   auto work = [&](int it, const T* k, const T* v) {
-    const int j0 = it * KT;
+    const int j0 = (SPLIT ? it * NW + w : it) * KT;
     if (j0 >= wave_end) return;
+    k += mine; v += mine;
 #pragma unroll
     for (int t = 0; t < KT / 32; ++t) {
       f32x16 s, dp;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { s[r] = lse; dp[r] = -delta; }
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = -delta; }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         s = O::mma(L::row_frag(k, 32 * t, c, lane), qf[c], s);
@@ -309,7 +370,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float pr = __builtin_amdgcn_exp2f(s[r] * sl2) * dp[r];
+        float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)) * dp[r];
         if (F16) pr *= dscale;
         s[r] = pr;
       }
@@ -328,9 +389,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && D > 64 ? 1 : 2) void att
   };
 #define FETCH(it, buf) fetch(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
 #define WORK(it, buf) work(it, buf ? ks1 : ks0, buf ? vs1 : vs0)
-  WALK((end + KT - 1) / KT, FETCH, WORK)
+  WALK(SPLIT ? (end + NW * KT - 1) / (NW * KT) : (end + KT - 1) / KT, FETCH, WORK)
 #undef FETCH
 #undef WORK
+  if constexpr (SPLIT) {
+    join_own<D, NW>(acc, reinterpret_cast<float*>(ks0), w, lane);
+    if (w) return;
+  }
   if (own) store_own<T, D>((T*)p.dq + row * p.dqr + (long long)head * p.dqh, acc, back, p.d, h);
 }
 
@@ -348,7 +413,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   __shared__ __attribute__((aligned(16))) T ds0[QT * D];
   __shared__ __attribute__((aligned(16))) T qs1[QT * D];
   __shared__ __attribute__((aligned(16))) T ds1[QT * D];
-  __shared__ __attribute__((aligned(16))) float cs0[3][64];   // per staged query: -delta, -lse / scale, exponent of its do scale
+  __shared__ __attribute__((aligned(16))) float cs0[3][64];   // per staged query: -delta, -lse (log2), exponent of its do scale
   __shared__ __attribute__((aligned(16))) float cs1[3][64];
   long long b; int n, tile;
   if (!locate(p, blockIdx.x / p.kv_heads, KB, b, n, tile)) return;
@@ -410,16 +475,19 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
       f32x16 s, dp;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 c0 = *reinterpret_cast<const f32x4*>(&cs[1][32 * t + 8 * g + 4 * h]);
         const f32x4 c1 = *reinterpret_cast<const f32x4*>(&cs[0][32 * t + 8 * g + 4 * h]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { s[4 * g + i] = c0[i]; dp[4 * g + i] = c1[i]; }
+        for (int i = 0; i < 4; ++i) { s[4 * g + i] = 0.f; dp[4 * g + i] = c1[i]; }
       }
       const bool edge = q0 + 32 * t < wave_max;
 #pragma unroll
       for (int c = 0; c < NC; ++c) s = O::mma(L::row_frag(qt, 32 * t, c, lane), kf[c], s);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * sl2);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 c0 = *reinterpret_cast<const f32x4*>(&cs[1][32 * t + 8 * g + 4 * h]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], sl2, c0[i]));
+      }
       if (edge) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -488,48 +556,53 @@ __global__ __launch_bounds__(256) void attn_bwd_sum(const AttnP p) {
   store4<T>(dst + ch, s[0], s[1], s[2], s[3]);
 }
 
-#ifndef NWF
-#define NWF 4
-#endif
-#ifndef NWQ
-#define NWQ 4
-#endif
-#ifndef NWK
-#define NWK 4
-#endif
 long long slots(const AttnP& p, int tr) {
   return p.cu ? p.rows / tr + p.nseq : (long long)p.nseq * ((p.seqlen + tr - 1) / tr);
 }
-template <typename T, int D> int fwd(const AttnP& p, hipStream_t st) {
-  attn_fwd<T, D, NWF><<<dim3((unsigned)(slots(p, 32 * NWF) * p.heads)), 64 * NWF, 0, st>>>(p);
+template <typename T, int D, int NW, bool SPLIT> int fwd(const AttnP& p, hipStream_t st) {
+  attn_fwd<T, D, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
-template <typename T, int D> int bwd(const AttnP& p, hipStream_t st) {
-  attn_bwd_q<T, D, NWQ><<<dim3((unsigned)(slots(p, 32 * NWQ) * p.heads)), 64 * NWQ, 0, st>>>(p);
+template <typename T, int D, int NW, bool SPLIT> int bwd(const AttnP& p, hipStream_t st) {
+  attn_bwd_q<T, D, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return 1;
-  attn_bwd_kv<T, D, NWK><<<dim3((unsigned)(slots(p, 32 * NWK) * p.kv_heads), (unsigned)p.parts), 64 * NWK, 0, st>>>(p);
+  attn_bwd_kv<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.kv_heads), (unsigned)p.parts), 256, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return 1;
   if (p.parts == 1) return 0;
   attn_bwd_sum<T><<<dim3((unsigned)((p.rows * p.kv_heads * p.d / 4 + 255) / 256), 2), 256, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
-template <typename T> int fwd_d(const AttnP& p, hipStream_t st) {
-  return p.d <= 32 ? fwd<T, 32>(p, st) : p.d <= 64 ? fwd<T, 64>(p, st) : p.d <= 96 ? fwd<T, 96>(p, st) : fwd<T, 128>(p, st);
+// Forward and dq, few rows: with W = rows * heads / 32 waves of queries and 1024 SIMDs, splitting the keys over the waves of
+// a workgroup pays up to W = 512 where two such workgroups fit a compute unit (D <= 64), to 256 above, and to twice that
+// for causal walks over long sequences, whose last tiles keep the rest waiting.  Forward, us, split / not:
+//   fp32 D 64:  16 x 1024 tokens x 1 head (W 512) 55 / 77;  4 x 1024 x 8 (W 1024) 107 / 86;  1 x 4096 x 8 causal 193 / 285
+//   bf16 D 128: 1 x 4096 x 2 (W 256) 43 / 77;  16 x 1024 x 1 (W 512) 32 / 26;  1 x 16384 x 1 causal (W 512) 171 / 291
+template <typename T, int D, bool BWD> int run(const AttnP& p, hipStream_t st) {
+  constexpr int NS = sizeof(T) == 4 && D > 64 ? 2 : 4;      // waves whose buffers fit LDS
+  const long long w = p.rows * p.heads / 32, most = (D <= 64 ? 512 : 256) * (p.block && p.rows / p.nseq >= 2048 ? 2 : 1);
+  if (w <= most) { if constexpr (BWD) return bwd<T, D, NS, true>(p, st); else return fwd<T, D, NS, true>(p, st); }
+  if constexpr (BWD) return bwd<T, D, 4, false>(p, st); else return fwd<T, D, 4, false>(p, st);
 }
-template <typename T> int bwd_d(const AttnP& p, hipStream_t st) {
-  return p.d <= 32 ? bwd<T, 32>(p, st) : p.d <= 64 ? bwd<T, 64>(p, st) : p.d <= 96 ? bwd<T, 96>(p, st) : bwd<T, 128>(p, st);
+template <typename T, bool BWD> int run_d(const AttnP& p, hipStream_t st) {
+  return p.d <= 32 ? run<T, 32, BWD>(p, st) : p.d <= 64 ? run<T, 64, BWD>(p, st) : p.d <= 96 ? run<T, 96, BWD>(p, st) : run<T, 128, BWD>(p, st);
+}
+template <bool BWD> int run_t(const AttnP& p, int dtype, hipStream_t st) {
+  return dtype == OP_F32 ? run_d<float, BWD>(p, st) : dtype == OP_BF16 ? run_d<__bf16, BWD>(p, st) : run_d<_Float16, BWD>(p, st);
 }
 
 }  // namespace
 
-int attention_parts(long long rows, int nseq, int heads, int kv_heads, int d) {
-  static const char* e = getenv("PARTS");
-  if (e) return atoi(e);
-  return 1;
+// dk/dv: parts until there is a workgroup per compute unit, and four where the walks are causal and long; a part keeps at
+// least 256 queries (fp32 128).  Whole backward pass, us, 1 / 2 / 4 parts:
+//   fp32 D 64: 16 x 1024 tokens x 1 head 251 / 197 / 197;  4 x 1024 x 8: 264 / 264 / 275;  1 x 4096 x 8 causal 912 / 888 / 775
+//   bf16 D 64: 1 x 4096 x 2: 140 / 108 / 95;  16 x 1024 x 4: 76 / 100 / 127;  the packed clips' dk/dv (12 of 4 heads) 300 / 203
+int attention_parts(int dtype, long long rows, int nseq, int heads, int kv_heads, int block) {
+  if (nseq < 1) return 1;
+  const long long blocks = (rows / 128 + nseq) * kv_heads, walk = rows / nseq * (heads / kv_heads);
+  long long parts = ((block && walk >= 4096 ? 1024 : 256) + blocks - 1) / blocks;
+  const long long most = walk / (dtype == OP_F32 ? 128 : 256);
+  if (parts > most) parts = most;
+  return parts < 1 ? 1 : parts > 8 ? 8 : (int)parts;
 }
-int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st) {
-  return dtype == OP_F32 ? fwd_d<float>(p, st) : dtype == OP_BF16 ? fwd_d<__bf16>(p, st) : fwd_d<_Float16>(p, st);
-}
-int launch_attention_bwd(const AttnP& p, int dtype, hipStream_t st) {
-  return dtype == OP_F32 ? bwd_d<float>(p, st) : dtype == OP_BF16 ? bwd_d<__bf16>(p, st) : bwd_d<_Float16>(p, st);
-}
+int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st) { return run_t<false>(p, dtype, st); }
+int launch_attention_bwd(const AttnP& p, int dtype, hipStream_t st) { return run_t<true>(p, dtype, st); }

@@ -28,11 +28,11 @@ __device__ __forceinline__ void turn_cs(double turns, float sign, float& c, floa
 template <typename T, int V> struct VecOf { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct VecOf<T, 1> { struct type { T v; __device__ T& operator[](int) { return v; } }; };
 
-// MODE 0: one pair (or one passed channel) a thread, any layout; 1: 16 bytes of neighbouring pairs; 2: two 16-byte pieces,
-// the first and second channels of V pairs
-template <typename T, int MODE>
+// INTER: V neighbouring channels (V / 2 pairs, V even) a thread; else V first and the V second channels of V pairs.  V = 1
+// takes any layout.
+template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const int units, const int hchunk) {
-  constexpr int V = MODE == 0 ? 1 : 16 / (int)sizeof(T), NPAIR = MODE == 1 ? V / 2 : V;
+  constexpr int MODE = INTER ? 1 : 2, NPAIR = INTER ? V / 2 : V;
   typedef typename VecOf<T, V>::type vec;
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / units;
   if (row >= p.rows) return;
@@ -79,28 +79,36 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const int 
   }
 }
 
-template <typename T> int run(const RotaryP& p, hipStream_t st) {
-  constexpr int V = 16 / (int)sizeof(T);
-  // 16-byte pieces where every address is a multiple of 16 and no piece crosses the border between turning and passing
-  // channels (halves: between an axis' halves)
-  bool vec = p.d % V == 0 && 2 * p.pairs % V == 0 && ((uintptr_t)p.x | (uintptr_t)p.y) % 16 == 0 &&
-             p.xr % V == 0 && p.xh % V == 0 && p.yr % V == 0 && p.yh % V == 0;
-  if (!p.interleaved)
-    for (int i = 0; i < p.pairs && vec; i += V)
-      vec = p.pairs % V == 0 && p.c0[i] % V == 0 && p.c1[i] % V == 0 && p.c0[i + V - 1] == p.c0[i] + V - 1 && p.axis[i + V - 1] == p.axis[i];
-  const int mode = !vec ? 0 : p.interleaved ? 1 : 2;
-  const int rest = p.copy ? p.d - 2 * p.pairs : 0;
-  const int units = mode == 0 ? p.pairs + rest : mode == 1 ? (2 * p.pairs + rest) / V : (p.pairs + rest) / V;
-  const long long threads = p.rows * units, blocks = (threads + 255) / 256;
+// vectors of V channels fit: every address is a multiple of their size, and none crosses the border between turning and
+// passing channels (halves: between an axis' halves)
+template <typename T> bool fits(const RotaryP& p, int v) {
+  if (p.interleaved && v < 2) return false;
+  const int bytes = v * (int)sizeof(T);
+  if (p.d % v || 2 * p.pairs % v || ((uintptr_t)p.x | (uintptr_t)p.y) % bytes || p.xr % v || p.xh % v || p.yr % v || p.yh % v) return false;
+  if (p.interleaved) return true;
+  if (p.pairs % v) return false;
+  for (int i = 0; i < p.pairs; i += v)
+    if (p.c0[i] % v || p.c1[i] % v || p.c0[i + v - 1] != p.c0[i] + v - 1 || p.axis[i + v - 1] != p.axis[i]) return false;
+  return true;
+}
+template <typename T, int V, bool INTER> int go(const RotaryP& p, hipStream_t st) {
+  const int rest = p.copy ? p.d - 2 * p.pairs : 0, units = ((INTER ? 2 * p.pairs : p.pairs) + rest) / V;
+  const long long blocks = (p.rows * units + 255) / 256;
   // few rows: the heads are split over the grid until there are about four workgroups per compute unit
   int split = 1;
   while (split < p.heads && blocks * split < 1024) split *= 2;
   const int hchunk = (p.heads + split - 1) / split;
-  const dim3 grid((unsigned)blocks, (unsigned)((p.heads + hchunk - 1) / hchunk));
-  if (mode == 0) rotary_kernel<T, 0><<<grid, 256, 0, st>>>(p, units, hchunk);
-  else if (mode == 1) rotary_kernel<T, 1><<<grid, 256, 0, st>>>(p, units, hchunk);
-  else rotary_kernel<T, 2><<<grid, 256, 0, st>>>(p, units, hchunk);
+  rotary_kernel<T, V, INTER><<<dim3((unsigned)blocks, (unsigned)((p.heads + hchunk - 1) / hchunk)), 256, 0, st>>>(p, units, hchunk);
   return hipGetLastError() != hipSuccess;
+}
+// the widest vectors that fit: 16, 8 or 4 bytes
+template <typename T> int run(const RotaryP& p, hipStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (fits<T>(p, V)) return p.interleaved ? go<T, V, true>(p, st) : go<T, V, false>(p, st);
+  if (fits<T>(p, V / 2)) return p.interleaved ? go<T, V / 2, true>(p, st) : go<T, V / 2, false>(p, st);
+  if constexpr (V == 8)
+    if (fits<T>(p, 2)) return p.interleaved ? go<T, 2, true>(p, st) : go<T, 2, false>(p, st);
+  return go<T, 1, false>(p, st);
 }
 
 }  // namespace

@@ -25,7 +25,7 @@ struct AttnP {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
   float* lse;                   // [heads, rows]
-  float* delta;                 // backward workspace [3, heads, rows]: -rowsum(dout out), -lse / scale, exponent of the row's scale (fp16)
+  float* delta;                 // backward workspace [3, heads, rows]: -rowsum(dout out), -lse (log2), exponent of the row's scale (fp16)
   float* partial;               // [parts, 2, rows, kv_heads, d]: dk and dv of each part, if parts > 1
   int parts;                    // ranges the queries of a key tile are cut into (attention_parts)
   const int* cu;                // [nseq + 1] first rows, or null: nseq sequences of seqlen rows each
@@ -34,7 +34,7 @@ struct AttnP {
   int nseq, seqlen, heads, kv_heads, d, block;   // block: causal block, 0 = bidirectional
   float scale;
 };
-int attention_parts(long long rows, int nseq, int heads, int kv_heads, int d);
+int attention_parts(int dtype, long long rows, int nseq, int heads, int kv_heads, int block);
 int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st);
 int launch_attention_bwd(const AttnP& p, int dtype, hipStream_t st);
 

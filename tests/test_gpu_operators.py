@@ -108,7 +108,7 @@ def test_rotary_no_rows():
 ATTN = [  # lens, tail, heads, kv_heads, head_dim, causal block
     ([1], 0, 1, 1, 16, 0), ([1, 0, 2, 0, 0, 1], 3, 2, 1, 32, 1), ([64], 0, 1, 1, 64, 0), ([65, 31, 128], 0, 2, 2, 64, 1),
     ([200], 5, 4, 2, 48, 0), ([129, 1, 257], 70, 6, 2, 128, 1), ([130, 300], 0, 3, 3, 80, 64), ([127, 128, 129], 0, 2, 1, 96, 5),
-    ([33, 500], 0, 4, 1, 24, 7), ([400], 0, 8, 8, 16, 196), ([0, 0, 90], 0, 2, 2, 8, 1), ([256], 0, 5, 5, 112, 1000), ([192], 1, 2, 1, 128, 0),
+    ([300] * 5 + [1, 260], 3, 12, 4, 48, 1), ([2100], 0, 2, 1, 64, 64), ([290, 300, 310], 0, 12, 6, 128, 0), ([33, 500], 0, 4, 1, 24, 7), ([400], 0, 8, 8, 16, 196), ([0, 0, 90], 0, 2, 2, 8, 1), ([256], 0, 5, 5, 112, 1000), ([192], 1, 2, 1, 128, 0),
 ]
 
 
