@@ -15,7 +15,7 @@
 // fp32 operands use v_mfma_f32_32x32x2_f32, 16-bit ones v_mfma_f32_32x32x16_*; a "chunk" is what one 16-byte register
 // piece per lane covers of the contraction: 8 channels in fp32, 16 in 16 bits.
 // All sums, statistics and accumulators are fp32.  The probabilities (and ds) of 16-bit operands are rounded to the
-// operands' type before their product, as the matrix unit takes them; their row sum is taken before that rounding.
+// operands' type before their product, as the matrix unit takes them; their row sum is taken before that rounding (lse is exact to fp32).
 //
 // No atomics: every output element is summed by one wave in a fixed order, so results repeat bit for bit.
 #include "op_tile.h"
@@ -338,10 +338,13 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     big = half_max(big);
     const int e = big > 0.f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
     dscale = __builtin_amdgcn_ldexpf(1.f, -e); back = __builtin_amdgcn_ldexpf(p.scale, e);
-    if (own && h == 0) p.delta[2 * plane + at] = big > 0.f ? (float)e : NO_EXP;
+    if (own && h == 0 && (!SPLIT || w == 0)) p.delta[2 * plane + at] = big > 0.f ? (float)e : NO_EXP;
   }
   const float lse2 = own ? p.lse[at] * CORA_LOG2E : 0.f, sl2 = p.scale * CORA_LOG2E;
-  if (own && h == 0) { p.delta[at] = -delta; p.delta[plane + at] = -lse2; }
+  // Where a wave sees one key tile only, delta is taken from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
+  // 16 bits, which delta otherwise inherits, counts most in rows that see few keys.
+  const bool whole = sizeof(T) == 2 && wave_end <= KT;
+  if (own && h == 0 && (!SPLIT || w == 0)) { if (!whole) p.delta[at] = -delta; p.delta[plane + at] = -lse2; }
 
   f32x16 acc[D / 32];
 #pragma unroll
@@ -358,6 +361,25 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     const int j0 = (SPLIT ? it * NW + w : it) * KT;
     if (j0 >= wave_end) return;
     k += mine; v += mine;
+    if (whole) {
+      float sum = 0.f;
+#pragma unroll 1
+      for (int t = 0; t < KT / 32; ++t) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s = O::mma(L::row_frag(k, 32 * t, c, lane), qf[c], s);
+          dp = O::mma(L::row_frag(v, 32 * t, c, lane), df[c], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * t + acc_row(r, h) < lim) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)), dp[r], sum);
+      }
+      delta = half_sum(sum);
+      if (own && h == 0) p.delta[at] = -delta;
+    }
 #pragma unroll
     for (int t = 0; t < KT / 32; ++t) {
       f32x16 s, dp;
