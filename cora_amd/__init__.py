@@ -9,7 +9,7 @@ from .model import (STATUS, STATUS_FORWARD, LayerParam, TransformerDecoder, Vode
 from .inference import calculate_psnr, extract_features_from_batch, make_mask, unmask_on_batch_enhanced
 from .loops import eval_pretext_metrics, train
 from .optim import (Optim, adamw, chain, clip_by_global_norm, create_learning_rate_schedule,
-                    make_optimizers, sgd)
+                    make_optimizers, muon, sgd)
 from .ops import attention, attention_backward, orthogonalize, rotary, rotary_backward
 from .serialisation import load_params, save_params
 
@@ -18,6 +18,6 @@ __all__ = [
     "transformer_config_from", "STATUS", "STATUS_FORWARD", "LayerParam", "TransformerDecoder",
     "VodeParam", "energy", "forward", "layer_energies", "step", "step_energies", "train_on_batch",
     "Optim", "adamw", "chain", "clip_by_global_norm", "create_learning_rate_schedule",
-    "make_optimizers", "sgd", "load_params", "save_params", "calculate_psnr", "extract_features_from_batch",
+    "make_optimizers", "muon", "sgd", "load_params", "save_params", "calculate_psnr", "extract_features_from_batch",
     "attention", "attention_backward", "orthogonalize", "rotary", "rotary_backward", "make_mask", "unmask_on_batch_enhanced", "eval_pretext_metrics", "train",
 ]

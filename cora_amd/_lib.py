@@ -33,6 +33,8 @@ def _struct(name: str, *fields):
     return type(name, (C.Structure,), {"_fields_": [(n, t) for t, names in fields for n in names.split()]})
 
 
+CoraAttnOptions = _struct("CoraAttnOptions", (C.c_int32, "n_axes"), (C.c_int32 * 4, "axes_dim"), (C.c_int32, "causal_block"),
+                          (C.c_double, "theta"))
 CoraRotaryArgs = _struct(
     "CoraRotaryArgs", (C.c_int32, "dtype heads head_dim n_axes"), (C.c_int32 * 4, "axes_dim"),
     (C.c_int32, "interleaved backward"), (C.c_double, "theta"), (C.c_int64, "rows pos_rows"), (C.c_void_p, "pos x y"),
@@ -53,6 +55,7 @@ _DP = C.POINTER(C.c_double)
 _SZ = C.c_size_t
 SIGNATURES = {
     "cora_create": (C.c_int, [C.POINTER(CoraConfig), C.c_int, C.POINTER(_P)]),
+    "cora_create_attn": (C.c_int, [C.POINTER(CoraConfig), C.POINTER(CoraAttnOptions), C.c_int, C.POINTER(_P)]),
     "cora_destroy": (C.c_int, [_P]),
     "cora_last_error": (C.c_char_p, [_P]),
     "cora_weights_size": (C.c_int, [_P, C.POINTER(_SZ)]),
@@ -68,6 +71,7 @@ SIGNATURES = {
     "cora_set_adam_state": (C.c_int, [_P, _P, _P, C.c_int64]),
     "cora_get_adam_state": (C.c_int, [_P, _P, _P, C.POINTER(C.c_int64)]),
     "cora_set_optim": (C.c_int, [_P] + [C.c_float] * 7),
+    "cora_set_muon": (C.c_int, [_P, C.c_int, C.c_float, C.c_int, C.c_float, C.c_int, _P, C.c_float]),
     "cora_step": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, C.c_float, C.POINTER(CoraStepOut)]),
     "cora_infer": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, C.POINTER(CoraStepOut)]),
     "cora_set_grad_options": (C.c_int, [_P, C.c_int, C.c_float, C.c_int, C.c_float]),

@@ -50,6 +50,11 @@ class TransformerConfig:
     vode_grad_norm_target: float = 1.0
     intermediate_l1_coeff: float = 0.0
     intermediate_l2_coeff: float = 0.0
+    # Not in the reference.  "rotary": queries and keys are turned by the patch's row and column (clips: frame, row, column),
+    # axes_dim channels of every head each, base theta, instead of the additive table.
+    pos_encoding: str = "sinusoidal"
+    # Not in the reference.  Clips: a patch sees the patches of its own and of earlier frames only.
+    causal_frames: bool = False
 
     def __post_init__(self):
         self.image_shape = tuple(self.image_shape)
@@ -64,6 +69,17 @@ class TransformerConfig:
         if not self.is_video and len(self.axes_dim) == 3:
             self.axes_dim = self.axes_dim[1:]
         self.mlp_hidden_dim = int(self.hidden_size * self.mlp_ratio)
+        if self.pos_encoding not in ("sinusoidal", "rotary"):
+            raise ValueError("pos_encoding must be 'sinusoidal' or 'rotary'")
+        if self.pos_encoding == "rotary":
+            n = 3 if self.is_video else 2
+            if len(self.axes_dim) != n or any(a < 2 or a % 2 for a in self.axes_dim):
+                raise ValueError(f"rotary positions need {n} positive, even axes_dim, got {self.axes_dim}")
+            if sum(self.axes_dim) > self.hidden_size // self.num_heads:
+                raise ValueError(f"axes_dim {self.axes_dim} take more channels than a head has "
+                                 f"({self.hidden_size // self.num_heads})")
+        if self.causal_frames and not self.is_video:
+            raise ValueError("causal_frames needs clips (is_video)")
 
 
 @dataclass
@@ -144,6 +160,10 @@ class ModelConfig:
     linear_probe_seed: int = 123
     intermediate_l1_coeff: float = 0.0
     intermediate_l2_coeff: float = 0.0
+    # not in the reference: see TransformerConfig and optim.muon
+    pos_encoding: str = "sinusoidal"
+    causal_frames: bool = False
+    use_muon_for_weight_optimizer: bool = False
 
 
 def _nblock(name: str, num_blocks: int, **over) -> ModelConfig:
@@ -224,10 +244,11 @@ def create_config(dataset="cifar10", hidden_size=48, num_blocks=1, num_heads=6, 
                   use_vode_state_layernorm: bool = False, use_vode_grad_norm: bool = False,
                   vode_grad_norm_target: float = 1.0, hidden_momentum: float = 0.1,
                   intermediate_l1_coeff: float = 0.0, intermediate_l2_coeff: float = 0.0,
-                  image_shape=None) -> TransformerConfig:
+                  image_shape=None, pos_encoding: str = "sinusoidal", causal_frames: bool = False) -> TransformerConfig:
     """Same signature and behaviour as src/config.py:524-569 (`hidden_momentum` is accepted and
     ignored there too).  Extension: `image_shape` lets the synthetic datasets of BASELINE.json
-    (imagenet / video) through; the reference raises ValueError for anything but cifar10."""
+    (imagenet / video) through; the reference raises ValueError for anything but cifar10.  `pos_encoding` and
+    `causal_frames` are passed on to TransformerConfig."""
     axes_dim = axes_dim or [16, 16]
     if dataset == "cifar10":
         shape = (3, 32, 32)
@@ -249,7 +270,8 @@ def create_config(dataset="cifar10", hidden_size=48, num_blocks=1, num_heads=6, 
         update_weights_every_inference_step=update_weights_every_inference_step,
         use_vode_state_layernorm=use_vode_state_layernorm, use_vode_grad_norm=use_vode_grad_norm,
         vode_grad_norm_target=vode_grad_norm_target,
-        intermediate_l1_coeff=intermediate_l1_coeff, intermediate_l2_coeff=intermediate_l2_coeff)
+        intermediate_l1_coeff=intermediate_l1_coeff, intermediate_l2_coeff=intermediate_l2_coeff,
+        pos_encoding=pos_encoding, causal_frames=causal_frames)
 
 
 def transformer_config_from(mc: ModelConfig) -> TransformerConfig:
@@ -271,4 +293,5 @@ def transformer_config_from(mc: ModelConfig) -> TransformerConfig:
         use_vode_state_layernorm=mc.use_vode_state_layernorm,
         use_vode_grad_norm=mc.use_vode_grad_norm, vode_grad_norm_target=mc.vode_grad_norm_target,
         intermediate_l1_coeff=mc.intermediate_l1_coeff,
-        intermediate_l2_coeff=mc.intermediate_l2_coeff)
+        intermediate_l2_coeff=mc.intermediate_l2_coeff,
+        pos_encoding=mc.pos_encoding, causal_frames=mc.causal_frames)

@@ -4,6 +4,7 @@
 // Step order follows train_on_batch, /root/reference/src/decoder_transformer.py:392-499 (mode 2).
 #include "../../include/cora_hip.h"
 #include "common.h"
+#include "ops.h"
 
 #include <rccl/rccl.h>
 #include <dlfcn.h>
@@ -130,6 +131,17 @@ struct cora_ctx {
   // and the one GEMM that reads them (da: gelu' epilogue -> W1^T GEMM; dqkv: attention backward -> Wqkv^T GEMM).  The
   // consumer rounds its A operand to bf16 anyway, so results are bit-identical; the learning pass keeps fp32.
   bool da16 = false, dqkv16 = false;
+  // attention options (cora_create_attn): rotary positions on queries and keys, frame-causal attention (per-op kernels)
+  cora_attn_options opt = {};
+  RotaryP rot = {};          // rows, pointers and sign are set per launch
+  int* rpos = nullptr;       // [N, n_axes]
+  void* aws = nullptr;       // workspace of the causal attention's backward pass
+  // orthogonalised-momentum weight step (cora_set_muon)
+  bool muon = false;
+  float muon_beta = 0.f, muon_wd = 0.f, muon_eps = 0.f, muon_coef[3 * ORTHO_STEPS] = {};
+  int muon_nesterov = 0, muon_steps = 0;
+  float* mbuf = nullptr;     // updates of the blocks' matrices: W1 and what lies before it from oWqkv, then W2
+  void* mws = nullptr;
   bool slotted() const { return fused || fusedw; }   // inference-step energies kept as 8 partial sums per vode (esum)
 
   // vodes
@@ -349,12 +361,69 @@ void out_proj(cora_ctx* c, const float* hin, float* out, int mode, const float* 
   run_gemm(c, p, false, false);
 }
 
+// parameter block of the frame-causal attention on the ctx's q | k | v scratch
+void fill_causal(cora_ctx* c, AttnP& p, int nseq) {
+  memset(&p, 0, sizeof p);
+  const int D = c->D, dh = D / c->H;
+  p.q = c->qkv; p.k = c->qkv + D; p.v = c->qkv + 2 * D; p.out = c->att; p.o = c->att; p.dout = c->dO; p.lse = c->lse;
+  p.dq = c->dqkv; p.dk = c->dqkv + D; p.dv = c->dqkv + 2 * D;
+  p.rows = (long long)nseq * c->N; p.nseq = nseq; p.seqlen = c->N;
+  p.heads = p.kv_heads = c->H; p.d = dh; p.block = c->opt.causal_block; p.scale = 1.f / sqrtf((float)dh);
+  p.qr = p.kr = p.vr = p.dqr = p.dkr = p.dvr = 3 * D;
+  p.orow = p.dor = D;
+  p.qh = p.kh = p.vh = p.dqh = p.dkh = p.dvh = p.oh = p.doh = dh;
+  if (c->aws) attention_ws(p, OP_F32, c->aws);
+}
+// Attention of nseq sequences of N tokens, q | k | v rows in c->qkv (turned first, if the ctx has rotary positions) -> c->att, c->lse
+int attention_forward(cora_ctx* c, int nseq) {
+  const int D = c->D, H = c->H;
+  const long long rows = (long long)nseq * c->N;
+  if (c->opt.n_axes) {
+    KScope s(c, K_OTHER, 0, 16.0 * rows * D);
+    RotaryP r = c->rot;
+    r.x = c->qkv; r.y = c->qkv; r.rows = rows; r.sign = 1.f;
+    if (launch_rotary(r, OP_F32, c->st)) FAIL(-3, "rotary positions: launch failed");
+  }
+  KScope s(c, K_ATTN_FWD, 4.0 * rows * (double)c->N * D, 4.0 * rows * 4 * D);
+  if (c->opt.causal_block) {
+    AttnP p; fill_causal(c, p, nseq);
+    if (launch_attention_fwd(p, OP_F32, c->st)) FAIL(-3, "causal attention: launch failed");
+  } else if (c->cfg.dtype_mode == 1 && attn_fwd_bf16_supported(c->N, H, D)) {
+    if (launch_attn_fwd_bf16(c->qkv, c->att, c->lse, nseq, c->N, H, D, c->st)) FAIL(-3, "attention (bf16): launch set-up failed");
+  } else if (launch_attn_fwd(c->qkv, c->att, c->lse, nseq, c->N, H, D, c->st)) FAIL(-3, "attention: head dim not supported (need 16,24,32,48,64,96,128)");
+  return 0;
+}
+// its backward pass: c->dO -> c->dqkv, with respect to the projections' outputs (dq16: as bf16, bf16 kernels only)
+int attention_backward(cora_ctx* c, int nseq, bool dq16) {
+  const int D = c->D, H = c->H;
+  const long long rows = (long long)nseq * c->N;
+  {
+    KScope s(c, K_ATTN_BWD, 14.0 * rows * (double)c->N * D, 4.0 * rows * 9 * D);   // 7 products (S and dP are recomputed per side)
+    if (c->opt.causal_block) {
+      AttnP p; fill_causal(c, p, nseq);
+      if (launch_attention_bwd(p, OP_F32, c->st)) FAIL(-3, "causal attention backward: launch failed");
+    } else if (c->cfg.dtype_mode == 1 && attn_bwd_bf16_supported(c->N, H, D)) {
+      if (launch_attn_bwd_bf16(c->qkv, c->att, c->lse, c->dO, c->delta, c->dqkv, nseq, c->N, H, D, c->st, dq16)) FAIL(-3, "attention backward (bf16): launch set-up failed");
+    } else {
+      if (dq16) FAIL(-3, "attention backward: bf16 scratch without the bf16 kernels");
+      if (launch_attn_bwd(c->qkv, c->att, c->lse, c->dO, c->delta, c->dqkv, nseq, c->N, H, D, c->st)) FAIL(-3, "attention backward: head dim not supported");
+    }
+  }
+  if (c->opt.n_axes) {
+    KScope s(c, K_OTHER, 0, 16.0 * rows * D);
+    RotaryP r = c->rot;
+    r.x = c->dqkv; r.y = c->dqkv; r.rows = rows; r.sign = -1.f;
+    if (launch_rotary(r, OP_F32, c->st)) FAIL(-3, "rotary positions (backward): launch failed");
+  }
+  return 0;
+}
+
 // Forward of G transformer blocks (blocks b0..b0+G-1), block g reading xin + g*BN*D:
 //   u = 2x + MHA(LN1 x) + MLP(LN2(x + MHA(LN1 x)))   (pcx/nn/_layer.py:428-447 + decoder :238)
 // mode OUT_ERR : C = tgt - u written to `out` (errors), energies accumulated at red[g]
 // mode OUT_STORE: C = u
 int block_forward(cora_ctx* c, int G, int b0, const float* xin, float* out, int mode, const float* tgt, double* red) {
-  const int D = c->D, M = c->M, H = c->H;
+  const int D = c->D, M = c->M;
   const int R = (int)c->BN;
   const long long rows = (long long)G * R;
   {
@@ -369,13 +438,7 @@ int block_forward(cora_ctx* c, int G, int b0, const float* xin, float* out, int 
   p.R = R; p.O = 3 * D; p.K = D; p.lda = D; p.ldb = D; p.ldc = 3 * D;
   p.sA = (long long)R * D; p.sB = 3LL * D * D; p.sC = (long long)R * 3 * D;
   run_gemm(c, p, false, false);
-  {
-    double fl = 4.0 * G * c->B * (double)c->N * c->N * D;
-    KScope s(c, K_ATTN_FWD, fl, 4.0 * rows * 4 * D);
-    if (c->cfg.dtype_mode == 1 && attn_fwd_bf16_supported(c->N, H, D)) {
-      if (launch_attn_fwd_bf16(c->qkv, c->att, c->lse, G * c->B, c->N, H, D, c->st)) FAIL(-3, "attention (bf16): launch set-up failed");
-    } else if (launch_attn_fwd(c->qkv, c->att, c->lse, G * c->B, c->N, H, D, c->st)) FAIL(-3, "attention: head dim not supported (need 16,24,32,48,64,96,128)");
-  }
+  if (int rc = attention_forward(c, G * c->B)) return rc;
   // y = x + att Wo^T
   p = gemm_base(c); p.groups = G;
   p.A = c->att; p.Bw = c->W + c->oWo + (size_t)b0 * D * D; p.C = c->y;
@@ -413,7 +476,7 @@ int block_forward(cora_ctx* c, int G, int b0, const float* xin, float* out, int 
 int block_backward(cora_ctx* c, int G, int b0, const float* xin, const float* r, const float* own, float* gout, double* red,
                    bool raw = false, bool half = false /* inference step: da / dqkv as bf16 where the ctx allows (da16, dqkv16) */) {
   const bool da16 = half && c->da16, dq16 = half && c->dqkv16;
-  const int D = c->D, M = c->M, H = c->H;
+  const int D = c->D, M = c->M;
   const int R = (int)c->BN;
   const long long rows = (long long)G * R;
   GemmP p = gemm_base(c, 1); p.groups = G;
@@ -442,16 +505,7 @@ int block_backward(cora_ctx* c, int G, int b0, const float* xin, const float* r,
   p.R = R; p.O = D; p.K = D; p.lda = D; p.ldc = D;
   p.sA = (long long)R * D; p.sB = (long long)D * D; p.sC = (long long)R * D;
   run_gemm(c, p, false, bwd_weight(c, p, c->oWo + (size_t)b0 * D * D, c->tWo + (size_t)b0 * D * D));
-  {
-    double fl = 14.0 * G * c->B * (double)c->N * c->N * D;   // 7 products (S and dP are recomputed per side)
-    KScope s(c, K_ATTN_BWD, fl, 4.0 * rows * 9 * D);
-    if (c->cfg.dtype_mode == 1 && attn_bwd_bf16_supported(c->N, H, D)) {
-      if (launch_attn_bwd_bf16(c->qkv, c->att, c->lse, c->dO, c->delta, c->dqkv, G * c->B, c->N, H, D, c->st, dq16)) FAIL(-3, "attention backward (bf16): launch set-up failed");
-    } else {
-      if (dq16) FAIL(-3, "attention backward: bf16 scratch without the bf16 kernels");
-      if (launch_attn_bwd(c->qkv, c->att, c->lse, c->dO, c->delta, c->dqkv, G * c->B, c->N, H, D, c->st)) FAIL(-3, "attention backward: head dim not supported");
-    }
-  }
+  if (int rc = attention_backward(c, G * c->B, dq16)) return rc;
   // dxn = dqkv Wqkv
   p = gemm_base(c, 1); p.groups = G;
   p.A = c->dqkv; p.C = c->dxn; p.a16 = dq16;
@@ -915,6 +969,35 @@ void wgrad_gemm(cora_ctx* c, int G, const float* A, int R, long long sA, const f
   run_gemm(c, p, true, true);
 }
 
+// the blocks' matrices as stacks of updates in c->mbuf
+void muon_stacks(const cora_ctx* c, OrthoP& p) {
+  memset(&p, 0, sizeof p);
+  const int D = c->D, M = c->M, L = c->L;
+  float* u = c->mbuf;
+  auto add = [&](size_t at, int count, int rows, int cols) { fill_stack(p, u + at, u + at, count, rows, cols); };
+  add(0, 3 * L, D, D); add(c->oWo - c->oWqkv, L, D, D); add(c->oW1 - c->oWqkv, L, M, D); add(c->ob1 - c->oWqkv, L, D, M);
+  p.eps = c->muon_eps;
+}
+int enqueue_muon(cora_ctx* c, float scale_by, const float* hyp) {
+  const size_t n1 = c->ob1 - c->oWqkv, n2 = c->ob2 - c->oW2;
+  KScope s(c, K_OTHER, 0, 32.0 * (n1 + n2));
+  MuonP m; memset(&m, 0, sizeof m);
+  m.sumsq = c->scal; m.gscale = scale_by; m.clip = c->cfg.clip_w; m.beta = c->muon_beta; m.nesterov = c->muon_nesterov;
+  m.hyp = hyp; m.wd = c->muon_wd;
+  auto range = [&](size_t at, size_t u, size_t n) { m.g = c->dW + at; m.mu = c->amu + at; m.w = c->W + at; m.u = c->mbuf + u; m.n = (long long)n; };
+  range(c->oWqkv, 0, n1); launch_muon_momentum(m, c->st);
+  range(c->oW2, n1, n2); launch_muon_momentum(m, c->st);
+  OrthoP p; muon_stacks(c, p);
+  ortho_ws_bytes(p);
+  ortho_place(p, c->mws);
+  if (launch_ortho(p, OP_F32, c->muon_steps, c->muon_coef, c->st)) FAIL(-3, "orthogonalisation: launch failed");
+  auto size = [](int rows, int cols) { return rows > cols ? sqrtf((float)rows / cols) : 1.f; };
+  m.size = 1.f; range(c->oWqkv, 0, c->oW1 - c->oWqkv); launch_muon_apply(m, c->st);
+  m.size = size(c->M, c->D); range(c->oW1, c->oW1 - c->oWqkv, c->ob1 - c->oW1); launch_muon_apply(m, c->st);
+  m.size = size(c->D, c->M); range(c->oW2, n1, n2); launch_muon_apply(m, c->st);
+  return 0;
+}
+
 }  // namespace
 
 // =================================================================================================
@@ -963,11 +1046,32 @@ static void layout_ctx(cora_ctx* c, const cora_config* cfg, int device) {
   c->nW = o;
 }
 
-int cora_create(const cora_config* cfg, int device, cora_ctx** out) {
+// what cora_create_attn checks beyond check_config: nullptr = fine
+static const char* check_attn(const cora_config* cfg, const cora_attn_options* o) {
+  if (o->causal_block < 0) return "causal_block is negative";
+  if (o->n_axes == 0) return nullptr;
+  if (o->n_axes != 2 && o->n_axes != 3) return "rotary positions: n_axes must be 2 (row, column) or 3 (frame, row, column)";
+  if (o->n_axes == 2 && cfg->F != 1) return "rotary positions: clips need 3 axes (frame, row, column)";
+  if (!(o->theta > 0.0) || !std::isfinite(o->theta)) return "rotary positions: theta must be positive and finite";
+  int sum = 0;
+  for (int i = 0; i < o->n_axes; ++i) {
+    if (o->axes_dim[i] < 2 || o->axes_dim[i] % 2 || o->axes_dim[i] > 128) return "rotary positions: axes_dim must be positive and even";
+    sum += o->axes_dim[i];
+  }
+  if (sum > cfg->D / cfg->H || sum > 128) return "rotary positions: axes_dim take more channels than a head has";
+  return nullptr;
+}
+
+int cora_create(const cora_config* cfg, int device, cora_ctx** out) { return cora_create_attn(cfg, nullptr, device, out); }
+
+int cora_create_attn(const cora_config* cfg, const cora_attn_options* opt, int device, cora_ctx** out) {
   if (!cfg || !out) { g_create_err = "null argument"; return -1; }
   *out = nullptr;
   auto bad = [&](const char* m) { g_create_err = m; return -1; };
   if (const char* e = check_config(cfg)) return bad(e);
+  if (opt)
+    if (const char* e = check_attn(cfg, opt)) return bad(e);
+  const bool plain_attn = !opt || (!opt->n_axes && !opt->causal_block);   // what the fused kernels compute
   int ndev = 0;
   if (hipGetDeviceCount(&ndev) != hipSuccess || ndev < 1) return bad("no HIP device visible");
   if (device < 0 || device >= ndev) return bad("device index out of range");
@@ -982,11 +1086,12 @@ int cora_create(const cora_config* cfg, int device, cora_ctx** out) {
   const size_t D = c->D, P = c->P, M = c->M, L = c->L;
 
   int rc = 0;
+  float* tmp_opt = nullptr;
 #define DA(ptr, n) if ((rc = dalloc(c, &(ptr), (long long)(n)))) return fail(rc)
   DA(c->W, c->nW); DA(c->dW, c->nW); DA(c->amu, c->nW); DA(c->anu, c->nW);
   DA(c->pos, (long long)c->N * D);
-  c->fused = (c->N == 64 && c->D == 64 && (c->H == 1 || c->H == 2 || c->H == 4) && c->M == 256 && c->P == 48 && c->L > 0 && cfg->dtype_mode == 0 && !c->vln && getenv("CORA_NO_FUSED") == nullptr);
-  c->fusedw = (!c->fused && c->L > 0 && cfg->dtype_mode == 0 && !c->vln && fused_wide_supported(c->N, c->P, c->D, c->H, c->M) &&
+  c->fused = (c->N == 64 && c->D == 64 && (c->H == 1 || c->H == 2 || c->H == 4) && c->M == 256 && c->P == 48 && c->L > 0 && cfg->dtype_mode == 0 && !c->vln && plain_attn && getenv("CORA_NO_FUSED") == nullptr);
+  c->fusedw = (!c->fused && c->L > 0 && cfg->dtype_mode == 0 && !c->vln && plain_attn && fused_wide_supported(c->N, c->P, c->D, c->H, c->M) &&
                getenv("CORA_NO_FUSED") == nullptr);
   c->fusedw2 = c->fusedw && fused_wide2_supported(c->N, c->P, c->D, c->H, c->M) && getenv("CORA_WIDE1") == nullptr;
   // bf16 mode (dtype_mode 1) takes the row kernels too where its bf16-MFMA attention applies (sequences longer than one
@@ -994,7 +1099,7 @@ int cora_create(const cora_config* cfg, int device, cora_ctx** out) {
   // D = 64 faster than the per-op bf16 GEMMs they replace -- with the bf16 attention kernels between them
   const bool rows_dtype = cfg->dtype_mode == 0 ||
                           (cfg->dtype_mode == 1 && attn_fwd_bf16_supported(c->N, c->H, c->D) && attn_bwd_bf16_supported(c->N, c->H, c->D));
-  c->frows = (!c->fused && !c->fusedw && c->L > 0 && rows_dtype && !c->vln && fused_rows_supported(c->BN, c->D, c->M) &&
+  c->frows = (!c->fused && !c->fusedw && c->L > 0 && rows_dtype && !c->vln && plain_attn && fused_rows_supported(c->BN, c->D, c->M) &&
               getenv("CORA_NO_FUSED") == nullptr && getenv("CORA_NO_ROWS") == nullptr);
   c->frows_bwd1 = c->frows && cfg->dtype_mode == 0 && (c->H == 1 || c->H == 2 || c->H == 4) &&
                   attn_bwd_fused_supported(c->N, c->H, c->D) && getenv("CORA_ATTN_BWD2") == nullptr;
@@ -1017,7 +1122,7 @@ int cora_create(const cora_config* cfg, int device, cora_ctx** out) {
     }
     if (cfg->dtype_mode == 1 && c->WTh && L > 0 && !getenv("CORA_NO_BWD16") && !getenv("CORA_BF16_NO_PRE") && !getenv("CORA_BF16_INREG")) {
       c->da16 = (M % 8 == 0);
-      c->dqkv16 = ((3 * D) % 8 == 0) && attn_bwd_bf16_supported(c->N, c->H, c->D);
+      c->dqkv16 = ((3 * D) % 8 == 0) && plain_attn && attn_bwd_bf16_supported(c->N, c->H, c->D);
     }
     if (c->fused) DA(c->colpart, (long long)fused_colpart_floats(L, c->B));
     if (c->frows) DA(c->colpart, (long long)fused_rows_colpart_floats((int)L, c->BN));
@@ -1041,6 +1146,26 @@ int cora_create(const cora_config* cfg, int device, cora_ctx** out) {
   DA(c->ua, c->nl); DA(c->ub, c->nl); DA(c->z, c->n0);
   if (c->fused) DA(c->stash, rows * c->H * D);
   if (c->fusedw) DA(c->stash, rows * (c->H * 64 + 3 * D));   // per token row: one 64-key row of P per head, then q (| k | v: two-workgroup form)
+  if (opt) c->opt = *opt;
+  if (c->opt.n_axes) {
+    const int n = c->opt.n_axes, wp = cfg->Wimg / cfg->patch, hp = cfg->Himg / cfg->patch;
+    std::vector<int> pos((size_t)c->N * n);
+    for (int t = 0; t < c->N; ++t) {
+      const int grid[3] = {t / (hp * wp), t / wp % hp, t % wp};
+      for (int a = 0; a < n; ++a) pos[(size_t)t * n + a] = grid[3 - n + a];
+    }
+    DA(tmp_opt, (long long)pos.size()); c->rpos = (int*)tmp_opt;
+    if (hipMemcpyAsync(c->rpos, pos.data(), pos.size() * sizeof(int), hipMemcpyHostToDevice, c->st) != hipSuccess ||
+        hipStreamSynchronize(c->st) != hipSuccess) { c->err = "upload of the positions failed"; return fail(-2); }
+    RotaryP& r = c->rot;
+    fill_rotary(r, n, c->opt.axes_dim, c->opt.theta, true);
+    r.pos = c->rpos; r.pos_rows = c->N; r.heads = 2 * c->H; r.d = c->D / c->H;     // q | k heads of a q | k | v row, in place
+    r.xr = r.yr = 3 * c->D; r.xh = r.yh = r.d; r.copy = 0;
+  }
+  if (c->opt.causal_block) {
+    const size_t ws = attention_ws_bytes(OP_F32, rows, c->Gmax * c->B, c->H, c->H, c->D / c->H, c->opt.causal_block);
+    DA(tmp_opt, (long long)(ws / sizeof(float) + 4)); c->aws = tmp_opt;
+  }
   DA(c->gscale, 64); DA(c->eta_dev, c->Tmax + 1);
   float* tmp = nullptr;
   DA(tmp, 2LL * (c->Tmax + 2) * (L + 3)); c->energies = (double*)tmp;
@@ -1273,6 +1398,39 @@ int cora_set_optim(cora_ctx* c, float clip_h, float momentum, float clip_w, floa
   return 0;
 }
 
+int cora_set_muon(cora_ctx* c, int enabled, float beta, int nesterov, float wd, int steps, const float* coef, float eps) {
+  if (!c) return -1;
+  if (enabled) {
+    if (!(beta >= 0.f && beta < 1.f)) FAIL(-1, "muon: beta must lie in [0, 1)");
+    if (!std::isfinite(wd) || !std::isfinite(eps) || eps < 0.f) FAIL(-1, "muon: weight decay must be finite, eps finite and not negative");
+    if (steps < 1 || steps > ORTHO_STEPS || !coef) FAIL(-1, "muon: steps must be 1 .. 32, coef not NULL");
+    if (ortho_bad_step(steps, coef) >= 0) FAIL(-1, "muon: the coefficients drive singular values of [0, 1] out of range");
+    if (c->M > 32768 || 3 * c->L > 65535) FAIL(-1, "muon: matrices too large");
+  }
+  const bool on = enabled && c->L > 0;       // without blocks there is no matrix to step
+  if (on == c->muon && (!on || (beta == c->muon_beta && (nesterov != 0) == (c->muon_nesterov != 0) && wd == c->muon_wd &&
+      steps == c->muon_steps && eps == c->muon_eps && !memcmp(coef, c->muon_coef, sizeof(float) * 3 * steps)))) return 0;
+  HCHECK(hipSetDevice(c->device));
+  if (int rc_ = settle_pending(c)) return rc_;
+  drop_learn_graphs(c);
+  HCHECK(hipStreamSynchronize(c->st));
+  if (on && !c->mbuf) {
+    if (int rc = dalloc(c, &c->mbuf, (long long)((c->ob1 - c->oWqkv) + (c->ob2 - c->oW2)))) return rc;
+    OrthoP p; muon_stacks(c, p);
+    float* w = nullptr;
+    if (int rc = dalloc(c, &w, (long long)(ortho_ws_bytes(p) / sizeof(float) + 64))) return rc;
+    c->mws = w;
+    HCHECK(hipStreamSynchronize(c->st));
+  }
+  c->muon = on;
+  if (on) {
+    c->muon_beta = beta; c->muon_nesterov = nesterov != 0; c->muon_wd = wd; c->muon_steps = steps; c->muon_eps = eps;
+    memcpy(c->muon_coef, coef, sizeof(float) * 3 * steps);
+  }
+  c->learn_warm = c->dist_warm = false;      // the next weight step runs eagerly once before it is captured
+  return 0;
+}
+
 int cora_set_grad_options(cora_ctx* c, int use_scaling, float scale_base, int use_grad_norm, float grad_norm_target) {
   if (!c) return -1;
   cora_config& f = c->cfg;
@@ -1431,17 +1589,26 @@ int enqueue_wgrad(cora_ctx* c) {
   return 0;
 }
 
-// clip + AdamW on dW (scaled by scale_by), transposes for the fused kernel, reconstruction with the
+// clip + AdamW (and orthogonalised momentum, cora_set_muon) on dW (scaled by scale_by), transposes for the fused kernel, reconstruction with the
 // updated weights and its clipped MSE (:484-494).  eta_w and the bias corrections come from
 // c->hyp_dev so the sequence can sit in a captured graph.  No synchronisation.
 int enqueue_adamw(cora_ctx* c, float scale_by, const float* hyp) {
   launch_zero(c->scal, 32, c->st);
   { KScope s(c, K_OTHER, 0, 4.0 * c->nW); launch_sumsq(c->dW, (long long)c->nW, scale_by, c->scal, c->st); }
   AdamP a; memset(&a, 0, sizeof a);
-  a.w = c->W; a.g = c->dW; a.mu = c->amu; a.nu = c->anu; a.n = (long long)c->nW; a.sumsq = c->scal;
-  a.gscale = scale_by; a.clip = c->cfg.clip_w; a.b1 = c->cfg.adam_b1; a.b2 = c->cfg.adam_b2;
+  a.sumsq = c->scal; a.gscale = scale_by; a.clip = c->cfg.clip_w; a.b1 = c->cfg.adam_b1; a.b2 = c->cfg.adam_b2;
   a.eps = c->cfg.adam_eps; a.wd = c->cfg.adam_wd; a.hyp = hyp;
-  { KScope s(c, K_OTHER, 0, 28.0 * c->nW); launch_adamw(a, c->st); }
+  auto adamw = [&](size_t from, size_t to) {
+    if (from >= to) return;
+    KScope s(c, K_OTHER, 0, 28.0 * (to - from));
+    a.w = c->W + from; a.g = c->dW + from; a.mu = c->amu + from; a.nu = c->anu + from; a.n = (long long)(to - from);
+    launch_adamw(a, c->st);
+  };
+  if (!c->muon) adamw(0, c->nW);
+  else {   // the arena: .. | Wqkv Wo W1 | b1 | W2 | .., the matrices by orthogonalised momentum
+    adamw(0, c->oWqkv); adamw(c->ob1, c->oW2); adamw(c->ob2, c->nW);
+    if (int rc = enqueue_muon(c, scale_by, hyp)) return rc;
+  }
   refresh_wt(c);
   return 0;
 }

@@ -85,16 +85,25 @@ int check_attention(const cora_attention_args* a, AttnP* p, const char* who, boo
   }
   memset(p, 0, sizeof *p);
   p->q = a->q; p->k = a->k; p->v = a->v; p->out = a->out; p->o = a->out; p->lse = a->lse;
-  p->dout = a->dout; p->dq = a->dq; p->dk = a->dk; p->dv = a->dv; p->delta = (float*)a->workspace; p->cu = a->cu_seqlens;
-  p->parts = backward ? attention_parts(a->dtype, a->rows, a->n_seq, a->heads, a->kv_heads, a->causal_block) : 1;
-  p->partial = (float*)((char*)a->workspace + ((size_t)a->heads * (size_t)a->rows * 3 * sizeof(float) + 15) / 16 * 16);
+  p->dout = a->dout; p->dq = a->dq; p->dk = a->dk; p->dv = a->dv; p->cu = a->cu_seqlens;
   p->rows = a->rows;
   p->qr = a->q_row; p->qh = a->q_head; p->kr = a->k_row; p->kh = a->k_head; p->vr = a->v_row; p->vh = a->v_head;
   p->orow = a->out_row; p->oh = a->out_head; p->dor = a->dout_row; p->doh = a->dout_head;
   p->dqr = a->dq_row; p->dqh = a->dq_head; p->dkr = a->dk_row; p->dkh = a->dk_head; p->dvr = a->dv_row; p->dvh = a->dv_head;
   p->nseq = a->n_seq; p->seqlen = a->seq_len; p->heads = a->heads; p->kv_heads = a->kv_heads; p->d = a->head_dim;
   p->block = a->causal_block; p->scale = a->scale;
+  if (backward) attention_ws(*p, a->dtype, a->workspace);
   return 0;
+}
+
+OrthoG& add_stack(OrthoP& p, int count, int rows, int cols) {
+  OrthoG& g = p.g[p.ngroups++];
+  g.count = count; g.rows = rows; g.cols = cols;
+  g.m = rows < cols ? rows : cols; g.n = rows < cols ? cols : rows;
+  g.ldn = (g.n + 63) / 64 * 64; g.ldm = (g.m + 63) / 64 * 64;
+  g.first = p.matrices;
+  p.matrices += count;
+  return g;
 }
 
 // up to ORTHO_GROUPS stacks from stacks[i0]; returns how many were taken
@@ -105,13 +114,8 @@ int take_stacks(const cora_matrices* stacks, int i0, int n, OrthoP* p) {
     const cora_matrices& s = stacks[i];
     if (s.count == 0) continue;
     if (p->matrices + s.count > 65535) break;
-    OrthoG& g = p->g[p->ngroups++];
+    OrthoG& g = add_stack(*p, s.count, s.rows, s.cols);
     g.x = s.x; g.y = s.y; g.xm = s.x_mat; g.xr = s.x_row; g.ym = s.y_mat; g.yr = s.y_row;
-    g.count = s.count; g.rows = s.rows; g.cols = s.cols;
-    g.m = s.rows < s.cols ? s.rows : s.cols; g.n = s.rows < s.cols ? s.cols : s.rows;
-    g.ldn = (g.n + 63) / 64 * 64; g.ldm = (g.m + 63) / 64 * 64;
-    g.first = p->matrices;
-    p->matrices += s.count;
   }
   return i - i0;
 }
@@ -129,6 +133,55 @@ int check_stacks(int dtype, const cora_matrices* s, int n, const char* who) {
 }
 
 }  // namespace
+
+// the iterates' formats hold singular values up to 8 and products up to 1000: follow the interval of singular values
+int ortho_bad_step(int steps, const float* coef) {
+  float sv[257];
+  for (int i = 0; i <= 256; ++i) sv[i] = i / 256.f;
+  for (int s = 0; s < steps; ++s)
+    for (float& x : sv) {
+      const float l = x * x, f = coef[3 * s] + coef[3 * s + 1] * l + coef[3 * s + 2] * l * l;
+      x = fabsf(x * f);
+      if (!(fabsf(f) <= 1000.f) || !(x <= 8.f) || !(fabsf(coef[3 * s]) <= 1000.f)) return s;
+    }
+  return -1;
+}
+
+void fill_rotary(RotaryP& p, int n_axes, const int* axes_dim, double theta, bool interleaved) {
+  int c = 0, k = 0;
+  for (int i = 0; i < n_axes; ++i) {
+    const int n = axes_dim[i];
+    for (int j = 0; j < n / 2; ++j, ++k) {
+      p.axis[k] = (unsigned char)i;
+      p.c0[k] = (unsigned char)(c + (interleaved ? 2 * j : j));
+      p.c1[k] = (unsigned char)(c + (interleaved ? 2 * j + 1 : j + n / 2));
+      p.turn[k] = std::pow(theta, -2.0 * j / n) / 6.283185307179586476925286766559;
+    }
+    c += n;
+  }
+  p.n_axes = n_axes; p.pairs = k; p.interleaved = interleaved;
+}
+
+void fill_stack(OrthoP& p, const float* x, float* y, int count, int rows, int cols) {
+  OrthoG& g = add_stack(p, count, rows, cols);
+  g.x = x; g.y = y; g.xr = g.yr = cols; g.xm = g.ym = (long long)rows * cols;
+}
+
+void ortho_place(OrthoP& p, void* ws) {
+  p.parts = (double*)ws;
+  p.ws = (unsigned short*)((char*)ws + ((size_t)p.matrices * ORTHO_PARTS * sizeof(double) + 255) / 256 * 256);
+}
+
+static size_t constants_bytes(long long rows, int heads) { return ((size_t)rows * heads * 3 * sizeof(float) + 15) / 16 * 16; }
+size_t attention_ws_bytes(int dtype, long long rows, int nseq, int heads, int kv_heads, int d, int block) {
+  const int parts = attention_parts(dtype, rows, nseq, heads, kv_heads, block);
+  return constants_bytes(rows, heads) + (parts > 1 ? (size_t)parts * 2 * sizeof(float) * (size_t)rows * (size_t)kv_heads * (size_t)d : 0);
+}
+void attention_ws(AttnP& p, int dtype, void* ws) {
+  p.parts = attention_parts(dtype, p.rows, p.nseq, p.heads, p.kv_heads, p.block);
+  p.delta = (float*)ws;
+  p.partial = (float*)((char*)ws + constants_bytes(p.rows, p.heads));
+}
 
 extern "C" {
 
@@ -159,19 +212,8 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream) {
   memset(&p, 0, sizeof p);
   p.x = a->x; p.y = a->y; p.pos = a->pos; p.rows = a->rows; p.pos_rows = a->pos_rows;
   p.xr = a->x_row; p.xh = a->x_head; p.yr = a->y_row; p.yh = a->y_head;
-  p.heads = a->heads; p.d = a->head_dim; p.n_axes = a->n_axes; p.pairs = sum / 2;
-  p.interleaved = a->interleaved != 0; p.copy = a->x != a->y; p.sign = a->backward ? -1.f : 1.f;
-  int c = 0, k = 0;
-  for (int i = 0; i < a->n_axes; ++i) {
-    const int n = a->axes_dim[i];
-    for (int j = 0; j < n / 2; ++j, ++k) {
-      p.axis[k] = (unsigned char)i;
-      p.c0[k] = (unsigned char)(c + (p.interleaved ? 2 * j : j));
-      p.c1[k] = (unsigned char)(c + (p.interleaved ? 2 * j + 1 : j + n / 2));
-      p.turn[k] = std::pow(a->theta, -2.0 * j / n) / 6.283185307179586476925286766559;
-    }
-    c += n;
-  }
+  p.heads = a->heads; p.d = a->head_dim; p.copy = a->x != a->y; p.sign = a->backward ? -1.f : 1.f;
+  fill_rotary(p, a->n_axes, a->axes_dim, a->theta, a->interleaved != 0);
   OnDevice dev(device);
   if (!dev.ok) return refuse("%s: device %d is not available", who, device);
   if (launch_rotary(p, a->dtype, (hipStream_t)hip_stream)) { refuse("%s: launch failed", who); return -3; }
@@ -180,9 +222,7 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream) {
 
 size_t cora_attention_workspace(const cora_attention_args* a) {
   if (!a || a->heads < 1 || a->kv_heads < 1 || a->head_dim < 1 || a->rows < 1 || a->n_seq < 0) return 16;
-  const size_t constants = ((size_t)a->heads * (size_t)a->rows * 3 * sizeof(float) + 15) / 16 * 16;
-  const int parts = attention_parts(a->dtype, a->rows, a->n_seq, a->heads, a->kv_heads, a->causal_block);
-  return constants + (parts > 1 ? (size_t)parts * 2 * sizeof(float) * (size_t)a->rows * (size_t)a->kv_heads * (size_t)a->head_dim : 0);
+  return attention_ws_bytes(a->dtype, a->rows, a->n_seq, a->heads, a->kv_heads, a->head_dim, a->causal_block);
 }
 
 int cora_attention(const cora_attention_args* a, int device, void* hip_stream) {
@@ -221,16 +261,8 @@ int cora_orthogonalize(int dtype, const cora_matrices* stacks, int n_stacks, int
   if (int rc = check_stacks(dtype, stacks, n_stacks, who)) return rc;
   if (steps < 1 || steps > ORTHO_STEPS || !coef) return refuse("%s: steps must be 1 .. %d, coef not NULL", who, ORTHO_STEPS);
   if (!(eps >= 0.f) || !std::isfinite(eps)) return refuse("%s: eps must be finite and not negative", who);
-  // the iterates' formats hold singular values up to 8 and products up to 1000: follow the interval of singular values
-  float sv[257];
-  for (int i = 0; i <= 256; ++i) sv[i] = i / 256.f;
-  for (int s = 0; s < steps; ++s)
-    for (float& x : sv) {
-      const float l = x * x, f = coef[3 * s] + coef[3 * s + 1] * l + coef[3 * s + 2] * l * l;
-      x = fabsf(x * f);
-      if (!(fabsf(f) <= 1000.f) || !(x <= 8.f) || !(fabsf(coef[3 * s]) <= 1000.f))
-        return refuse("%s: coefficients of step %d drive singular values of [0, 1] out of range", who, s);
-    }
+  const int bad = ortho_bad_step(steps, coef);
+  if (bad >= 0) return refuse("%s: coefficients of step %d drive singular values of [0, 1] out of range", who, bad);
   bool any = false;
   for (int i = 0; i < n_stacks; ++i) {
     const cora_matrices& s = stacks[i];
@@ -257,8 +289,7 @@ int cora_orthogonalize(int dtype, const cora_matrices* stacks, int n_stacks, int
     if (!p.ngroups) continue;
     p.eps = eps;
     ortho_ws_bytes(p);
-    p.parts = (double*)workspace;
-    p.ws = (unsigned short*)((char*)workspace + ((size_t)p.matrices * ORTHO_PARTS * sizeof(double) + 255) / 256 * 256);
+    ortho_place(p, workspace);
     if (launch_ortho(p, dtype, steps, coef, (hipStream_t)hip_stream)) { refuse("%s: launch failed", who); return -3; }
   }
   return 0;

@@ -542,3 +542,30 @@ int launch_ortho(const OrthoP& p, int dtype, int steps, const float* coef, hipSt
   return dtype == OP_F32 ? run<float, true>(p, steps, coef, st)
                          : dtype == OP_BF16 ? run<__bf16, false>(p, steps, coef, st) : run<half, true>(p, steps, coef, st);
 }
+
+// ---- orthogonalised momentum: what goes in and what comes out, one pass each, bound by memory -------
+namespace {
+__global__ __launch_bounds__(256) void muon_momentum_kernel(const MuonP p) {
+  float cm = 1.f;                                          // clip_by_global_norm, as adamw_kernel
+  if (p.clip > 0.f) {
+    const double gn = sqrt(p.sumsq[0]);
+    if (!(gn < (double)p.clip)) cm = (float)((double)p.clip / gn);
+  }
+  const float gmul = p.gscale * cm;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.n; i += (long long)gridDim.x * 256) {
+    const float g = p.g[i] * gmul, m = __builtin_fmaf(p.beta, p.mu[i], g);
+    p.mu[i] = m;
+    p.u[i] = p.nesterov ? __builtin_fmaf(p.beta, m, g) : m;
+  }
+}
+__global__ __launch_bounds__(256) void muon_apply_kernel(const MuonP p) {
+  const float lr = p.hyp[0];
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.n; i += (long long)gridDim.x * 256) {
+    const float w = p.w[i];
+    p.w[i] = w - lr * (p.size * p.u[i] + p.wd * w);
+  }
+}
+unsigned muon_blocks(long long n) { const long long b = (n + 255) / 256; return (unsigned)(b > 2048 ? 2048 : b); }
+}  // namespace
+void launch_muon_momentum(const MuonP& p, hipStream_t st) { muon_momentum_kernel<<<muon_blocks(p.n), 256, 0, st>>>(p); }
+void launch_muon_apply(const MuonP& p, hipStream_t st) { muon_apply_kernel<<<muon_blocks(p.n), 256, 0, st>>>(p); }

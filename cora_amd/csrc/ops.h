@@ -56,4 +56,21 @@ struct OrthoP {
 struct OrthoCoef { int steps; float c[3 * ORTHO_STEPS]; };
 bool ortho_is_small(const OrthoG& g);   // worked on by one workgroup, in LDS
 size_t ortho_ws_bytes(OrthoP& p);   // sets the groups' ws offsets
+void ortho_place(OrthoP& p, void* ws);  // the workspace's two parts (256-byte aligned)
 int launch_ortho(const OrthoP& p, int dtype, int steps, const float* coef, hipStream_t st);
+int ortho_bad_step(int steps, const float* coef);   // first step whose coefficients leave the iterates' range, -1: none
+
+// ---- orthogonalised momentum (ctx.hip's weight step) -----------------------------------------------
+// u = momentum of the scaled, clipped gradient over n elements
+struct MuonP {
+  const float* g; float* mu; float* u; float* w; long long n;
+  const double* sumsq; float gscale, clip, beta; int nesterov;
+  const float* hyp; float wd, size;   // apply: w -= hyp[0] (size u + wd w)
+};
+void launch_muon_momentum(const MuonP& p, hipStream_t st);
+void launch_muon_apply(const MuonP& p, hipStream_t st);
+// fills what both operators' callers inside the library share
+void fill_rotary(RotaryP& p, int n_axes, const int* axes_dim, double theta, bool interleaved);
+void fill_stack(OrthoP& p, const float* x, float* y, int count, int rows, int cols);
+size_t attention_ws_bytes(int dtype, long long rows, int nseq, int heads, int kv_heads, int d, int block);
+void attention_ws(AttnP& p, int dtype, void* ws);   // places delta, partial and parts

@@ -20,7 +20,7 @@ import numpy as np
 
 from . import _lib
 from .config import TransformerConfig
-from .optim import Optim, adamw, lr_at, sgd
+from .optim import Optim, adamw, lr_at, muon, sgd
 from .params import (BLOCK_LEAVES, K_BOUT, K_BP, K_WOUT, K_WP, block_key, init_params, param_shapes, vln_key,
                      vode_key)
 from .posenc import create_positional_encoding
@@ -164,6 +164,8 @@ class TransformerDecoder:
         self.positional_embedding = create_positional_encoding(
             image_shape=c.image_shape, hidden_size=c.hidden_size, patch_size=c.patch_size,
             is_video=c.is_video, num_frames=c.num_frames if c.is_video else None, theta=c.theta)
+        if c.pos_encoding == "rotary":   # positions turn queries and keys instead
+            self.positional_embedding = np.zeros((self.N, self.D), dtype=np.float32)
         self.vodes: List[Vode] = [Vode(self, l) for l in range(self.L + 3)]
         self.vodes[-1].h.frozen = True
         self.transformer_blocks = [TransformerBlock(self, i, self.D, self.M) for i in range(self.L)]
@@ -178,6 +180,7 @@ class TransformerDecoder:
         self._B = None
         self._offsets: Dict[str, tuple] = {}
         self._optim_sig = None
+        self._muon_sig = None
         self._x_host: Optional[np.ndarray] = None
         self._dp = None
 
@@ -204,6 +207,12 @@ class TransformerDecoder:
             grad_norm_target=float(c.vode_grad_norm_target), max_T=self.max_T,
             use_vode_ln=int(bool(c.use_vode_state_layernorm)))
 
+    def _make_attn_options(self) -> _lib.CoraAttnOptions:
+        c = self.config
+        axes = [int(a) for a in c.axes_dim] if c.pos_encoding == "rotary" else []
+        return _lib.CoraAttnOptions(n_axes=len(axes), axes_dim=(C.c_int32 * 4)(*axes), theta=float(c.theta),
+                                    causal_block=self.N // self._F if c.causal_frames else 0)
+
     def _ensure_ctx(self, B: int):
         if self._ctx is not None:
             if B != self._B:
@@ -213,7 +222,7 @@ class TransformerDecoder:
         lib = _lib.load()
         cfg = self._make_cfg(B)
         ctx = C.c_void_p()
-        _lib.check(lib.cora_create(C.byref(cfg), self.device, C.byref(ctx)), None)
+        _lib.check(lib.cora_create_attn(C.byref(cfg), C.byref(self._make_attn_options()), self.device, C.byref(ctx)), None)
         self._ctx, self._B = ctx, B
         n = C.c_size_t()
         _lib.check(lib.cora_weights_size(ctx, C.byref(n)), ctx)
@@ -341,10 +350,17 @@ class TransformerDecoder:
         rh, rw = optim_h._recipe(), optim_w._recipe()
         if not isinstance(rh.base, sgd):
             raise NotImplementedError("vode optimizer must be sgd(lr, momentum) (AdamW-for-h: SURVEY 8(f) rank 4)")
-        if not isinstance(rw.base, adamw):
-            raise NotImplementedError("weight optimizer must be adamw")
-        sig = (float(rh.clip or 0.0), float(rh.base.momentum or 0.0), float(rw.clip or 0.0),
-               float(rw.base.b1), float(rw.base.b2), float(rw.base.eps), float(rw.base.weight_decay))
+        if not isinstance(rw.base, (adamw, muon)):
+            raise NotImplementedError("weight optimizer must be adamw or muon")
+        w, m = rw.base, isinstance(rw.base, muon)
+        adam = (w.adam_b1, w.adam_b2, w.adam_eps, w.adam_weight_decay) if m else (w.b1, w.b2, w.eps, w.weight_decay)
+        coef = [v for t in w.coefficients() for v in t] if m else []
+        muon_sig = (float(w.beta), bool(w.nesterov), float(w.weight_decay), int(w.ns_steps), tuple(coef), float(w.eps)) if m else None
+        if muon_sig != self._muon_sig:
+            args = (1, *muon_sig[:4], (C.c_float * len(coef))(*coef), muon_sig[5]) if m else (0, 0.0, 0, 0.0, 0, None, 0.0)
+            _lib.check(_lib.load().cora_set_muon(self._ctx, *args), self._ctx)
+            self._muon_sig = muon_sig
+        sig = (float(rh.clip or 0.0), float(rh.base.momentum or 0.0), float(rw.clip or 0.0)) + tuple(float(v) for v in adam)
         if sig != self._optim_sig:
             _lib.check(_lib.load().cora_set_optim(self._ctx, *[C.c_float(v) for v in sig]), self._ctx)
             self._optim_sig = sig

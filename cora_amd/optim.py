@@ -4,8 +4,8 @@ The reference builds optax transformations and wraps them in pcx `Optim`
 (/root/reference/examples/debug_transformer_wandb.py:1116-1167,
 /root/reference/pcx/utils/_optim.py:32-169).  The HIP step implements exactly the recipes used
 there -- `chain(clip_by_global_norm(c), sgd(lr, momentum))` for the vodes and
-`chain(clip_by_global_norm(c), adamw(lr, weight_decay=...))` for the weights -- so these classes
-only DESCRIBE a recipe (same constructor names and argument meaning as optax 0.2.3); the
+`chain(clip_by_global_norm(c), adamw(lr, weight_decay=...))` for the weights, and beyond the reference
+`muon(lr, ...)` for the weights -- so these classes only DESCRIBE a recipe (same constructor names and argument meaning as optax 0.2.3); the
 arithmetic runs in the fused vode-update / AdamW kernels.
 """
 from __future__ import annotations
@@ -42,13 +42,40 @@ class adamw:
     weight_decay: float = 1e-4
 
 
+@dataclass
+class muon:
+    """Weight steps by orthogonalised momentum for the blocks' matrices (query, key, value and output projections, both MLP
+    matrices); every other parameter takes the AdamW step of the adam_* values with the same learning rate.
+    m <- beta m + g;  u = g + beta m (nesterov) or m;  O = Newton-Schulz(u), ns_steps products with ns_coeffs, (a, b, c) or a
+    triple for every step (`cora_amd.orthogonalize`);  W <- W - lr (sqrt(max(1, rows / cols)) O + weight_decay W)."""
+    learning_rate: Schedule
+    beta: float = 0.95
+    nesterov: bool = True
+    weight_decay: float = 0.0
+    ns_steps: int = 5
+    ns_coeffs: tuple = (3.4445, -4.7750, 2.0315)
+    eps: float = 1e-7
+    adam_b1: float = 0.9
+    adam_b2: float = 0.999
+    adam_eps: float = 1e-8
+    adam_weight_decay: float = 0.0
+
+    def coefficients(self):
+        """One (a, b, c) per step."""
+        c = [tuple(float(v) for v in t) for t in self.ns_coeffs] if hasattr(self.ns_coeffs[0], "__len__") else \
+            [tuple(float(v) for v in self.ns_coeffs)] * int(self.ns_steps)
+        if len(c) != int(self.ns_steps) or any(len(t) != 3 for t in c):
+            raise ValueError("ns_coeffs must be (a, b, c) or one such triple for every step")
+        return c
+
+
 class chain:
     def __init__(self, *transforms):
         self.transforms = tuple(transforms)
         clips = [t for t in transforms if isinstance(t, clip_by_global_norm)]
-        bases = [t for t in transforms if isinstance(t, (sgd, adamw))]
+        bases = [t for t in transforms if isinstance(t, (sgd, adamw, muon))]
         if len(clips) > 1 or len(bases) != 1 or len(clips) + len(bases) != len(transforms):
-            raise ValueError("supported recipes: chain([clip_by_global_norm], sgd | adamw)")
+            raise ValueError("supported recipes: chain([clip_by_global_norm], sgd | adamw | muon)")
         if clips and transforms[0] is not clips[0]:
             raise ValueError("clip_by_global_norm must precede the optimizer (reference order)")
         self.clip = clips[0].max_norm if clips else None
@@ -98,11 +125,11 @@ class Optim:
 
     def init(self, parameters=None) -> None:
         """(Re-)initialise the optimizer state (pcx/utils/_optim.py:150-163): the schedule count restarts
-        and, for an AdamW recipe bound to a model, the moments and the bias-correction count on the
+        and, for an AdamW or Muon recipe bound to a model, the moments and the bias-correction count on the
         device are zeroed with it -- in the reference mu, nu and count are one optax state."""
         self.recipe = _as_chain(self.optax_opt_fn())
         self.count = 0
-        if parameters is not None and isinstance(self.recipe.base, adamw) and hasattr(parameters, "_reset_adam_state"):
+        if parameters is not None and isinstance(self.recipe.base, (adamw, muon)) and hasattr(parameters, "_reset_adam_state"):
             parameters._reset_adam_state()
 
     def clear(self) -> None:
@@ -138,7 +165,10 @@ def make_optimizers(cfg, model=None, total_train_steps: int = 1):
     h_steps.append(sgd(h_lr, momentum=cfg.hidden_momentum))
     if cfg.w_grad_clip_norm is not None and cfg.w_grad_clip_norm > 0:
         w_steps.append(clip_by_global_norm(cfg.w_grad_clip_norm))
-    w_steps.append(adamw(w_lr, weight_decay=cfg.weight_decay))
+    if getattr(cfg, "use_muon_for_weight_optimizer", False):
+        w_steps.append(muon(w_lr, weight_decay=cfg.weight_decay, adam_weight_decay=cfg.weight_decay))
+    else:
+        w_steps.append(adamw(w_lr, weight_decay=cfg.weight_decay))
     optim_h = Optim(lambda: chain(*h_steps))
     optim_w = Optim(lambda: chain(*w_steps), parameters=model)
     return optim_w, optim_h

@@ -85,6 +85,16 @@ typedef struct cora_step_out {
 /* Replaces TransformerDecoder.__init__ (src/decoder_transformer.py:129-218): allocates vodes,
  * weights, optimizer state and scratch on `device`. */
 int cora_create(const cora_config* cfg, int device, cora_ctx** out);
+/* The same with what the blocks' attention does beyond the reference's (pcx/nn/_layer.py:428-447, bidirectional, additive
+ * positions only).  Per-op kernels; cora_forward_static does not serve it.
+ * n_axes 2 (row, column of the patch; F = 1) or 3 (frame, row, column): queries and keys are turned by the token's position
+ * as cora_rotary does (interleaved pairs), so cora_set_pos should be given zeros; 0: not.  axes_dim[0 .. n_axes-1] must fit
+ * the head dim.  causal_block b >= 1: a token sees the tokens of its own and of earlier blocks of b tokens (N / F: frames). */
+typedef struct cora_attn_options {
+  int32_t n_axes, axes_dim[4], causal_block;
+  double  theta;
+} cora_attn_options;
+int cora_create_attn(const cora_config* cfg, const cora_attn_options* opt /* NULL: as cora_create */, int device, cora_ctx** out);
 int cora_destroy(cora_ctx* ctx);
 const char* cora_last_error(const cora_ctx* ctx /* may be NULL */);
 
@@ -115,6 +125,13 @@ int cora_get_adam_state(cora_ctx* ctx, float* mu, float* nu, int64_t* count);
  * a value changes.  AdamW moments and count are kept. */
 int cora_set_optim(cora_ctx* ctx, float clip_h, float momentum, float clip_w, float adam_b1,
                    float adam_b2, float adam_eps, float adam_wd);
+
+/* Weight steps by orthogonalised momentum (Muon) instead of AdamW for the blocks' matrices -- query, key, value and output
+ * projections and the two MLP matrices.  With g the scaled, clipped gradient: m <- beta m + g, u = g + beta m (nesterov) or m,
+ * O = Newton-Schulz(u) as cora_orthogonalize (steps, coef [steps, 3], eps), W <- W - eta_w (sqrt(max(1, rows / cols)) O + wd W).
+ * Every other parameter keeps the AdamW step of cora_set_optim with the same eta_w.  m lives in the first AdamW moment.
+ * enabled 0 goes back to AdamW for all.  The reference has AdamW only (examples/debug_transformer_wandb.py:1154-1159). */
+int cora_set_muon(cora_ctx* ctx, int enabled, float beta, int nesterov, float wd, int steps, const float* coef, float eps);
 
 /* --- the step ------------------------------------------------------------------------------- */
 /* Whole train_on_batch (src/decoder_transformer.py:392-499, mode 2): set the sensory vode to x,
