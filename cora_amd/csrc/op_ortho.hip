@@ -290,7 +290,7 @@ __global__ __launch_bounds__(1024) void ortho_small(const OrthoP p, const OrthoC
 // swizzled tile.  Rows and columns outside a matrix are read from its last one; what they give is not stored, and along
 // the contraction they meet zeros (columns up to ldn and ldm are stored as zeros).
 template <typename T, int STEP, bool FULL>
-__global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const int cur, const int last, const float ca, const float cb, const float cc) {
+__global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const int cuts, const int cur, const int last, const float ca, const float cb, const float cc) {
   constexpr int TK = 32;
   constexpr bool BLO = FULL || STEP == 1, ALO = FULL || STEP != 0;
   constexpr int NPL = 2 + BLO + ALO, PB1 = 1, PA0 = BLO ? 2 : 1, PA1 = PA0 + 1;   // planes: B hi, (B lo,) A hi, (A lo)
@@ -298,17 +298,27 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
   typedef Op<half> O;
   __shared__ __attribute__((aligned(16))) half buf0[NPL][128 * TK];
   __shared__ __attribute__((aligned(16))) half buf1[NPL][128 * TK];
-  int gi = 0, id = blockIdx.x, per = 0;
-  for (;; ++gi) {                                          // group of this tile
+  // Workgroups go round robin over the 8 XCDs; each matrix' tiles are cut into `cuts` runs and the runs dealt to the XCDs, so
+  // that the tiles that read the same rows share one XCD's L2.
+  const int xcd = blockIdx.x & 7;
+  int gi = 0, k = blockIdx.x >> 3, per, run, mat, tl;
+  for (;; ++gi) {
     if (gi == p.ngroups) return;
     const int tm = (p.g[gi].m + 127) / 128, tn = (p.g[gi].ldn + 127) / 128;
     per = STEP == 2 ? tm * tn : tm * (tm + 1) / 2;
-    if (id < per * p.g[gi].count) break;
-    id -= per * p.g[gi].count;
+    run = (per + cuts - 1) / cuts;
+    const int off = (xcd - p.g[gi].first * cuts) & 7, have = (p.g[gi].count * cuts - off + 7) >> 3;
+    if (k < have * run) {
+      const int unit = off + 8 * (k / run);
+      mat = unit / cuts;
+      tl = unit % cuts * run + k % run;
+      break;
+    }
+    k -= max(have, 0) * run;
   }
+  if (tl >= per) return;
   const OrthoG& g = p.g[gi];
   const int m = g.m, ldn = g.ldn, ldm = g.ldm;
-  const int mat = id / per, tl = id % per;
   int ti, tj;
   if (STEP == 2) { const int tm = (m + 127) / 128; ti = tl % tm; tj = tl / tm; }
   else {
@@ -466,24 +476,38 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
       }
 }
 
-template <typename T, bool FULL> int run_tiled(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
-  int load_tiles = 0;
-  long long sym = 0, full = 0;
-  for (int i = 0; i < p.ngroups; ++i) {
-    const OrthoG& g = p.g[i];
-    const int t = g.ldn / 64 * (g.ldm / 64), tm = (g.m + 127) / 128, tn = (g.ldn + 127) / 128;
-    if (t > load_tiles) load_tiles = t;
-    sym += (long long)g.count * tm * (tm + 1) / 2;
-    full += (long long)g.count * tm * tn;
+// workgroups of a launch over `tiles(group)` tiles a matrix cut into `cuts` runs: the fullest XCD's, eight times
+template <typename F> unsigned grid_of(const OrthoP& p, int cuts, F tiles) {
+  long long most = 0;
+  for (int x = 0; x < 8; ++x) {
+    long long n = 0;
+    for (int i = 0; i < p.ngroups; ++i) {
+      const int per = tiles(p.g[i]), run = (per + cuts - 1) / cuts, off = (x - p.g[i].first * cuts) & 7;
+      const long long have = ((long long)p.g[i].count * cuts - off + 7) >> 3;
+      if (have > 0) n += have * run;
+    }
+    if (n > most) most = n;
   }
+  return (unsigned)(8 * most);
+}
+
+template <typename T, bool FULL> int run_tiled(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
+  int load_tiles = 0, cuts = 1;
+  for (int i = 0; i < p.ngroups; ++i) {
+    const int t = p.g[i].ldn / 64 * (p.g[i].ldm / 64);
+    if (t > load_tiles) load_tiles = t;
+  }
+  while (cuts < 8 && p.matrices * cuts < 64) cuts *= 2;
+  const unsigned sym = grid_of(p, cuts, [](const OrthoG& g) { const int tm = (g.m + 127) / 128; return tm * (tm + 1) / 2; });
+  const unsigned full = grid_of(p, cuts, [](const OrthoG& g) { return (g.m + 127) / 128 * ((g.ldn + 127) / 128); });
   ortho_sumsq<T><<<dim3(p.matrices, ORTHO_PARTS), 256, 0, st>>>(p);
   ortho_load<T><<<dim3(load_tiles, p.matrices), 256, 0, st>>>(p);
   for (int s = 0; s < steps; ++s) {
     const int cur = 2 * (s & 1), last = s == steps - 1;
     const float a = coef[3 * s], b = coef[3 * s + 1], c = coef[3 * s + 2];
-    ortho_product<T, 0, FULL><<<dim3((unsigned)sym), 256, 0, st>>>(p, cur, 0, a, b, c);
-    ortho_product<T, 1, FULL><<<dim3((unsigned)sym), 256, 0, st>>>(p, cur, 0, a, b, c);
-    ortho_product<T, 2, FULL><<<dim3((unsigned)full), 256, 0, st>>>(p, cur, last, a, b, c);
+    ortho_product<T, 0, FULL><<<dim3(sym), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
+    ortho_product<T, 1, FULL><<<dim3(sym), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
+    ortho_product<T, 2, FULL><<<dim3(full), 256, 0, st>>>(p, cuts, cur, last, a, b, c);
   }
   return hipGetLastError() != hipSuccess;
 }

@@ -29,40 +29,47 @@ template <typename T, int V> struct VecOf { typedef T type __attribute__((ext_ve
 template <typename T> struct VecOf<T, 1> { struct type { T v; __device__ T& operator[](int) { return v; } }; };
 
 // INTER: V neighbouring channels (V / 2 pairs, V even) a thread; else V first and the V second channels of V pairs.  V = 1
-// takes any layout.
+// takes any layout.  Threads of channels that pass through move one (INTER) or two vectors in the same loop.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const int units, const int hchunk) {
-  constexpr int MODE = INTER ? 1 : 2, NPAIR = INTER ? V / 2 : V;
+  constexpr int NPAIR = INTER ? V / 2 : V;
   typedef typename VecOf<T, V>::type vec;
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / units;
   if (row >= p.rows) return;
   const int u = (int)(id - row * units);
   const int h0 = blockIdx.y * hchunk, h1 = min(p.heads, h0 + hchunk);
-  const int turning = MODE == 1 ? 2 * p.pairs / V : p.pairs / V;
+  const int turning = p.pairs / NPAIR;
+  const bool turns = u < turning;
   const T* x = (const T*)p.x + row * p.xr + h0 * p.xh;
   T* y = (T*)p.y + row * p.yr + h0 * p.yh;
-  if (u >= turning) {                                    // channels that pass through
-    const int c = 2 * p.pairs + (u - turning) * V;
-    for (int h = h0; h < h1; ++h, x += p.xh, y += p.yh) *reinterpret_cast<vec*>(y + c) = *reinterpret_cast<const vec*>(x + c);
-    return;
-  }
-  const int* pos = p.pos + (row % p.pos_rows) * p.n_axes;
   float cs[NPAIR], sn[NPAIR];
+  int ca, cb;
+  if (turns) {
+    const int* pos = p.pos + (row % p.pos_rows) * p.n_axes;
 #pragma unroll
-  for (int i = 0; i < NPAIR; ++i) {
-    const int pr = u * NPAIR + i;
-    turn_cs((double)pos[p.axis[pr]] * p.turn[pr], p.sign, cs[i], sn[i]);
+    for (int i = 0; i < NPAIR; ++i) {
+      const int pr = u * NPAIR + i;
+      turn_cs((double)pos[p.axis[pr]] * p.turn[pr], p.sign, cs[i], sn[i]);
+    }
+    ca = INTER ? u * V : p.c0[u * NPAIR];
+    cb = INTER ? 0 : p.c1[u * NPAIR];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NPAIR; ++i) cs[i] = sn[i] = 0.f;
+    ca = 2 * p.pairs + (u - turning) * (INTER ? V : 2 * V);
+    cb = min(ca + V, p.d - V);
   }
-  const int ca = MODE == 1 ? u * V : p.c0[u * NPAIR], cb = MODE == 1 ? 0 : p.c1[u * NPAIR];
 #pragma unroll 4
   for (int h = h0; h < h1; ++h, x += p.xh, y += p.yh) {
-    if (MODE == 1) {
+    if (INTER) {
       vec a = *reinterpret_cast<const vec*>(x + ca);
 #pragma unroll
       for (int i = 0; i < NPAIR; ++i) {
         const float ua = (float)a[2 * i], ub = (float)a[(2 * i + 1) % V];
-        a[2 * i] = (T)(ua * cs[i] - ub * sn[i]);
-        a[(2 * i + 1) % V] = (T)(ua * sn[i] + ub * cs[i]);
+        if (turns) {
+          a[2 * i] = (T)(ua * cs[i] - ub * sn[i]);
+          a[(2 * i + 1) % V] = (T)(ua * sn[i] + ub * cs[i]);
+        }
       }
       *reinterpret_cast<vec*>(y + ca) = a;
     } else {
@@ -70,8 +77,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const int 
 #pragma unroll
       for (int i = 0; i < NPAIR; ++i) {
         const float ua = (float)a[i], ub = (float)b[i];
-        a[i] = (T)(ua * cs[i] - ub * sn[i]);
-        b[i] = (T)(ua * sn[i] + ub * cs[i]);
+        if (turns) {
+          a[i] = (T)(ua * cs[i] - ub * sn[i]);
+          b[i] = (T)(ua * sn[i] + ub * cs[i]);
+        }
       }
       *reinterpret_cast<vec*>(y + ca) = a;
       *reinterpret_cast<vec*>(y + cb) = b;
@@ -92,7 +101,8 @@ template <typename T> bool fits(const RotaryP& p, int v) {
   return true;
 }
 template <typename T, int V, bool INTER> int go(const RotaryP& p, hipStream_t st) {
-  const int rest = p.copy ? p.d - 2 * p.pairs : 0, units = ((INTER ? 2 * p.pairs : p.pairs) + rest) / V;
+  const int rest = p.copy ? p.d - 2 * p.pairs : 0;
+  const int units = INTER ? (2 * p.pairs + rest) / V : p.pairs / V + (rest + 2 * V - 1) / (2 * V);
   const long long blocks = (p.rows * units + 255) / 256;
   // few rows: the heads are split over the grid until there are about four workgroups per compute unit
   int split = 1;
