@@ -101,6 +101,7 @@ OrthoG& add_stack(OrthoP& p, int count, int rows, int cols) {
   g.count = count; g.rows = rows; g.cols = cols;
   g.m = rows < cols ? rows : cols; g.n = rows < cols ? cols : rows;
   g.ldn = (g.n + 63) / 64 * 64; g.ldm = (g.m + 63) / 64 * 64;
+  g.sn = g.ldn | 64; g.sm = g.ldm | 64;
   g.first = p.matrices;
   p.matrices += count;
   return g;

@@ -23,15 +23,6 @@
 
 namespace {
 
-// Direct requests of 16 or 4 bytes a lane: the lane's bytes at base + at go to lds + 16 (4) * lane, zeros where at is behind
-// `bytes`.  (The host pass has no buffer descriptor type and silently drops kernels that name one.)
-#ifdef __HIP_DEVICE_COMPILE__
-#define REQUEST(base, bytes, lds, n, at) \
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)(base), 0, bytes, 0x00020000), (LDS3 void*)(lds), n, at, 0, 0, 0)
-#else
-#define REQUEST(base, bytes, lds, n, at) (void)0
-#endif
-
 // Staging of R rows x D channels straight from global memory into an LDS tile by NW waves.  A wave's request fills 64
 // consecutive 16-byte places; each lane asks for the piece that belongs there (Tile::swz).  The buffer descriptor ends
 // with the last valid row, and the pieces of channels >= d ask for an address past any end: both arrive as zeros.
@@ -110,7 +101,7 @@ __device__ __forceinline__ int limit(int i, int n, int block) {
 
 // The tiles a workgroup walks pass through two LDS buffers, each an object of its own so that the compiler sees that the
 // requests for one do not touch what is read from the other.  Between two barriers the next tile is under way while the
-// current one is worked on.
+// current one is worked on.  (One exit only: a second one makes the compiler keep two copies of the accumulators.)
 #define WALK(COUNT, FETCH, WORK)                                                   \
   FETCH(0, 0);                                                                     \
   for (int it_ = 0; it_ < (COUNT); it_ += 2) {                                     \
@@ -118,11 +109,10 @@ __device__ __forceinline__ int limit(int i, int n, int block) {
     if (it_ + 1 < (COUNT)) FETCH(it_ + 1, 1);                                      \
     __builtin_amdgcn_sched_barrier(0);                                             \
     WORK(it_, 0);                                                                  \
-    if (it_ + 1 >= (COUNT)) break;                                                 \
     arrive_barrier();                                                              \
     if (it_ + 2 < (COUNT)) FETCH(it_ + 2, 0);                                      \
     __builtin_amdgcn_sched_barrier(0);                                             \
-    WORK(it_ + 1, 1);                                                              \
+    if (it_ + 1 < (COUNT)) WORK(it_ + 1, 1);                                       \
   }
 
 // Queries of a workgroup and its walk over keys.  SPLIT = false: NW waves of 32 queries each share every staged tile of KT

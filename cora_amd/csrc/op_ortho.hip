@@ -12,10 +12,11 @@
 // exponents, but all iterates have singular values of at most a few units, so a fixed power of two places them: X is
 // stored times 2^12 (entries of a large matrix are near 1 / sqrt(m n)), A and P times 2^6 (what matters of them is their
 // size next to a ~ 3); the caller's coefficients are refused where the iterates could leave these ranges.
-// For bf16 results the two large products save instructions where the error does not grow: A from the upper halves of X
-// alone (one instruction), and P X with the upper half of P = b A + c A^2 (two), a X being added in fp32; A^2 keeps all
-// three, since at singular values near 1 an error of A^2 is amplified.  The result is then 1e-3 (rms) off the exact
-// iterates before its own rounding of 1.7e-3, against 2.5e-3 with one instruction throughout.
+// For bf16 results of large matrices the products with X take one instruction: A from the upper halves of X, and B X with
+// the upper halves of X and of B = b A + c A^2, while a X is added in fp32 from both halves, so that what the iteration
+// amplifies most is never rounded to 11 bits; A^2 keeps all three, since at singular values near 1 its errors are
+// amplified.  The result is then 1.1e-3 (rms) off the exact iterates before its own rounding of 1.7e-3; with A^2 from upper
+// halves too it is 2e-3, and with X itself in 11 bits 2.5e-3.
 #include "op_tile.h"
 #include "ops.h"
 
@@ -25,46 +26,47 @@ typedef _Float16 half;
 typedef half h16x4 __attribute__((ext_vector_type(4)));
 constexpr float SX = 4096.f, SA = 64.f;
 
-// workspace of one matrix, in halves: X hi, X lo, Y hi, Y lo (m x ldn each), A hi, A lo, P hi, P lo (m x ldm each)
+// workspace of one matrix, in halves: X hi, X lo, Y hi, Y lo (m rows of stride sn each), A hi, A lo, P hi, P lo (stride sm).
+// Strides are odd multiples of 128 bytes: with a power of two the rows of a tile all lie in one channel of the L2 cache.
 __device__ __forceinline__ half* plane_x(const OrthoP& p, const OrthoG& g, int mat, int which) {
-  return (half*)p.ws + g.ws + (long long)mat * (4LL * g.m * g.ldn + 4LL * g.m * g.ldm) + (long long)which * g.m * g.ldn;
+  return (half*)p.ws + g.ws + (long long)mat * (4LL * g.m * (g.sn + g.sm)) + (long long)which * g.m * g.sn;
 }
 __device__ __forceinline__ half* plane_a(const OrthoP& p, const OrthoG& g, int mat, int which) {
-  return plane_x(p, g, mat, 4) + (long long)which * g.m * g.ldm;
+  return plane_x(p, g, mat, 4) + (long long)which * g.m * g.sm;
 }
 
 __device__ __forceinline__ void split2(float v, half& hi, half& lo) { hi = (half)v; lo = (half)(v - (float)hi); }
 
-// partial sums of squares in 64 bits: part z of a matrix takes every ORTHO_PARTS-th strip of 2048 elements of its rows
+// partial sums of squares in 64 bits: part z of a matrix takes every ORTHO_PARTS-th run of 256 vectors
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_sumsq(const OrthoP p) {
   constexpr int V = 16 / (int)sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(V)));
   __shared__ double sh[4];
   const int id = blockIdx.x, part = blockIdx.y;
   int gi = 0;
   while (gi + 1 < p.ngroups && id >= p.g[gi + 1].first) ++gi;
   const OrthoG& g = p.g[gi];
   const T* x = (const T*)g.x + (long long)(id - g.first) * g.xm;
-  const bool vec = (uintptr_t)x % 16 == 0 && g.xr % V == 0;
-  const int strips = (g.cols + 2047) / 2048;
+  const unsigned cols = g.cols, total = (unsigned)g.rows * cols;      // at most 2^30
+  const long long xr = g.xr;
+  const bool packed = xr == cols;
   double s = 0.0;
-  for (long long t = part; t < (long long)g.rows * strips; t += ORTHO_PARTS) {
-    const long long r = t / strips;
-    const int c0 = (int)(t - r * strips) * 2048, c1 = min(g.cols, c0 + 2048);
-    const T* row = x + r * g.xr;
-    if (vec) {
-      for (int c = c0 + (int)threadIdx.x * V; c < c1; c += 256 * V) {
-        typedef T vecT __attribute__((ext_vector_type(V)));
-        if (c + V <= c1) {
-          const vecT v = *reinterpret_cast<const vecT*>(row + c);
+  if ((uintptr_t)x % 16 == 0 && xr % V == 0 && cols % V == 0) {
+#pragma unroll 4
+    for (unsigned e = (part * 256 + threadIdx.x) * V; e < total; e += ORTHO_PARTS * 256 * V) {
+      const unsigned r = packed ? 0 : e / cols, c = packed ? e : e - r * cols;
+      const vec v = *reinterpret_cast<const vec*>(x + r * xr + c);
 #pragma unroll
-          for (int i = 0; i < V; ++i) s += (double)(float)v[i] * (double)(float)v[i];
-        } else
-          for (int i = c; i < c1; ++i) s += (double)(float)row[i] * (double)(float)row[i];
-      }
-    } else
-      for (int c = c0 + (int)threadIdx.x; c < c1; c += 256) s += (double)(float)row[c] * (double)(float)row[c];
-  }
+      for (int i = 0; i < V; ++i) s += (double)(float)v[i] * (double)(float)v[i];
+    }
+  } else
+#pragma unroll 4
+    for (unsigned e = part * 256 + threadIdx.x; e < total; e += ORTHO_PARTS * 256) {
+      const unsigned r = e / cols, c = e - r * cols;
+      const double v = (double)(float)x[r * xr + c];
+      s += v * v;
+    }
   s = block_sum_256(s, sh);
   if (threadIdx.x == 0) p.parts[(long long)id * ORTHO_PARTS + part] = s;
 }
@@ -80,8 +82,10 @@ __global__ __launch_bounds__(256) void ortho_load(const OrthoP p) {
   const int mat = id - g.first, tn = g.ldn / 64, tm = g.ldm / 64;
   if ((int)blockIdx.x >= tn * tm) return;
   const int i0 = blockIdx.x / tn * 64, j0 = blockIdx.x % tn * 64;
-  static_assert(ORTHO_PARTS == 64, "one part per lane");
-  const double s = wave_sum_d(p.parts[(long long)id * ORTHO_PARTS + (threadIdx.x & 63)]);
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < ORTHO_PARTS / 64; ++i) s += p.parts[(long long)id * ORTHO_PARTS + 64 * i + (threadIdx.x & 63)];
+  s = wave_sum_d(s);
   const double f = (double)SX / (sqrt(s) + (double)p.eps);
   const bool tall = g.rows > g.cols;
   const T* x = (const T*)g.x + (long long)mat * g.xm;
@@ -100,7 +104,7 @@ __global__ __launch_bounds__(256) void ortho_load(const OrthoP p) {
       h16x4 vh, vl;
 #pragma unroll
       for (int e = 0; e < 4; ++e) { half u, v; split2(t[k][4 * (threadIdx.x & 15) + e], u, v); vh[e] = u; vl[e] = v; }
-      const long long o = (long long)(i0 + k) * g.ldn + j0 + 4 * (threadIdx.x & 15);
+      const long long o = (long long)(i0 + k) * g.sn + j0 + 4 * (threadIdx.x & 15);
       *reinterpret_cast<h16x4*>(hi + o) = vh;
       *reinterpret_cast<h16x4*>(lo + o) = vl;
     }
@@ -284,27 +288,28 @@ __global__ __launch_bounds__(1024) void ortho_small(const OrthoP p, const OrthoC
 }
 
 // One product for all matrices.  STEP 0: A = X X^T; 1: P = a I + b A + c A A; 2: X' = P X (last: to the caller's matrix).
-// Tile 128 x 128, four waves of 64 x 64, slabs of 32: the first operand gives the output's columns, the second its rows
-// (op_tile.h), so a lane holds four neighbouring columns of one output row.  Slabs go from global memory straight into one
+// Tile TS x TS: 128 with four waves of 64 x 64, two workgroups a compute unit; or 256 with eight waves of 128 x 64, which
+// halves what a flop reads from L2 (the 128 tile's 43 bytes a cycle and compute unit exceed it).  The first operand gives
+// the output's columns, the second its rows (op_tile.h), so a lane holds four neighbouring columns of one output row.  Slabs go from global memory straight into one
 // of two LDS buffers while the other is worked on; a lane fetches the 16-byte piece that belongs at its place of the
-// swizzled tile.  Rows and columns outside a matrix are read from its last one; what they give is not stored, and along
-// the contraction they meet zeros (columns up to ldn and ldm are stored as zeros).
-template <typename T, int STEP, bool FULL>
-__global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const int cuts, const int cur, const int last, const float ca, const float cb, const float cc) {
-  constexpr int TK = 32;
-  constexpr bool BLO = FULL || STEP == 1, ALO = FULL || STEP != 0;
-  constexpr int NPL = 2 + BLO + ALO, PB1 = 1, PA0 = BLO ? 2 : 1, PA1 = PA0 + 1;   // planes: B hi, (B lo,) A hi, (A lo)
-  typedef Tile<half, TK> LR; typedef Tile<half, 128> LC;
+// swizzled tile.  Rows outside a matrix arrive as zeros, columns behind it as whatever follows (the columns up to ldn and ldm
+// are stored as zeros, what lies behind gives nothing that is stored).
+template <typename T, int STEP, bool FULL, int TS>
+__global__ __launch_bounds__(2 * TS, 2) void ortho_product(const OrthoP p, const int cuts, const int cur, const int last, const float ca, const float cb, const float cc) {
+  constexpr bool LO = FULL || STEP == 1;                  // both halves of both operands
+  constexpr int NPL = LO ? 4 : 2, PB1 = 1, PA0 = LO ? 2 : 1, PA1 = LO ? 3 : 0;    // planes: B hi, (B lo,) A hi, (A lo)
+  constexpr int TK = LO ? 32 : 64, NW = TS / 32, NB = TS / 64, NI = TS * TK / 512 / NW;   // slab, waves, row tiles of a wave, requests of a wave and plane
+  typedef Tile<half, TK> LR; typedef Tile<half, TS> LC;
   typedef Op<half> O;
-  __shared__ __attribute__((aligned(16))) half buf0[NPL][128 * TK];
-  __shared__ __attribute__((aligned(16))) half buf1[NPL][128 * TK];
+  __shared__ __attribute__((aligned(16))) half buf0[NPL][TS * TK];
+  __shared__ __attribute__((aligned(16))) half buf1[NPL][TS * TK];
   // Workgroups go round robin over the 8 XCDs; each matrix' tiles are cut into `cuts` runs and the runs dealt to the XCDs, so
   // that the tiles that read the same rows share one XCD's L2.
   const int xcd = blockIdx.x & 7;
   int gi = 0, k = blockIdx.x >> 3, per, run, mat, tl;
   for (;; ++gi) {
     if (gi == p.ngroups) return;
-    const int tm = (p.g[gi].m + 127) / 128, tn = (p.g[gi].ldn + 127) / 128;
+    const int tm = (p.g[gi].m + TS - 1) / TS, tn = (p.g[gi].ldn + TS - 1) / TS;
     per = STEP == 2 ? tm * tn : tm * (tm + 1) / 2;
     run = (per + cuts - 1) / cuts;
     const int off = (xcd - p.g[gi].first * cuts) & 7, have = (p.g[gi].count * cuts - off + 7) >> 3;
@@ -318,53 +323,46 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
   }
   if (tl >= per) return;
   const OrthoG& g = p.g[gi];
-  const int m = g.m, ldn = g.ldn, ldm = g.ldm;
+  const int m = g.m, ldn = g.ldn, ldm = g.ldm, sn = g.sn, sm = g.sm;
   int ti, tj;
-  if (STEP == 2) { const int tm = (m + 127) / 128; ti = tl % tm; tj = tl / tm; }
+  if (STEP == 2) { const int tm = (m + TS - 1) / TS; ti = tl % tm; tj = tl / tm; }
   else {
     ti = (int)((sqrtf(8.f * tl + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > tl) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= tl) ++ti;
     tj = tl - ti * (ti + 1) / 2;
   }
-  const int ld = STEP == 0 ? ldn : ldm;                    // contraction length
+  const int ld = STEP == 0 ? ldn : ldm, sk = STEP == 0 ? sn : sm;   // contraction length, stride of the planes along it
   const half* bh = STEP == 0 ? plane_x(p, g, mat, cur) : plane_a(p, g, mat, STEP == 1 ? 0 : 2);
   const half* bl = STEP == 0 ? plane_x(p, g, mat, cur + 1) : plane_a(p, g, mat, STEP == 1 ? 1 : 3);
   const half* ah = STEP == 2 ? plane_x(p, g, mat, cur) : bh;
   const half* al = STEP == 2 ? plane_x(p, g, mat, cur + 1) : bl;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int r0 = ti * 128, c0 = tj * 128;
+  const int r0 = ti * TS, c0 = tj * TS;
 
-  // wave w fills chunks w and w + 4 (64 pieces each) of every plane
-  const half* src[NPL][2];
+  // wave w fills chunks w, w + NW, .. (64 pieces each) of every plane.  A lane's piece is at a constant offset; the slab's
+  // start goes into the descriptor (64-bit pointers kept for every request cost the 256 tile its accumulators' registers).
+  int at[2][NI];                                           // B, A
 #pragma unroll
-  for (int pl = 0; pl < NPL; ++pl)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = (4 * i + w) * 64 + lane;
-      const bool a = pl >= PA0;
-      const half* base = pl == 0 ? bh : (BLO && pl == PB1) ? bl : pl == PA0 ? ah : al;
-      if (STEP == 2 && a) {
-        const int r = q / 16, c = min(c0 + 8 * ((q & 15) ^ LC::swz(r)), ldn - 8);
-        src[pl][i] = base + (long long)r * ldn + c;       // r < 32: rows behind m are met at the last slab only (below)
-      } else {
-        const int r = q / 4, c = (q & 3) ^ LR::swz(r);
-        src[pl][i] = base + (long long)min((a ? c0 : r0) + r, m - 1) * ld + 8 * c;
-      }
+  for (int i = 0; i < NI; ++i) {
+    const int q = (NW * i + w) * 64 + lane, r = q / (TK / 8), c = (q % (TK / 8)) ^ LR::swz(r);
+    at[0][i] = (int)(2u * ((unsigned)(r0 + r) * sk + 8 * c));       // planes have less than 2^32 bytes
+    at[1][i] = (int)(2u * ((unsigned)(c0 + r) * sk + 8 * c));
+    if (STEP == 2) {
+      const int rk = q / (TS / 8), ck = c0 + 8 * ((q % (TS / 8)) ^ LC::swz(rk));
+      at[1][i] = 2 * (rk * sn + ck);
     }
-  auto fetch = [&](half (&dst)[NPL][128 * TK], int k0) {
+  }
+  auto fetch = [&](half (&dst)[NPL][TS * TK], int k0) {
 #pragma unroll
-    for (int pl = 0; pl < NPL; ++pl)
+    for (int pl = 0; pl < NPL; ++pl) {
+      [[maybe_unused]] const half* base = pl == 0 ? bh : (LO && pl == PB1) ? bl : pl == PA0 ? ah : al;
+      const long long from = STEP == 2 && pl >= PA0 ? (long long)k0 * sn : k0;
+      [[maybe_unused]] const long long bytes = 2 * ((STEP == 2 && pl >= PA0 ? (long long)m * sn : (long long)m * sk) - from);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const half* s;
-        if (STEP == 2 && pl >= PA0) {
-          const int r = ((4 * i + w) * 64 + lane) / 16;
-          s = src[pl][i] + (long long)(min(k0 + r, m - 1) - r) * ldn;
-        } else s = src[pl][i] + k0;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s,
-                                         (LDS3 void*)(dst[pl] + (4 * i + w) * 512), 16, 0, 0);
-      }
+      for (int i = 0; i < NI; ++i)
+        REQUEST(base + from, k0 < ld && bytes > 0 ? (int)(unsigned)bytes : 0, dst[pl] + (NW * i + w) * 512, 16, at[pl >= PA0][i]);
+    }
     __builtin_amdgcn_sched_barrier(0);                     // the requests leave before the work on the other buffer starts
   };
   // first operand from a tile of contraction rows x columns, in contraction order 16 s + 8 h + 0 .. 7 as row_frag gives it
@@ -377,42 +375,50 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
     for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
     return __builtin_bit_cast(h16x8, v);
   };
-  const int wr = 64 * (w >> 1), wc = 64 * (w & 1);
-  f32x16 acc[2][2];
+  const int wr = (TS / 2) * (w / (NW / 2)), wc = 64 * (w % (NW / 2));
+  f32x16 acc[NB][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  auto work = [&](half (&t)[NPL][128 * TK]) {
+  auto work = [&](half (&t)[NPL][TS * TK]) {
 #pragma unroll
     for (int s = 0; s < TK / 16; ++s) {
-      h16x8 b0[2], b1[2], a0[2], a1[2];
+      h16x8 a0[2], a1[2], b0 = LR::row_frag(t[0], wr, s, lane), b1 = LO ? LR::row_frag(t[PB1], wr, s, lane) : b0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        b0[i] = LR::row_frag(t[0], wr + 32 * i, s, lane);
-        if (BLO) b1[i] = LR::row_frag(t[PB1], wr + 32 * i, s, lane);
         a0[i] = STEP != 2 ? LR::row_frag(t[PA0], wc + 32 * i, s, lane) : col(t[PA0], s, wc + 32 * i);
-        if (ALO) a1[i] = STEP != 2 ? LR::row_frag(t[PA1 < NPL ? PA1 : 0], wc + 32 * i, s, lane) : col(t[PA1 < NPL ? PA1 : 0], s, wc + 32 * i);
+        if (LO) a1[i] = STEP != 2 ? LR::row_frag(t[PA1], wc + 32 * i, s, lane) : col(t[PA1], s, wc + 32 * i);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < NB; ++i) {
+        const h16x8 c0 = b0, c1 = b1;
+        if (i + 1 < NB) {
+          b0 = LR::row_frag(t[0], wr + 32 * (i + 1), s, lane);
+          if (LO) b1 = LR::row_frag(t[PB1], wr + 32 * (i + 1), s, lane);
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          acc[i][j] = O::mma(a0[j], b0[i], acc[i][j]);
-          if (ALO) acc[i][j] = O::mma(a1[j], b0[i], acc[i][j]);
-          if (BLO) acc[i][j] = O::mma(a0[j], b1[i], acc[i][j]);
+          acc[i][j] = O::mma(a0[j], c0, acc[i][j]);
+          if (LO) acc[i][j] = O::mma(a1[j], c0, acc[i][j]);
+          if (LO) acc[i][j] = O::mma(a0[j], c1, acc[i][j]);
         }
+        if (TS == 256) __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
+  // two slabs a turn; an odd number ends with a slab of zeros (a second exit from the loop makes the compiler keep two
+  // copies of the accumulators)
+  const int slabs = ld / TK;                               // ld is a multiple of 64
   fetch(buf0, 0);
-  for (int k0 = 0; k0 < ld; k0 += 2 * TK) {                // ld is a multiple of 64
+  for (int k = 0; k < slabs; k += 2) {
     arrive_barrier();                                      // buf0 has arrived, buf1 is no longer read
-    fetch(buf1, k0 + TK);
+    fetch(buf1, (k + 1) * TK);
     work(buf0);
     arrive_barrier();
-    if (k0 + 2 * TK < ld) fetch(buf0, k0 + 2 * TK);
+    if (k + 2 < slabs) fetch(buf0, (k + 2) * TK);
     work(buf1);
   }
   const bool mirror = STEP != 2 && ti != tj;
@@ -420,9 +426,9 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
   if (STEP == 0) { oh = plane_a(p, g, mat, 0); ol = plane_a(p, g, mat, 1); }
   else if (STEP == 1) { oh = plane_a(p, g, mat, 2); ol = plane_a(p, g, mat, 3); }
   else { oh = plane_x(p, g, mat, 2 - cur); ol = plane_x(p, g, mat, 3 - cur); }
-  const int lo_out = STEP == 2 ? ldn : ldm;
+  const int lo_out = STEP == 2 ? ldn : ldm, so = STEP == 2 ? sn : sm;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -438,8 +444,8 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= SA / (SX * SX);
         } else if (STEP == 1 && in) {
-          const h16x4 xh = *reinterpret_cast<const h16x4*>(bh + (long long)r * ldm + c);
-          const h16x4 xl = *reinterpret_cast<const h16x4*>(bl + (long long)r * ldm + c);
+          const h16x4 xh = *reinterpret_cast<const h16x4*>(bh + (long long)r * sm + c);
+          const h16x4 xl = *reinterpret_cast<const h16x4*>(bl + (long long)r * sm + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             v[e] = __builtin_fmaf(cc / SA, v[e], cb * ((float)xh[e] + (float)xl[e])) + (FULL && r == c + e ? ca * SA : 0.f);
@@ -447,8 +453,8 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= 1.f / SA;
           if (!FULL) {
-            const h16x4 xh = *reinterpret_cast<const h16x4*>(ah + (long long)r * ldn + c);
-            const h16x4 xl = *reinterpret_cast<const h16x4*>(al + (long long)r * ldn + c);
+            const h16x4 xh = *reinterpret_cast<const h16x4*>(ah + (long long)r * sn + c);
+            const h16x4 xl = *reinterpret_cast<const h16x4*>(al + (long long)r * sn + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ca, (float)xh[e] + (float)xl[e], v[e]);
           }
@@ -465,13 +471,13 @@ __global__ __launch_bounds__(256, 2) void ortho_product(const OrthoP p, const in
 #pragma unroll
         for (int e = 0; e < 4; ++e) { half a, b; split2(v[e], a, b); vh[e] = a; vl[e] = b; }
         if (in) {
-          *reinterpret_cast<h16x4*>(oh + (long long)r * lo_out + c) = vh;
-          *reinterpret_cast<h16x4*>(ol + (long long)r * lo_out + c) = vl;
+          *reinterpret_cast<h16x4*>(oh + (long long)r * so + c) = vh;
+          *reinterpret_cast<h16x4*>(ol + (long long)r * so + c) = vl;
         }
         if (mirror) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c + e < m) { oh[(long long)(c + e) * lo_out + r] = vh[e]; ol[(long long)(c + e) * lo_out + r] = vl[e]; }
+            if (c + e < m) { oh[(long long)(c + e) * so + r] = vh[e]; ol[(long long)(c + e) * so + r] = vl[e]; }
         }
       }
 }
@@ -491,23 +497,31 @@ template <typename F> unsigned grid_of(const OrthoP& p, int cuts, F tiles) {
   return (unsigned)(8 * most);
 }
 
-template <typename T, bool FULL> int run_tiled(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
+// TS: tile of P X; the symmetric products, which have far fewer tiles, take 256 only where there are two per compute unit
+template <typename T, bool FULL, int TS> int run_tiled(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
   int load_tiles = 0, cuts = 1;
   for (int i = 0; i < p.ngroups; ++i) {
     const int t = p.g[i].ldn / 64 * (p.g[i].ldm / 64);
     if (t > load_tiles) load_tiles = t;
   }
   while (cuts < 8 && p.matrices * cuts < 64) cuts *= 2;
-  const unsigned sym = grid_of(p, cuts, [](const OrthoG& g) { const int tm = (g.m + 127) / 128; return tm * (tm + 1) / 2; });
-  const unsigned full = grid_of(p, cuts, [](const OrthoG& g) { return (g.m + 127) / 128 * ((g.ldn + 127) / 128); });
+  auto sym = [&](int ts) { return grid_of(p, cuts, [=](const OrthoG& g) { const int tm = (g.m + ts - 1) / ts; return tm * (tm + 1) / 2; }); };
+  const unsigned sym_ts = sym(TS), sym_128 = sym(128);
+  const bool wide = TS == 128 || sym_ts >= 512;
+  const unsigned full = grid_of(p, cuts, [](const OrthoG& g) { return (g.m + TS - 1) / TS * ((g.ldn + TS - 1) / TS); });
   ortho_sumsq<T><<<dim3(p.matrices, ORTHO_PARTS), 256, 0, st>>>(p);
   ortho_load<T><<<dim3(load_tiles, p.matrices), 256, 0, st>>>(p);
   for (int s = 0; s < steps; ++s) {
     const int cur = 2 * (s & 1), last = s == steps - 1;
     const float a = coef[3 * s], b = coef[3 * s + 1], c = coef[3 * s + 2];
-    ortho_product<T, 0, FULL><<<dim3(sym), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
-    ortho_product<T, 1, FULL><<<dim3(sym), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
-    ortho_product<T, 2, FULL><<<dim3(full), 256, 0, st>>>(p, cuts, cur, last, a, b, c);
+    if (wide) {
+      ortho_product<T, 0, FULL, TS><<<dim3(sym_ts), 2 * TS, 0, st>>>(p, cuts, cur, 0, a, b, c);
+      ortho_product<T, 1, FULL, TS><<<dim3(sym_ts), 2 * TS, 0, st>>>(p, cuts, cur, 0, a, b, c);
+    } else {
+      ortho_product<T, 0, FULL, 128><<<dim3(sym_128), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
+      ortho_product<T, 1, FULL, 128><<<dim3(sym_128), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
+    }
+    ortho_product<T, 2, FULL, TS><<<dim3(full), 2 * TS, 0, st>>>(p, cuts, cur, last, a, b, c);
   }
   return hipGetLastError() != hipSuccess;
 }
@@ -522,12 +536,17 @@ template <typename T, int MT> int run_small(const OrthoP& p, const OrthoCoef& co
   return hipGetLastError() != hipSuccess;
 }
 
-// the stacks of p in one class: small with mt row tiles, or (0) too large for one workgroup
-OrthoP only(const OrthoP& p, int mt) {
+// How a stack is worked on: in one workgroup with 2, 4, 6 or 8 row tiles of 16, or with tiles of 128 (256: m >= 1024) and,
+// for bf16 results (+ 1) of m >= 256, fewer instructions a product (below that it costs precision and saves nothing)
+int class_of(const OrthoG& g, bool bf16) {
+  if (ortho_is_small(g)) return (g.m + 31) / 32 * 2;
+  return (g.m >= 1024 ? 256 : 128) + (bf16 && g.m >= 256);
+}
+OrthoP only(const OrthoP& p, bool bf16, int cls) {
   OrthoP q = p;
   q.ngroups = 0; q.matrices = 0;
   for (int i = 0; i < p.ngroups; ++i)
-    if ((ortho_is_small(p.g[i]) ? (p.g[i].m + 31) / 32 * 2 : 0) == mt) {
+    if (class_of(p.g[i], bf16) == cls) {
       q.g[q.ngroups] = p.g[i];
       q.g[q.ngroups++].first = q.matrices;
       q.matrices += p.g[i].count;
@@ -535,15 +554,17 @@ OrthoP only(const OrthoP& p, int mt) {
   return q;
 }
 
-template <typename T, bool FULL> int run(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
+template <typename T> int run(const OrthoP& p, int steps, const float* coef, hipStream_t st) {
+  constexpr bool BF16 = __is_same(T, __bf16);
   OrthoCoef co;
   co.steps = steps;
   for (int i = 0; i < 3 * steps; ++i) co.c[i] = coef[i];
-  for (int mt = 0; mt <= 8; mt += 2) {
-    const OrthoP q = only(p, mt);
+  for (int cls : {256 + BF16, 128 + 1, 128, 8, 6, 4, 2}) {
+    const OrthoP q = only(p, BF16, cls);
     if (!q.ngroups) continue;
-    const int rc = mt == 0 ? run_tiled<T, FULL>(q, steps, coef, st) : mt == 2 ? run_small<T, 2>(q, co, st) :
-                   mt == 4 ? run_small<T, 4>(q, co, st) : mt == 6 ? run_small<T, 6>(q, co, st) : run_small<T, 8>(q, co, st);
+    const int rc = cls >= 256 ? run_tiled<T, !BF16, 256>(q, steps, coef, st) : cls == 128 + 1 ? run_tiled<T, !BF16, 128>(q, steps, coef, st) :
+                   cls == 128 ? run_tiled<T, true, 128>(q, steps, coef, st) : cls == 8 ? run_small<T, 8>(q, co, st) :
+                   cls == 6 ? run_small<T, 6>(q, co, st) : cls == 4 ? run_small<T, 4>(q, co, st) : run_small<T, 2>(q, co, st);
     if (rc) return rc;
   }
   return 0;
@@ -557,14 +578,13 @@ size_t ortho_ws_bytes(OrthoP& p) {
   long long at = 0;
   for (int i = 0; i < p.ngroups; ++i) {
     p.g[i].ws = at;
-    if (!ortho_is_small(p.g[i])) at += (long long)p.g[i].count * (4LL * p.g[i].m * p.g[i].ldn + 4LL * p.g[i].m * p.g[i].ldm);
+    if (!ortho_is_small(p.g[i])) at += (long long)p.g[i].count * (4LL * p.g[i].m * (p.g[i].sn + p.g[i].sm));
   }
   return (size_t)at * 2 + (size_t)p.matrices * ORTHO_PARTS * sizeof(double) + 256;
 }
 
 int launch_ortho(const OrthoP& p, int dtype, int steps, const float* coef, hipStream_t st) {
-  return dtype == OP_F32 ? run<float, true>(p, steps, coef, st)
-                         : dtype == OP_BF16 ? run<__bf16, false>(p, steps, coef, st) : run<half, true>(p, steps, coef, st);
+  return dtype == OP_F32 ? run<float>(p, steps, coef, st) : dtype == OP_BF16 ? run<__bf16>(p, steps, coef, st) : run<half>(p, steps, coef, st);
 }
 
 // ---- orthogonalised momentum: what goes in and what comes out, one pass each, bound by memory -------

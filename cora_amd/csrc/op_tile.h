@@ -9,6 +9,15 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 #define LDS3 __attribute__((address_space(3)))
 
+// Direct requests of 16 or 4 bytes a lane: the lane's bytes at base + at go to lds + 16 (4) * lane, zeros where at is behind
+// `bytes`.  (The host pass has no buffer descriptor type and silently drops kernels that name one.)
+#ifdef __HIP_DEVICE_COMPILE__
+#define REQUEST(base, bytes, lds, n, at) \
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)(base), 0, bytes, 0x00020000), (LDS3 void*)(lds), n, at, 0, 0, 0)
+#else
+#define REQUEST(base, bytes, lds, n, at) (void)0
+#endif
+
 template <typename T> struct Op;
 template <> struct Op<float> {
   typedef f32x4 frag;
@@ -62,7 +71,7 @@ template <typename T, int D> struct Tile {
       if (D == 64 || D == 128) return (r & 3) | (((r >> 3) & 1) << 2) | (((r >> 2) & 1) << 3);
       return (r >> 1) & 7;
     }
-    const int hi = D == 128 ? (r & 3) : (D == 64 ? ((r >> 1) & 1) : 0);
+    const int hi = D >= 128 ? (r & 3) : (D == 64 ? ((r >> 1) & 1) : 0);
     return ((r >> 2) & 3) | (hi << 2);
   }
   static __device__ __forceinline__ int at(int r, int c) { return r * D + ((c ^ swz(r)) * E); }   // element offset of a piece

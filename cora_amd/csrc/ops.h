@@ -39,11 +39,12 @@ int launch_attention_fwd(const AttnP& p, int dtype, hipStream_t st);
 int launch_attention_bwd(const AttnP& p, int dtype, hipStream_t st);
 
 // ---- orthogonalisation of updates ----------------------------------------------------------------
-constexpr int ORTHO_GROUPS = 16, ORTHO_STEPS = 32, ORTHO_PARTS = 64;
+constexpr int ORTHO_GROUPS = 16, ORTHO_STEPS = 32, ORTHO_PARTS = 256;
 struct OrthoG {                 // a stack of equal matrices; m = min(rows, cols), n = max
   const void* x; void* y;
   long long xm, xr, ym, yr;     // strides in elements: matrix, row
   int count, rows, cols, m, n, ldn, ldm, first;   // ldn, ldm: n, m rounded up to 64; first: matrices of the groups before
+  int sn, sm;                   // row strides of the n and m columns wide planes: odd multiples of 128 bytes (op_ortho.hip)
   long long ws;                 // first 16-bit element of its matrices in the workspace
 };
 struct OrthoP {

@@ -125,7 +125,8 @@ def ortho_bound(G, steps, coef, eps, dtype):
     """Relative Frobenius error the kernels may make: four times what independent errors of the size of every rounding they
     make do to the exact iteration, plus the result's own rounding.  Roundings: X, A, P to 22 bits (2^-22; lower halves
     times lower halves are left out, 2^-22 more of every product) and sums of K terms in fp32 (sqrt(K) U of the product of
-    absolute values, as independent roundings add up); bfloat16: A from 11-bit X (2^-12 a factor), P X from 11-bit P."""
+    absolute values, as independent roundings add up); bfloat16 with min(rows, cols) >= 256: A from 11-bit X (2^-12 a factor),
+    (b A + c A^2) X from 11-bit factors, a X from X itself."""
     gen = torch.Generator().manual_seed(1)
     noise = lambda t, rel: t * (1 + rel * (2 * torch.rand(t.shape, generator=gen, dtype=torch.float64) - 1))
     X = G.double()
@@ -134,7 +135,7 @@ def ortho_bound(G, steps, coef, eps, dtype):
     E = X.clone()
     m, n = X.shape
     eye = torch.eye(m, dtype=torch.float64)
-    low = dtype == torch.bfloat16
+    low = dtype == torch.bfloat16 and m >= 256
 
     def prod(L, R, rel):
         mag = (L.abs() @ R.abs()) * (2.0 ** -22 + math.sqrt(L.shape[1]) * U)
@@ -147,6 +148,6 @@ def ortho_bound(G, steps, coef, eps, dtype):
         A = prod(N, N.T, 2.0 ** -12 if low else 2.0 ** -22)
         A = noise((A + A.T) / 2, 2.0 ** -22)
         P = b * A + c * prod(A, A, 2.0 ** -22)
-        X = a * N + prod(noise(P, 2.0 ** -12), N, 0.0) if low else prod(a * eye + P, N, 2.0 ** -22)
+        X = a * N + prod(P, N, 2.0 ** -12) if low else prod(a * eye + P, N, 2.0 ** -22)
     norm = E.norm().clamp_min(1e-300)
     return 4 * float((X - E).norm() / norm) + half_eps(dtype) + 2.0 ** -22

@@ -299,7 +299,7 @@ def test_refusals_on_the_gpu():
 
 
 # ---- orthogonalisation -----------------------------------------------------------------------------------------------
-SHAPES = [(1, 1), (1, 70), (70, 1), (13, 22), (64, 64), (64, 256), (256, 64), (100, 37), (128, 128), (129, 200), (200, 320), (333, 130)]
+SHAPES = [(1, 1), (1, 70), (70, 1), (13, 22), (64, 64), (64, 256), (256, 64), (100, 37), (128, 128), (129, 200), (200, 320), (333, 130), (300, 520), (1030, 1100), (2100, 1025)]
 
 
 def gradient(r, c, seed, scale=1e-3):
