@@ -111,10 +111,10 @@ __global__ __launch_bounds__(256) void ortho_load(const OrthoP p) {
 }
 
 // ---- matrices that fit one compute unit's LDS ----------------------------------------------------
-// All steps of one matrix in one workgroup of 16 waves: X, then A and P in A's place, as two fp16 planes each in LDS; 16 x 16
-// tiles (v_mfma_f32_16x16x32_f16), three instructions a product for every type.  A wave keeps whole columns of X, so
-// X <- P X happens in place.  Bound by the chain of 3 products and 4 barriers a step, about 1.5 us; against the tiled path
-// this saves its 2 + 3 * steps launches.
+// All steps of one matrix in one workgroup of 8 waves: X, then A and P in A's place, as two fp16 planes each in LDS; 32 x 32
+// tiles, three instructions a product for every type.  What a step costs is the chain of its three products, the splitting
+// of their results into halves and 5 barriers: 2.5 us at 64 x 64, 4.4 at 64 x 256, 9.7 at 128 x 128 (16 x 16 tiles on 16 waves:
+// 2.4, 4.9, 14).  Against the tiled path this saves 2 + 3 steps launches: the 6-block model's 36 updates 38 us instead of 156.
 // Rows are padded to a stride of 80 bytes mod 256 (the 16 rows of a row read start 16 bytes apart mod 256, the 4 rows of a
 // transposing read 80 apart) or, where that does not fit, to 16 mod 256.
 constexpr int SMALL_LDS = 160 * 1024 - 256;
@@ -130,111 +130,118 @@ __host__ __device__ inline SmallDim small_dim(int m, int n) {
   return d;
 }
 
-// the steps, for matrices of MT row tiles
-template <typename T, int MT>
-__device__ __forceinline__ void small_steps(half* lds, const OrthoG& g, const SmallDim d, T* y, const OrthoCoef& co) {
-  constexpr int MP = 16 * MT, NZ = (MT * MT + 15) / 16;    // tiles of A per wave
-  const int m = g.m, n = g.n, np = d.np, sx = d.sx, sa = d.sa;
-  const long long yr = g.yr;
-  const bool tall = g.rows > g.cols;
+// the steps, for matrices of RT row tiles and X of at most 8 XT tiles
+template <int RT, int XT>
+__device__ __forceinline__ void small_steps(half* lds, const SmallDim d, const OrthoCoef& co) {
+  constexpr int MP = 32 * RT, NZ = (RT * RT + 7) / 8;      // tiles of A per wave
+  typedef Op<half> O;
+  const int np = d.np, sx = d.sx, sa = d.sa, units = np / 32 * RT;
   half *xh = lds, *xl = xh + MP * sx, *ah = xl + MP * sx, *al = ah + MP * sa;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g16 = lane >> 4;
-  // 16 x 32 operand pieces: lane holds index l & 15, contraction 8 (l >> 4) + 0 .. 7
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, h = lane >> 5;
+  // 32 x 16 operand pieces: lane holds index l & 31, contraction 8 (l >> 5) + 0 .. 7
   auto row = [&](const half* t, int stride, int i0, int k0) {
-    return *reinterpret_cast<const h16x8*>(t + (i0 + r16) * stride + k0 + 8 * g16);
+    return *reinterpret_cast<const h16x8*>(t + (i0 + r32) * stride + k0 + 8 * h);
   };
-  auto col = [&](const half* t, int stride, int k0, int j0) {
-    const half* q = t + (k0 + 8 * g16 + (r16 >> 2)) * stride + j0 + 4 * (r16 & 3);
+  auto col = [&](const half* t, int k0, int j0) {
+    const int i = lane & 15;
+    const half* q = t + (k0 + 8 * h + (i >> 2)) * sx + j0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
     s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS3 s16x4*)q);
-    s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS3 s16x4*)(q + 4 * stride));
+    s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS3 s16x4*)(q + 4 * sx));
     s16x8 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
     return __builtin_bit_cast(h16x8, v);
   };
-  auto mma = [](h16x8 a, h16x8 b, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0); };
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  // four neighbouring columns of a lane's row, split
-  auto put = [&](half* hi, half* lo, int o, f32x4 v) {
-    h16x4 vh, vl;
+  auto zero = [](f32x16& v) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { half a, b; split2(v[e], a, b); vh[e] = a; vl[e] = b; }
-    *reinterpret_cast<h16x4*>(hi + o) = vh;
-    *reinterpret_cast<h16x4*>(lo + o) = vl;
+    for (int r = 0; r < 16; ++r) v[r] = 0.f;
+  };
+  // hi hi + hi lo + lo hi over `len` values (a multiple of 32) of the contraction; the operands of the next 32 are under way
+  // while the current ones are multiplied
+  auto product = [&](f32x16& acc, int len, auto first, auto second) {
+    zero(acc);
+    h16x8 a[4], b[4];
+    auto get = [&](h16x8 (&p)[4], h16x8 (&q)[4], int k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { p[e] = first(e & 1, k + 16 * (e >> 1)); q[e] = second(e & 1, k + 16 * (e >> 1)); }
+    };
+    get(a, b, 0);
+#pragma unroll 1
+    for (int k = 32; k <= len; k += 32) {
+      h16x8 an[4], bn[4];
+      get(an, bn, k < len ? k : 0);
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        acc = O::mma(a[e], b[e], acc); acc = O::mma(a[e + 1], b[e], acc); acc = O::mma(a[e], b[e + 1], acc);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { a[e] = an[e]; b[e] = bn[e]; }
+    }
+  };
+  // a lane's four times four columns of its row, times f, split
+  auto put = [&](half* hi, half* lo, int o, const f32x16& v, float f) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      h16x4 vh, vl;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { half a, b; split2(v[4 * q + e] * f, a, b); vh[e] = a; vl[e] = b; }
+      *reinterpret_cast<h16x4*>(hi + o + 8 * q) = vh;
+      *reinterpret_cast<h16x4*>(lo + o + 8 * q) = vl;
+    }
   };
   for (int step = 0; step < co.steps; ++step) {
     const float ca = co.c[3 * step], cb = co.c[3 * step + 1], cc = co.c[3 * step + 2];
-    f32x4 pt[NZ];
+    f32x16 pt[NZ];
     __syncthreads();
 #pragma unroll
     for (int z = 0; z < NZ; ++z) {                         // A = X X^T
-      const int t = w + 16 * z;
-      if (MT * MT % 16 && t >= MT * MT) continue;
-      const int i = 16 * (t / MT), j = 16 * (t % MT);
-      f32x4 hh = zero, hl = zero, lh = zero;
-      for (int k = 0; k < np; k += 32) {
-        const h16x8 a0 = row(xh, sx, j, k), a1 = row(xl, sx, j, k), b0 = row(xh, sx, i, k), b1 = row(xl, sx, i, k);
-        hh = mma(a0, b0, hh); hl = mma(a0, b1, hl); lh = mma(a1, b0, lh);
-      }
-      put(ah, al, (i + r16) * sa + j + 4 * g16, (hh + (hl + lh)) * (SA / (SX * SX)));
+      const int t = w + 8 * z, i = 32 * (t / RT), j = 32 * (t % RT);
+      if (t >= RT * RT) continue;
+      product(pt[z], np, [&](int lo, int k) { return row(lo ? xl : xh, sx, j, k); }, [&](int lo, int k) { return row(lo ? xl : xh, sx, i, k); });
+      put(ah, al, (i + r32) * sa + j + 4 * h, pt[z], SA / (SX * SX));
     }
     __syncthreads();
 #pragma unroll
     for (int z = 0; z < NZ; ++z) {                         // P = a I + b A + c A A
-      const int t = w + 16 * z;
-      if (MT * MT % 16 && t >= MT * MT) continue;
-      const int i = 16 * (t / MT), j = 16 * (t % MT), r = i + r16, c = j + 4 * g16;
-      f32x4 hh = zero, hl = zero, lh = zero;
+      const int t = w + 8 * z, i = 32 * (t / RT), j = 32 * (t % RT);
+      if (t >= RT * RT) continue;
+      product(pt[z], MP, [&](int lo, int k) { return row(lo ? al : ah, sa, j, k); }, [&](int lo, int k) { return row(lo ? al : ah, sa, i, k); });
 #pragma unroll
-      for (int k = 0; k < MP; k += 32) {
-        const h16x8 a0 = row(ah, sa, j, k), a1 = row(al, sa, j, k), b0 = row(ah, sa, i, k), b1 = row(al, sa, i, k);
-        hh = mma(a0, b0, hh); hl = mma(a0, b1, hl); lh = mma(a1, b0, lh);
+      for (int q = 0; q < 4; ++q) {
+        const int r = i + r32, c = j + 8 * q + 4 * h;
+        const h16x4 vh = *reinterpret_cast<const h16x4*>(ah + r * sa + c), vl = *reinterpret_cast<const h16x4*>(al + r * sa + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          pt[z][4 * q + e] = __builtin_fmaf(cc / SA, pt[z][4 * q + e], cb * ((float)vh[e] + (float)vl[e])) + (r == c + e ? ca * SA : 0.f);
       }
-      const h16x4 vh = *reinterpret_cast<const h16x4*>(ah + r * sa + c), vl = *reinterpret_cast<const h16x4*>(al + r * sa + c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        pt[z][e] = __builtin_fmaf(cc / SA, hh[e] + (hl[e] + lh[e]), cb * ((float)vh[e] + (float)vl[e])) + (r == c + e ? ca * SA : 0.f);
     }
     __syncthreads();
 #pragma unroll
     for (int z = 0; z < NZ; ++z) {
-      const int t = w + 16 * z;
-      if (MT * MT % 16 && t >= MT * MT) continue;
-      put(ah, al, (16 * (t / MT) + r16) * sa + 16 * (t % MT) + 4 * g16, pt[z]);
+      const int t = w + 8 * z, i = 32 * (t / RT), j = 32 * (t % RT);
+      if (t < RT * RT) put(ah, al, (i + r32) * sa + j + 4 * h, pt[z], 1.f);
     }
     __syncthreads();
-    for (int j = 16 * w; j < np; j += 256) {               // X <- P X, 16 columns at a time
-      f32x4 hh[MT], lo[MT];
+    f32x16 xt[XT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) { hh[i] = zero; lo[i] = zero; }
+    for (int z = 0; z < XT; ++z) {                         // X <- P X: row tile u % RT of columns 32 (u / RT) ..
+      const int u = w + 8 * z, i = 32 * (u % RT), j = 32 * (u / RT);
+      if (u >= units) continue;
+      product(xt[z], MP, [&](int lo, int k) { return col(lo ? xl : xh, k, j); }, [&](int lo, int k) { return row(lo ? al : ah, sa, i, k); });
+    }
+    __syncthreads();                                       // X has been read
 #pragma unroll
-      for (int k = 0; k < MP; k += 32) {
-        const h16x8 a0 = col(xh, sx, k, j), a1 = col(xl, sx, k, j);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const h16x8 b0 = row(ah, sa, 16 * i, k), b1 = row(al, sa, 16 * i, k);
-          hh[i] = mma(a0, b0, hh[i]); lo[i] = mma(a1, b0, lo[i]); lo[i] = mma(a0, b1, lo[i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int r = 16 * i + r16, c = j + 4 * g16;
-        const f32x4 v = hh[i] + lo[i];
-        if (step == co.steps - 1) {
-          if (r < m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c + e < n) y[tall ? (c + e) * yr + r : r * yr + c + e] = (T)(v[e] * (1.f / (SA * SX)));
-        } else put(xh, xl, r * sx + c, v * (1.f / SA));
-      }
+    for (int z = 0; z < XT; ++z) {
+      const int u = w + 8 * z;
+      if (u < units) put(xh, xl, (32 * (u % RT) + r32) * sx + 32 * (u / RT) + 4 * h, xt[z], 1.f / SA);
     }
   }
 }
 
-template <typename T, int MT>
-__global__ __launch_bounds__(1024) void ortho_small(const OrthoP p, const OrthoCoef co) {
+template <typename T, int RT, int XT>
+__global__ __launch_bounds__(512) void ortho_small(const OrthoP p, const OrthoCoef co) {
   extern __shared__ __attribute__((aligned(16))) half lds[];
-  __shared__ double red[16];
+  __shared__ double red[8];
   const int id = blockIdx.x;
   int gi = 0;
   while (gi + 1 < p.ngroups && id >= p.g[gi + 1].first) ++gi;
@@ -248,34 +255,53 @@ __global__ __launch_bounds__(1024) void ortho_small(const OrthoP p, const OrthoC
 
   // The matrix goes to its place with its bits halved between the planes and is scaled and split there once its norm is
   // known.  Loops are kept short: a workgroup lives for some 10 us and fetches its code cold.
-  for (int i = tid; i < d.mp * sx / 4; i += 1024) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0u, 0u, 0u, 0u);   // both planes
+  for (int i = tid; i < d.mp * sx / 4; i += 512) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0u, 0u, 0u, 0u);   // both planes
   __syncthreads();
+  // four neighbouring elements a lane where rows allow it, else one; eight of them under way at a time
   double s = 0.0;
-  const int dr = 1024 / cols, dc = 1024 - dr * cols;       // element tid + 1024 i: its row and column step by these
-  int r = tid / cols, c = tid - r * cols;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const bool wide = cols % 4 == 0 && xr % 4 == 0 && (uintptr_t)x % sizeof(vec4) == 0;
+  const int per = wide ? 4 : 1, cv = cols / per;           // vectors a row
+  const int dr = 512 / cv, dc = 512 - dr * cv;             // vector tid + 512 i: its row and column step by these
+  int r = tid / cv, c = tid - r * cv;
   while (r < rows) {
-    float v[8]; int o[8];
+    float v[8][4]; int o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = r < rows ? (float)x[r * xr + c] : 0.f;
-      o[i] = r < rows ? (tall ? c * sx + r : r * sx + c) : -1;
+      o[i] = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
+      if (r < rows) {
+        if (wide) {
+          const vec4 t = *reinterpret_cast<const vec4*>(x + r * xr + 4 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i][e] = (float)t[e];
+        } else v[i][0] = (float)x[r * xr + c];
+        o[i] = tall ? per * c * sx + r : r * sx + per * c;
+      }
       r += dr; c += dc;
-      if (c >= cols) { c -= cols; ++r; }
+      if (c >= cv) { c -= cv; ++r; }
     }
+    const int de = tall ? sx : 1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s += (double)v[i] * (double)v[i];
-      if (o[i] >= 0) { const unsigned u = __float_as_uint(v[i]); xh[o[i]] = (unsigned short)(u >> 16); xl[o[i]] = (unsigned short)u; }
-    }
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s += (double)v[i][e] * (double)v[i][e];
+        if (o[i] >= 0 && e < per) {
+          const unsigned u = __float_as_uint(v[i][e]);
+          xh[o[i] + e * de] = (unsigned short)(u >> 16); xl[o[i] + e * de] = (unsigned short)u;
+        }
+      }
   }
   s = wave_sum_d(s);
   if ((tid & 63) == 0) red[tid >> 6] = s;
   __syncthreads();
   s = 0.0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s += red[i];
+  for (int i = 0; i < 8; ++i) s += red[i];
   const double f = (double)SX / (sqrt(s) + (double)p.eps);
-  for (int i = tid; i < d.mp * sx / 4; i += 1024) {
+  for (int i = tid; i < d.mp * sx / 4; i += 512) {
     const ushort4 uh = reinterpret_cast<ushort4*>(xh)[i], ul = reinterpret_cast<ushort4*>(xl)[i];
     const unsigned u[4] = {(unsigned)uh.x << 16 | ul.x, (unsigned)uh.y << 16 | ul.y, (unsigned)uh.z << 16 | ul.z, (unsigned)uh.w << 16 | ul.w};
     h16x4 vh, vl;
@@ -283,22 +309,35 @@ __global__ __launch_bounds__(1024) void ortho_small(const OrthoP p, const OrthoC
     for (int e = 0; e < 4; ++e) { half a, b; split2((float)((double)__uint_as_float(u[e]) * f), a, b); vh[e] = a; vl[e] = b; }
     reinterpret_cast<h16x4*>(xh)[i] = vh; reinterpret_cast<h16x4*>(xl)[i] = vl;
   }
+  small_steps<RT, XT>(lds, d, co);
+  __syncthreads();
   T* y = (T*)g.y + (long long)(id - g.first) * g.ym;
-  small_steps<T, MT>(lds, g, d, y, co);
+  const long long yr = g.yr;
+  const int er = 512 / cols, ec = 512 - er * cols;
+  r = tid / cols; c = tid - r * cols;
+  while (r < rows) {
+    const int o = tall ? c * sx + r : r * sx + c;
+    y[r * yr + c] = (T)(((float)lds[o] + (float)lds[d.mp * sx + o]) * (1.f / SX));
+    r += er; c += ec;
+    if (c >= cols) { c -= cols; ++r; }
+  }
 }
 
 // One product for all matrices.  STEP 0: A = X X^T; 1: P = a I + b A + c A A; 2: X' = P X (last: to the caller's matrix).
-// Tile TS x TS: 128 with four waves of 64 x 64, two workgroups a compute unit; or 256 with eight waves of 128 x 64, which
-// halves what a flop reads from L2 (the 128 tile's 43 bytes a cycle and compute unit exceed it).  The first operand gives
+// Tile TS x TS: 64 with four waves of 32 x 32, for matrices that give few tiles; 128 with four waves of 64 x 64, two
+// workgroups a compute unit (the symmetric products of few wide matrices); or 256 with eight waves of 128 x 64, which halves what a flop reads from L2 (the 128 tile's 43
+// bytes a cycle and compute unit exceed it).  The first operand gives
 // the output's columns, the second its rows (op_tile.h), so a lane holds four neighbouring columns of one output row.  Slabs go from global memory straight into one
 // of two LDS buffers while the other is worked on; a lane fetches the 16-byte piece that belongs at its place of the
 // swizzled tile.  Rows outside a matrix arrive as zeros, columns behind it as whatever follows (the columns up to ldn and ldm
 // are stored as zeros, what lies behind gives nothing that is stored).
+constexpr int threads_of(int ts) { return ts == 256 ? 512 : 256; }
 template <typename T, int STEP, bool FULL, int TS>
-__global__ __launch_bounds__(2 * TS, 2) void ortho_product(const OrthoP p, const int cuts, const int cur, const int last, const float ca, const float cb, const float cc) {
+__global__ __launch_bounds__(threads_of(TS), 2) void ortho_product(const OrthoP p, const int cuts, const int cur, const int last, const float ca, const float cb, const float cc) {
   constexpr bool LO = FULL || STEP == 1;                  // both halves of both operands
   constexpr int NPL = LO ? 4 : 2, PB1 = 1, PA0 = LO ? 2 : 1, PA1 = LO ? 3 : 0;    // planes: B hi, (B lo,) A hi, (A lo)
-  constexpr int TK = LO ? 32 : 64, NW = TS / 32, NB = TS / 64, NI = TS * TK / 512 / NW;   // slab, waves, row tiles of a wave, requests of a wave and plane
+  constexpr int TK = LO && TS > 64 ? 32 : 64, NW = threads_of(TS) / 64, NI = TS * TK / 512 / NW;   // slab, waves, requests of a wave and plane
+  constexpr int NB = TS / 64, NA = TS / (NW / 2) / 32, CW = 32 * NA;       // row and column tiles of a wave, its columns
   typedef Tile<half, TK> LR; typedef Tile<half, TS> LC;
   typedef Op<half> O;
   __shared__ __attribute__((aligned(16))) half buf0[NPL][TS * TK];
@@ -375,20 +414,20 @@ __global__ __launch_bounds__(2 * TS, 2) void ortho_product(const OrthoP p, const
     for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
     return __builtin_bit_cast(h16x8, v);
   };
-  const int wr = (TS / 2) * (w / (NW / 2)), wc = 64 * (w % (NW / 2));
-  f32x16 acc[NB][2];
+  const int wr = (TS / 2) * (w / (NW / 2)), wc = CW * (w % (NW / 2));
+  f32x16 acc[NB][NA];
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NA; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   auto work = [&](half (&t)[NPL][TS * TK]) {
 #pragma unroll
     for (int s = 0; s < TK / 16; ++s) {
-      h16x8 a0[2], a1[2], b0 = LR::row_frag(t[0], wr, s, lane), b1 = LO ? LR::row_frag(t[PB1], wr, s, lane) : b0;
+      h16x8 a0[NA], a1[NA], b0 = LR::row_frag(t[0], wr, s, lane), b1 = LO ? LR::row_frag(t[PB1], wr, s, lane) : b0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < NA; ++i) {
         a0[i] = STEP != 2 ? LR::row_frag(t[PA0], wc + 32 * i, s, lane) : col(t[PA0], s, wc + 32 * i);
         if (LO) a1[i] = STEP != 2 ? LR::row_frag(t[PA1], wc + 32 * i, s, lane) : col(t[PA1], s, wc + 32 * i);
       }
@@ -400,7 +439,7 @@ __global__ __launch_bounds__(2 * TS, 2) void ortho_product(const OrthoP p, const
           if (LO) b1 = LR::row_frag(t[PB1], wr + 32 * (i + 1), s, lane);
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NA; ++j) {
           acc[i][j] = O::mma(a0[j], c0, acc[i][j]);
           if (LO) acc[i][j] = O::mma(a1[j], c0, acc[i][j]);
           if (LO) acc[i][j] = O::mma(a0[j], c1, acc[i][j]);
@@ -421,65 +460,113 @@ __global__ __launch_bounds__(2 * TS, 2) void ortho_product(const OrthoP p, const
     if (k + 2 < slabs) fetch(buf0, (k + 2) * TK);
     work(buf1);
   }
-  const bool mirror = STEP != 2 && ti != tj;
+  // Epilogue, 32 rows x CW columns of a wave at a time through its own piece of LDS, so that every row is read and written as
+  // whole 128-byte lines (stored as the matrix unit leaves them, 16 bytes a row and instruction, P X of the wide layers
+  // took 404 us instead of 244).  Place of the four columns 4 k of row r: k ^ (r mod CW / 4).
+  const bool mirror = STEP != 2 && ti != tj, tall = g.rows > g.cols;
   half *oh, *ol;
   if (STEP == 0) { oh = plane_a(p, g, mat, 0); ol = plane_a(p, g, mat, 1); }
   else if (STEP == 1) { oh = plane_a(p, g, mat, 2); ol = plane_a(p, g, mat, 3); }
   else { oh = plane_x(p, g, mat, 2 - cur); ol = plane_x(p, g, mat, 3 - cur); }
-  const int lo_out = STEP == 2 ? ldn : ldm, so = STEP == 2 ? sn : sm;
+  const int cols = STEP == 2 ? ldn : ldm, so = STEP == 2 ? sn : sm;
+  T* y = (T*)g.y + (long long)mat * g.ym;
+  constexpr int VT = 16 / (int)sizeof(T);                  // 16-byte pieces of the caller's rows
+  const bool vec = !tall && (uintptr_t)y % 16 == 0 && g.yr % VT == 0;
+  static_assert(sizeof buf0 >= NW * CW * 128, "the first buffer holds every wave's piece");
+  float* mine = reinterpret_cast<float*>(&buf0[0][0]) + w * (CW * 32);
+  auto place = [&](int r, int c4) { return mine + r * CW + ((c4 ^ (r & (CW / 4 - 1))) << 2); };
+  __syncthreads();                                         // the slabs are no longer read
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NA; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = r0 + wr + 32 * i + (lane & 31), c = c0 + wc + 32 * j + 8 * q + 4 * h;
-        // A and P: rows behind the matrix are zero, their mirror images fill the columns up to ldm
-        if (r >= (STEP == 2 ? m : ldm) || c >= lo_out) continue;
-        const bool in = r < m;
-        float v[4];
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(place(lane & 31, 8 * j + 2 * q + h)) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = in && (STEP == 2 || c + e < m) ? acc[i][j][4 * q + e] : 0.f;
-        if (STEP == 0) {
+    for (int z = 0; z < CW / 16; ++z) {
+      const int lr = 512 / CW * z + lane / (CW / 8), k4 = 2 * (lane % (CW / 8));
+      const int r = r0 + wr + 32 * i + lr, c = c0 + wc + 4 * k4;
+      // A and P: rows behind the matrix are zero, their mirror images fill the columns up to ldm
+      const bool in = r < m, some = r < (STEP == 2 ? m : ldm) && c < cols;
+      float v[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= SA / (SX * SX);
-        } else if (STEP == 1 && in) {
-          const h16x4 xh = *reinterpret_cast<const h16x4*>(bh + (long long)r * sm + c);
-          const h16x4 xl = *reinterpret_cast<const h16x4*>(bl + (long long)r * sm + c);
+      for (int e = 0; e < 8; e += 4) {
+        const f32x4 f = *reinterpret_cast<const f32x4*>(place(lr, k4 + e / 4));
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+        for (int x = 0; x < 4; ++x) v[e + x] = in && (STEP == 2 || c + e + x < m) ? f[x] : 0.f;
+      }
+      if (STEP == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= SA / (SX * SX);
+      } else if (STEP == 1) {
+        if (in && some) {
+          const h16x8 xh = *reinterpret_cast<const h16x8*>(bh + (long long)r * sm + c);
+          const h16x8 xl = *reinterpret_cast<const h16x8*>(bl + (long long)r * sm + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
             v[e] = __builtin_fmaf(cc / SA, v[e], cb * ((float)xh[e] + (float)xl[e])) + (FULL && r == c + e ? ca * SA : 0.f);
-        } else if (STEP == 2) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= 1.f / SA;
-          if (!FULL) {
-            const h16x4 xh = *reinterpret_cast<const h16x4*>(ah + (long long)r * sn + c);
-            const h16x4 xl = *reinterpret_cast<const h16x4*>(al + (long long)r * sn + c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ca, (float)xh[e] + (float)xl[e], v[e]);
-          }
         }
-        if (STEP == 2 && last) {
-          T* y = (T*)g.y + (long long)mat * g.ym;
-          const bool tall = g.rows > g.cols;
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < g.n) y[tall ? (long long)(c + e) * g.yr + r : (long long)r * g.yr + c + e] = (T)(v[e] * (1.f / SX));
-          continue;
-        }
-        h16x4 vh, vl;
+        for (int e = 0; e < 8; ++e) v[e] *= 1.f / SA;
+        if (!FULL && some) {
+          const h16x8 xh = *reinterpret_cast<const h16x8*>(ah + (long long)r * sn + c);
+          const h16x8 xl = *reinterpret_cast<const h16x8*>(al + (long long)r * sn + c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { half a, b; split2(v[e], a, b); vh[e] = a; vl[e] = b; }
-        if (in) {
-          *reinterpret_cast<h16x4*>(oh + (long long)r * so + c) = vh;
-          *reinterpret_cast<h16x4*>(ol + (long long)r * so + c) = vl;
-        }
-        if (mirror) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < m) { oh[(long long)(c + e) * so + r] = vh[e]; ol[(long long)(c + e) * so + r] = vl[e]; }
+          for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(ca, (float)xh[e] + (float)xl[e], v[e]);
         }
       }
+      if ((STEP == 2 && last && tall) || mirror) {         // the transpose is read from LDS below
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) *reinterpret_cast<f32x4*>(place(lr, k4 + e / 4)) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+      }
+      if (!some || !in) continue;
+      if (STEP == 2 && last) {
+        if (tall) continue;
+        T* row = y + (long long)r * g.yr + c;
+        if (vec && c + 8 <= g.n) {
+          typedef T vecT __attribute__((ext_vector_type(VT)));
+#pragma unroll
+          for (int e = 0; e < 8; e += VT) {
+            vecT t;
+#pragma unroll
+            for (int x = 0; x < VT; ++x) t[x] = (T)(v[e + x] * (1.f / SX));
+            *reinterpret_cast<vecT*>(row + e) = t;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < g.n) row[e] = (T)(v[e] * (1.f / SX));
+        }
+      } else {
+        h16x8 vh, vl;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { half a, b; split2(v[e], a, b); vh[e] = a; vl[e] = b; }
+        *reinterpret_cast<h16x8*>(oh + (long long)r * so + c) = vh;
+        *reinterpret_cast<h16x8*>(ol + (long long)r * so + c) = vl;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    if ((STEP == 2 && last && tall) || mirror) {
+      const int lr = lane & 31, r = r0 + wr + 32 * i + lr;
+#pragma unroll 4
+      for (int k = 0; k < CW / 2; ++k) {                   // two columns at a time, 32 rows each
+        const int lc = 2 * k + h, c = c0 + wc + lc;
+        const float v = place(lr, lc >> 2)[lc & 3];
+        if (STEP == 2) {
+          if (r < m && c < g.n) y[(long long)c * g.yr + r] = (T)(v * (1.f / SX));
+        } else if (r < ldm && c < m) {
+          half a, b;
+          split2(v, a, b);
+          oh[(long long)c * so + r] = a; ol[(long long)c * so + r] = b;
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
 }
 
 // workgroups of a launch over `tiles(group)` tiles a matrix cut into `cuts` runs: the fullest XCD's, eight times
@@ -507,40 +594,44 @@ template <typename T, bool FULL, int TS> int run_tiled(const OrthoP& p, int step
   while (cuts < 8 && p.matrices * cuts < 64) cuts *= 2;
   auto sym = [&](int ts) { return grid_of(p, cuts, [=](const OrthoG& g) { const int tm = (g.m + ts - 1) / ts; return tm * (tm + 1) / 2; }); };
   const unsigned sym_ts = sym(TS), sym_128 = sym(128);
-  const bool wide = TS == 128 || sym_ts >= 512;
-  const unsigned full = grid_of(p, cuts, [](const OrthoG& g) { return (g.m + TS - 1) / TS * ((g.ldn + TS - 1) / TS); });
+  const bool wide = TS == 64 || sym_ts >= 512;
+  // P X of the 64 class: 128 where that still gives two workgroups a compute unit (36 x 384 x 384 and 12 x 384 x 1536: 37 us, 47 with 64)
+  long long full_128 = 0;
+  for (int i = 0; i < p.ngroups; ++i) full_128 += (long long)p.g[i].count * ((p.g[i].m + 127) / 128) * ((p.g[i].ldn + 127) / 128);
+  auto full = [&](int ts) { return grid_of(p, cuts, [=](const OrthoG& g) { return (g.m + ts - 1) / ts * ((g.ldn + ts - 1) / ts); }); };
   ortho_sumsq<T><<<dim3(p.matrices, ORTHO_PARTS), 256, 0, st>>>(p);
   ortho_load<T><<<dim3(load_tiles, p.matrices), 256, 0, st>>>(p);
   for (int s = 0; s < steps; ++s) {
     const int cur = 2 * (s & 1), last = s == steps - 1;
     const float a = coef[3 * s], b = coef[3 * s + 1], c = coef[3 * s + 2];
     if (wide) {
-      ortho_product<T, 0, FULL, TS><<<dim3(sym_ts), 2 * TS, 0, st>>>(p, cuts, cur, 0, a, b, c);
-      ortho_product<T, 1, FULL, TS><<<dim3(sym_ts), 2 * TS, 0, st>>>(p, cuts, cur, 0, a, b, c);
+      ortho_product<T, 0, FULL, TS><<<dim3(sym_ts), threads_of(TS), 0, st>>>(p, cuts, cur, 0, a, b, c);
+      ortho_product<T, 1, FULL, TS><<<dim3(sym_ts), threads_of(TS), 0, st>>>(p, cuts, cur, 0, a, b, c);
     } else {
       ortho_product<T, 0, FULL, 128><<<dim3(sym_128), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
       ortho_product<T, 1, FULL, 128><<<dim3(sym_128), 256, 0, st>>>(p, cuts, cur, 0, a, b, c);
     }
-    ortho_product<T, 2, FULL, TS><<<dim3(full), 2 * TS, 0, st>>>(p, cuts, cur, last, a, b, c);
+    if (TS == 64 && full_128 >= 512) ortho_product<T, 2, FULL, 128><<<dim3(full(128)), 256, 0, st>>>(p, cuts, cur, last, a, b, c);
+    else ortho_product<T, 2, FULL, TS><<<dim3(full(TS)), threads_of(TS), 0, st>>>(p, cuts, cur, last, a, b, c);
   }
   return hipGetLastError() != hipSuccess;
 }
 
-template <typename T, int MT> int run_small(const OrthoP& p, const OrthoCoef& co, hipStream_t st) {
+template <typename T, int RT, int XT> int run_small(const OrthoP& p, const OrthoCoef& co, hipStream_t st) {
   static bool seen[64];
   if (first_use_on_device(seen) &&
-      hipFuncSetAttribute((const void*)ortho_small<T, MT>, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS) != hipSuccess) return 1;
+      hipFuncSetAttribute((const void*)ortho_small<T, RT, XT>, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS) != hipSuccess) return 1;
   int bytes = 0;
   for (int i = 0; i < p.ngroups; ++i) { const int b = small_dim(p.g[i].m, p.g[i].n).bytes; if (b > bytes) bytes = b; }
-  ortho_small<T, MT><<<dim3(p.matrices), 1024, bytes, st>>>(p, co);
+  ortho_small<T, RT, XT><<<dim3(p.matrices), 512, bytes, st>>>(p, co);
   return hipGetLastError() != hipSuccess;
 }
 
-// How a stack is worked on: in one workgroup with 2, 4, 6 or 8 row tiles of 16, or with tiles of 128 (256: m >= 1024) and,
-// for bf16 results (+ 1) of m >= 256, fewer instructions a product (below that it costs precision and saves nothing)
+// How a stack is worked on: in one workgroup with 1 to 4 row tiles of 32 (+ 8: more than 16 tiles of X), or with tiles: 64, or 256 for m >= 1024, and for
+// bf16 results (+ 1) of m >= 256 with fewer instructions a product (below that it costs precision and saves nothing)
 int class_of(const OrthoG& g, bool bf16) {
-  if (ortho_is_small(g)) return (g.m + 31) / 32 * 2;
-  return (g.m >= 1024 ? 256 : 128) + (bf16 && g.m >= 256);
+  if (ortho_is_small(g)) return (g.m + 31) / 32 + ((g.m + 31) / 32 * ((g.n + 31) / 32) > 16 ? 8 : 0);
+  return (g.m >= 1024 ? 256 : 64) + (bf16 && g.m >= 256);
 }
 OrthoP only(const OrthoP& p, bool bf16, int cls) {
   OrthoP q = p;
@@ -559,12 +650,19 @@ template <typename T> int run(const OrthoP& p, int steps, const float* coef, hip
   OrthoCoef co;
   co.steps = steps;
   for (int i = 0; i < 3 * steps; ++i) co.c[i] = coef[i];
-  for (int cls : {256 + BF16, 128 + 1, 128, 8, 6, 4, 2}) {
+  for (int cls : {256 + BF16, 64 + 1, 64, 8 + 4, 8 + 3, 8 + 2, 8 + 1, 4, 3, 2, 1}) {
     const OrthoP q = only(p, BF16, cls);
     if (!q.ngroups) continue;
-    const int rc = cls >= 256 ? run_tiled<T, !BF16, 256>(q, steps, coef, st) : cls == 128 + 1 ? run_tiled<T, !BF16, 128>(q, steps, coef, st) :
-                   cls == 128 ? run_tiled<T, true, 128>(q, steps, coef, st) : cls == 8 ? run_small<T, 8>(q, co, st) :
-                   cls == 6 ? run_small<T, 6>(q, co, st) : cls == 4 ? run_small<T, 4>(q, co, st) : run_small<T, 2>(q, co, st);
+    // 256 tiles need half the compute units to have one: 5 steps of 2 x 2048 x 8192 fp32 in 5.0 ms with 64, 4.2 with 128, 4.0
+    // with 256; of 1 x 2048 x 2048 868, 878, 1194 us; of 36 x 384 x 384 357, 375, 438 us; of 1 x 768 x 768 221, 401, 542 us
+    long long wide = 0;
+    for (int i = 0; i < q.ngroups; ++i) wide += (long long)q.g[i].count * ((q.g[i].m + 255) / 256) * ((q.g[i].n + 255) / 256);
+    const int rc = cls >= 256 ? (wide >= 128 ? run_tiled<T, !BF16, 256>(q, steps, coef, st) : run_tiled<T, !BF16, 64>(q, steps, coef, st)) :
+                   cls == 64 + 1 ? run_tiled<T, !BF16, 64>(q, steps, coef, st) : cls == 64 ? run_tiled<T, true, 64>(q, steps, coef, st) :
+                   cls == 12 ? run_small<T, 4, 5>(q, co, st) : cls == 11 ? run_small<T, 3, 5>(q, co, st) :
+                   cls == 10 ? run_small<T, 2, 5>(q, co, st) : cls == 9 ? run_small<T, 1, 5>(q, co, st) :
+                   cls == 4 ? run_small<T, 4, 2>(q, co, st) : cls == 3 ? run_small<T, 3, 2>(q, co, st) :
+                   cls == 2 ? run_small<T, 2, 2>(q, co, st) : run_small<T, 1, 2>(q, co, st);
     if (rc) return rc;
   }
   return 0;
