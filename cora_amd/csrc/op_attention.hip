@@ -69,7 +69,7 @@ __device__ __forceinline__ bool locate(const AttnP& p, int slot, int TR, long lo
   return n > 0 && tile >= 0 && (long long)tile * TR < n;
 }
 
-constexpr float NO_EXP = -1e30f;   // exponent of a row of zeros (attn_bwd_q)
+constexpr float NO_EXP = -1e30f;   // exponent of a row of zeros, or with an infinity (attn_bwd_q)
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 __device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 // row of accumulator register r of lane half h in a 32 x 32 tile
@@ -115,6 +115,37 @@ __device__ __forceinline__ int limit(int i, int n, int block) {
     if (it_ + 1 < (COUNT)) WORK(it_ + 1, 1);                                       \
   }
 
+// What a mask hides must not count, even if it is not finite: hidden scores are replaced, but in the product behind them 0 times
+// infinity would.  A tile of which some rows of the workgroup do not see all is therefore searched first (each lane its own
+// 16-byte pieces, as it requested them): elements that are not finite become zeros, and mark(piece) makes the score
+// of their row NaN, so that whoever sees the row comes out as NaN in all channels.
+template <typename T, int D, int R, int NW, typename M> __device__ __forceinline__ void quarantine(T* t, int w, int lane, const M& mark) {
+  constexpr unsigned INF = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;     // the exponent's bits
+#pragma unroll 1
+  for (int i = 0; i < R * D / Op<T>::E / 64 / NW; ++i) {
+    const int id = (i * NW + w) * 64 + lane;
+    uint4& at = reinterpret_cast<uint4*>(t)[id];
+    uint4 v = at;
+    unsigned* u = &v.x;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      unsigned keep = ~0u;
+      if ((u[e] & INF) == INF) keep = sizeof(T) == 4 ? 0u : 0xffff0000u;
+      if (sizeof(T) == 2 && (u[e] >> 16 & INF) == INF) keep &= 0xffffu;
+      bad |= keep != ~0u;
+      u[e] &= keep;
+    }
+    if (bad) { at = v; mark(id); }
+  }
+}
+// the waves' LDS writes are done; requests under way stay under way
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Queries of a workgroup and its walk over keys.  SPLIT = false: NW waves of 32 queries each share every staged tile of KT
 // keys.  SPLIT = true, for few rows: NW waves share the same 32 queries, wave w walks the key tiles w, w + NW, .. through
 // buffers of its own, and the waves' results are joined in LDS at the end (join_own).
@@ -153,6 +184,7 @@ __device__ __forceinline__ void join_own(f32x16 (&acc)[D / 32], float* lds, int 
 // ---- forward -------------------------------------------------------------------------------------
 // The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
+// Each row goes by its own scores, so its result does not depend on which other rows share its tile.
 template <typename T, int D, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_fwd(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
@@ -172,6 +204,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   const int lim = own ? limit(qi, n, p.block) : 0;
   const int wave_end = qw < n ? limit(min(qw + 31, n - 1), n, p.block) : 0;      // keys the wave needs
   const int wave_min = limit(min(qw, n - 1), n, p.block);                        // keys every query of it sees
+  const int all_min = limit(tile * QT, n, p.block);                              // keys every query of the workgroup sees
   const int end = limit(min(tile * QT + QT, n) - 1, n, p.block);                 // keys the workgroup needs
 
   const T* kb = (const T*)p.k + b * p.kr + (long long)kv * p.kh;
@@ -196,10 +229,14 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     fk(kb + j0 * p.kr, end - j0, k + mine, fw);
     fv(vb + j0 * p.vr, end - j0, v + mine, fw);
   };
-  auto work = [&](int it, const T* k, const T* v) {
+  auto work = [&](int it, T* k, T* v) {
     const int j0 = (SPLIT ? it * NW + w : it) * KT;
-    if (j0 >= wave_end) return;
     k += mine; v += mine;
+    if (j0 + KT > all_min && j0 < end && p.block) {
+      quarantine<T, D, KT, W::FW>(v, fw, lane, [&](int id) { k[id * Op<T>::E] = (T)NAN; });
+      if (!SPLIT) lds_barrier();
+    }
+    if (j0 >= wave_end) return;
     f32x16 s[KT / 32];
     float mx = -INFINITY;
 #pragma unroll
@@ -222,7 +259,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
     mx = half_max(mx) * sl2;
     if (__any(mx > m + 8.f)) {
-      const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      const float mn = mx > m + 8.f ? mx : m, al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= al;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -304,7 +341,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   const bool own = qi < n;
   const int lim = own ? limit(qi, n, p.block) : 0;
   const int wave_end = qw < n ? limit(min(qw + 31, n - 1), n, p.block) : 0;
-  const int wave_min = limit(min(qw, n - 1), n, p.block);
+  const int wave_min = limit(min(qw, n - 1), n, p.block), all_min = limit(tile * QT, n, p.block);
   const int end = limit(min(tile * QT + QT, n) - 1, n, p.block);
 
   const T* kb = (const T*)p.k + b * p.kr + (long long)kv * p.kh;
@@ -328,7 +365,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     big = half_max(big);
     const int e = big > 0.f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
     dscale = __builtin_amdgcn_ldexpf(1.f, -e); back = __builtin_amdgcn_ldexpf(p.scale, e);
-    if (own && h == 0 && (!SPLIT || w == 0)) p.delta[2 * plane + at] = big > 0.f ? (float)e : NO_EXP;
+    if (own && h == 0 && (!SPLIT || w == 0)) p.delta[2 * plane + at] = big > 0.f && big < INFINITY ? (float)e : NO_EXP;
   }
   const float lse2 = own ? p.lse[at] * CORA_LOG2E : 0.f, sl2 = p.scale * CORA_LOG2E;
   // Where a wave sees one key tile only, delta is taken from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
@@ -347,10 +384,14 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     fk(kb + j0 * p.kr, end - j0, k + mine, fw);
     fv(vb + j0 * p.vr, end - j0, v + mine, fw);
   };
-  auto work = [&](int it, const T* k, const T* v) {
+  auto work = [&](int it, T* k, T* v) {
     const int j0 = (SPLIT ? it * NW + w : it) * KT;
-    if (j0 >= wave_end) return;
     k += mine; v += mine;
+    if (j0 + KT > all_min && j0 < end && p.block) {
+      quarantine<T, D, KT, W::FW>(k, fw, lane, [&](int id) { v[id * Op<T>::E] = (T)NAN; });
+      if (!SPLIT) lds_barrier();
+    }
+    if (j0 >= wave_end) return;
     if (whole) {
       float sum = 0.f;
 #pragma unroll 1
@@ -435,11 +476,12 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   const bool own = ki < n;
   const int qmin = p.block ? ki / p.block * p.block : 0;              // the first query that sees the lane's key
   const int wave_max = p.block ? (kw + 31) / p.block * p.block : 0;   // the first that sees all keys of the wave
+  const int all_max = p.block ? (min(k0 + KB, n) - 1) / p.block * p.block : 0;     // .. all keys of the workgroup
   const int qbeg = p.block ? k0 / p.block * p.block / QT * QT : 0;    // the first tile with a query that sees key k0
   const int ntile = (n - qbeg + QT - 1) / QT, total = ntile * group;
   const int it0 = (int)((long long)total * blockIdx.y / p.parts), it1 = (int)((long long)total * (blockIdx.y + 1) / p.parts);
 
-  const Fetch<T, D, QT, NW> fq(p.qr, p.d, w, lane), fd(p.dor, p.d, w, lane);
+  const Fetch<T, D, QT, NW> into_q(p.qr, p.d, w, lane), into_d(p.dor, p.d, w, lane);
   frag kf[NC], vf[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -455,18 +497,26 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   float ecur = NO_EXP;                                  // F16: exponent ak is scaled by
   [[maybe_unused]] const long long plane = (long long)p.heads * p.rows;
 
-  auto fetch = [&](int it, T* q, T* d, float (&cs)[3][64]) {
-    it += it0;
-    const int g = it / ntile, q0 = qbeg + (it - g * ntile) * QT, head = kv * group + g;
-    fq((const T*)p.q + (b + q0) * p.qr + (long long)head * p.qh, n - q0, q, w);
-    fd((const T*)p.dout + (b + q0) * p.dor + (long long)head * p.doh, n - q0, d, w);
+  int fhead = kv * group + it0 / ntile, fq = it0 % ntile, wq = fq;       // the next tile to fetch and to work on (counted: a division per tile is 6 % of the time)
+  auto fetch = [&](int, T* q, T* d, float (&cs)[3][64]) {
+    const int q0 = qbeg + fq * QT, head = fhead;
+    if (++fq == ntile) { fq = 0; ++fhead; }
+    into_q((const T*)p.q + (b + q0) * p.qr + (long long)head * p.qh, n - q0, q, w);
+    into_d((const T*)p.dout + (b + q0) * p.dor + (long long)head * p.doh, n - q0, d, w);
     // constants: one request of 64 floats each (fp32 stages 32 queries and asks for 32 more than it needs)
 #pragma unroll
     for (int k = 0; k < (F16 ? 3 : 2); ++k)
       if (w == k % NW) REQUEST(p.delta + k * plane + (long long)head * p.rows + b + q0, 4 * min(n - q0, 64), cs[k], 4, 4 * lane);
   };
-  auto work = [&](int it, const T* qt, const T* dt_, const float (&cs)[3][64]) {
-    const int q0 = qbeg + ((it0 + it) % ntile) * QT;
+  auto work = [&](int, T* qt, T* dt_, float (&cs)[3][64]) {
+    const int q0 = qbeg + wq * QT;
+    if (++wq == ntile) wq = 0;
+    if (q0 < all_max) {
+      auto mark = [&](int id) { cs[1][id / (D / O::E)] = NAN; };
+      quarantine<T, D, QT, NW>(qt, w, lane, mark);
+      quarantine<T, D, QT, NW>(dt_, w, lane, mark);
+      lds_barrier();
+    }
     if (kw >= n) return;
     if (F16) {
       float e = q0 + lane < n ? cs[2][lane] : NO_EXP;

@@ -172,7 +172,8 @@ def attention(q, k, v, *, cu_seqlens=None, seq_len: Optional[int] = None, causal
     Sequence s owns rows cu_seqlens[s] .. cu_seqlens[s+1] - 1 (int32 on the GPU; lengths may differ, be 1 or 0), or every
     `seq_len` rows (default: all) are one.  `causal_block` 0: bidirectional; b: a token sees the tokens of its own and of
     earlier blocks of b tokens (1: causal; tokens per frame: frame-causal).  `scale` defaults to head_dim ** -0.5.
-    `lse` [heads, rows] float32 is the log of the softmax' denominator.  Rows of no sequence are left as they were in
+    What the mask hides does not count even if it is not finite; a row that sees a value that is not finite may come out as
+    NaN in all its channels.  `lse` [heads, rows] float32 is the log of the softmax' denominator.  Rows of no sequence are left as they were in
     `out` and `lse` (undefined in freshly allocated ones)."""
     head, strides = _attention_inputs(q, k, v, cu_seqlens, seq_len, causal_block, scale)
     if out is None:

@@ -236,6 +236,51 @@ def test_attention_other_sequences_do_not_leak(dtype):
         within(t[70:103], ref[n][70:103], bound[n][70:103], n)
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lens,heads,kv,d,block", [([150, 3, 90], 4, 2, 64, 1), ([150, 90], 2, 2, 48, 50), ([300], 2, 1, 128, 7),
+                                                   ([200] * 90, 4, 2, 32, 40), ([700] * 40, 2, 2, 96, 1)])
+def test_attention_what_the_mask_hides_does_not_count(lens, heads, kv, d, block, dtype, value):
+    """One token of every sequence has keys, values, queries or gradients that are not finite: what does not see it keeps its
+    result.  Forward and dq repeat the untouched ones bit for bit (products with zero weights add zeros)."""
+    cu, qkv, dout = packed(lens, 0, heads, kv, d, dtype)
+    rows = cu[-1]
+    lim, bad = torch.empty(rows, dtype=torch.long), torch.empty(rows, dtype=torch.long)
+    for b, e in zip(cu, cu[1:]):
+        i = torch.arange(e - b)
+        lim[b:e], bad[b:e] = b + torch.clamp((i // block + 1) * block, max=e - b), b + (e - b) // 2
+    at = torch.unique(bad)
+    kw = dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), causal_block=block)
+    q, k, v = split(qkv.cuda(), heads, kv)
+    g = dout.cuda()
+    out, lse = ca.attention(q, k, v, **kw)
+    dq, dk, dv = ca.attention_backward(g, q, k, v, out, lse, **kw)
+    hides = (lim <= bad).cuda()                                      # rows that do not see the token's key
+    assert hides.any()
+    for name in ("k", "v"):
+        t = {"k": k.clone(), "v": v.clone()}
+        t[name][at, -1, d // 3] = value
+        out2, lse2 = ca.attention(q, t["k"], t["v"], **kw)
+        assert torch.equal(out2[hides], out[hides]) and torch.equal(lse2[:, hides], lse[:, hides]), name
+        dq2 = ca.attention_backward(g, q, t["k"], t["v"], out2, lse2, **kw)[0]
+        assert torch.equal(dq2[hides], dq[hides]), name
+        if value != value:
+            assert torch.isnan(out2[~hides][:, -1]).any(-1).all() and torch.isnan(dq2[~hides][:, -1]).any(-1).all(), name
+    first = torch.arange(rows) >= lim[bad]                           # keys that the token's query does not see
+    ref, bound = attention_ref(*split(qkv, heads, kv), cu, block, d ** -0.5, dout)
+    for name in ("q", "dout"):
+        t = {"q": q.clone(), "dout": g.clone()}
+        t[name][at, -1, d // 3] = value
+        out2, lse2 = ca.attention(t["q"], k, v, **kw)
+        got = ca.attention_backward(t["dout"], t["q"], k, v, out2, lse2, **kw)
+        for n, new, old in zip(("dk", "dv"), got[1:], (dk, dv)):
+            within(new[first.cuda()], ref[n][first], bound[n][first], (name, n))
+            if dtype is not F16:                                     # fp16: the rows' common exponent may have changed
+                assert torch.equal(new[first.cuda()], old[first.cuda()]), (name, n)
+        if value != value:
+            assert torch.isnan(got[2][~first.cuda()][:, -1]).any(-1).all(), name
+
+
 def test_attention_broken_tables_stay_in_bounds():
     """Descending and out-of-range bounds: rows outside [0, rows) are never touched and the call ends."""
     q = randn(50, 2, 32, dtype=BF16).cuda()
