@@ -452,6 +452,15 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   if (own) store_own<T, D>((T*)p.dq + row * p.dqr + (long long)head * p.dqh, acc, back, p.d, h);
 }
 
+// Issue order of the block it stands in: READS reads of LDS first, then N matrix instructions, each followed by PER more reads.
+// Left alone the compiler reads an operand right before its use, and with one wave per SIMD (128 channels) nothing else hides
+// the way from LDS.
+template <int READS, int PER, int N, int GROUP> __device__ __forceinline__ void feed() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, GROUP);
+#pragma unroll
+  for (int c = 0; c < N; ++c) { __builtin_amdgcn_sched_group_barrier(0x8, 1, GROUP); __builtin_amdgcn_sched_group_barrier(0x100, PER, GROUP); }
+}
+
 // ---- backward: dk and dv -------------------------------------------------------------------------
 // A workgroup owns 32 NW keys of one key head and walks the queries that see any of them, head after head of its group.
 // With p.parts > 1 that walk is cut into as many ranges, one per workgroup (blockIdx.y), whose sums go to the workspace in
@@ -541,44 +550,38 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
 #pragma unroll
         for (int i = 0; i < 4; ++i) { s[4 * g + i] = 0.f; dp[4 * g + i] = c1[i]; }
       }
-      const bool edge = q0 + 32 * t < wave_max;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) s = O::mma(L::row_frag(qt, 32 * t, c, lane), kf[c], s);
+      for (int c = 0; c < NC; ++c) {
+        s = O::mma(L::row_frag(qt, 32 * t, c, lane), kf[c], s);
+        dp = O::mma(L::row_frag(dt_, 32 * t, c, lane), vf[c], dp);
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 c0 = *reinterpret_cast<const f32x4*>(&cs[1][32 * t + 8 * g + 4 * h]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], sl2, c0[i]));
       }
-      if (edge) {
+      if (sizeof(T) == 2) feed<12, 1, 2 * NC, 0>();
+      if (q0 + 32 * t < wave_max) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (q0 + 32 * t + acc_row(r, h) < qmin) s[r] = 0.f;
+          if (q0 + 32 * t + acc_row(r, h) < qmin) { s[r] = 0.f; dp[r] = 0.f; }       // p = 0 does not hide an infinite do v
       }
-#pragma unroll
-      for (int c = 0; c < 32 / O::CH; ++c) {
-        const frag pf = O::pack(s, c);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) av[i] = O::mma(L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), pf, av[i]);
-      }
-#pragma unroll
-      for (int c = 0; c < NC; ++c) dp = O::mma(L::row_frag(dt_, 32 * t, c, lane), vf[c], dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         dp[r] *= s[r];
         if (F16) dp[r] *= dscale;
       }
-      if (edge) {                                       // p = 0 does not hide an infinite do v
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (q0 + 32 * t + acc_row(r, h) < qmin) dp[r] = 0.f;
-      }
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
-        const frag gf = O::pack(dp, c);
+        const frag pf = O::pack(s, c), gf = O::pack(dp, c);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) ak[i] = O::mma(L::col_frag(qt, t * (32 / O::CH) + c, i, lane), gf, ak[i]);
+        for (int i = 0; i < D / 32; ++i) {
+          av[i] = O::mma(L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), pf, av[i]);
+          ak[i] = O::mma(L::col_frag(qt, t * (32 / O::CH) + c, i, lane), gf, ak[i]);
+        }
       }
+      if (sizeof(T) == 2) feed<8, 2, D / 8, 1>();
     }
   };
 #define FETCH(it, buf) fetch(it, buf ? qs1 : qs0, buf ? ds1 : ds0, buf ? cs1 : cs0)
