@@ -75,14 +75,17 @@ int check_attention(const cora_attention_args* a, AttnP* p, const char* who, boo
   }
   if (!a->lse || (uintptr_t)a->lse % 4 || (a->cu_seqlens && (uintptr_t)a->cu_seqlens % 4))
     return refuse("%s: lse is NULL, or lse or cu_seqlens is not 4-byte aligned", who);
-  // workgroups: at most one per 16 rows and sequence and head
-  const long long tiles = a->cu_seqlens ? a->rows / 16 + a->n_seq : (long long)a->n_seq * ((a->seq_len + 15) / 16);
-  if (tiles * a->heads >= (1LL << 31)) return refuse("%s: too many tiles for one launch", who);
+  // workgroups of up to 256 threads, fewer than 2^32 threads: one per 128 rows of a sequence and head (32 where there are few rows)
+  const long long tiles = a->cu_seqlens ? a->rows / 128 + a->n_seq : (long long)a->n_seq * ((a->seq_len + 127) / 128);
+  if ((tiles + 1024) * a->heads >= (1LL << 24)) return refuse("%s: too many tiles for one launch", who);
   if (backward) {
     if (!a->workspace || (uintptr_t)a->workspace % 16 || a->workspace_bytes < cora_attention_workspace(a))
       return refuse("%s: workspace is NULL, not 16-byte aligned or smaller than cora_attention_workspace says (%zu bytes)", who,
                     cora_attention_workspace(a));
   }
+  for (const Ref& r : refs)
+    for (const Ref& s : refs)
+      if (r.out && &r != &s && (backward || !s.bwd) && r.ptr == s.ptr) return refuse("%s: %s is %s", who, r.name, s.name);
   memset(p, 0, sizeof *p);
   p->q = a->q; p->k = a->k; p->v = a->v; p->out = a->out; p->o = a->out; p->lse = a->lse;
   p->dout = a->dout; p->dq = a->dq; p->dk = a->dk; p->dv = a->dv; p->cu = a->cu_seqlens;
@@ -107,14 +110,20 @@ OrthoG& add_stack(OrthoP& p, int count, int rows, int cols) {
   return g;
 }
 
+// a launch has fewer than 2^32 threads, 256 a tile (and some idle ones)
+constexpr long long ORTHO_TILES = 1LL << 22;
+long long tiles_64(const cora_matrices& s) { return ((long long)s.rows + 63) / 64 * ((s.cols + 63) / 64) * s.count; }
+
 // up to ORTHO_GROUPS stacks from stacks[i0]; returns how many were taken
 int take_stacks(const cora_matrices* stacks, int i0, int n, OrthoP* p) {
   p->ngroups = 0; p->matrices = 0;
   int i = i0;
+  long long tiles = 0;
   for (; i < n && p->ngroups < ORTHO_GROUPS; ++i) {
     const cora_matrices& s = stacks[i];
     if (s.count == 0) continue;
-    if (p->matrices + s.count > 65535) break;
+    tiles += tiles_64(s);
+    if (p->matrices + s.count > 65535 || (p->ngroups && tiles >= ORTHO_TILES)) break;
     OrthoG& g = add_stack(*p, s.count, s.rows, s.cols);
     g.x = s.x; g.y = s.y; g.xm = s.x_mat; g.xr = s.x_row; g.ym = s.y_mat; g.yr = s.y_row;
   }
@@ -127,8 +136,7 @@ int check_stacks(int dtype, const cora_matrices* s, int n, const char* who) {
   for (int i = 0; i < n; ++i) {
     if (s[i].count < 0 || s[i].count > 65535 || s[i].rows < 1 || s[i].cols < 1 || s[i].rows > 32768 || s[i].cols > 32768)
       return refuse("%s: stack %d: count must be 0 .. 65535, rows and cols 1 .. 32768", who, i);
-    const long long t = ((long long)s[i].rows + 127) / 128 * ((s[i].cols + 127) / 128) * s[i].count;
-    if (t >= (1LL << 26)) return refuse("%s: stack %d: too many tiles for one launch", who, i);
+    if (tiles_64(s[i]) >= ORTHO_TILES) return refuse("%s: stack %d: too many tiles for one launch", who, i);
   }
   return 0;
 }
@@ -278,6 +286,10 @@ int cora_orthogonalize(int dtype, const cora_matrices* stacks, int n_stacks, int
     if (s.x == s.y && ((s.rows > 1 && s.x_row != s.y_row) || (s.count > 1 && s.x_mat != s.y_mat)))
       return refuse("%s: stack %d: in place, x and y need the same strides", who, i);
   }
+  for (int i = 0; i < n_stacks; ++i)
+    for (int j = 0; j < n_stacks; ++j)
+      if (i != j && stacks[i].count && stacks[j].count && (stacks[i].y == stacks[j].y || stacks[i].y == stacks[j].x))
+        return refuse("%s: y of stack %d is x or y of stack %d", who, i, j);
   if (!any) return 0;
   const size_t need = cora_orthogonalize_workspace(dtype, stacks, n_stacks);
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < need)

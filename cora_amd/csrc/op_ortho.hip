@@ -20,6 +20,8 @@
 #include "op_tile.h"
 #include "ops.h"
 
+#include <atomic>
+
 namespace {
 
 typedef _Float16 half;
@@ -635,9 +637,14 @@ template <typename T, bool FULL, int TS> int run_tiled(const OrthoP& p, int step
 }
 
 template <typename T, int RT, int XT> int run_small(const OrthoP& p, const OrthoCoef& co, hipStream_t st) {
-  static bool seen[64];
-  if (first_use_on_device(seen) &&
-      hipFuncSetAttribute((const void*)ortho_small<T, RT, XT>, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS) != hipSuccess) return 1;
+  static std::atomic<unsigned long long> ready{0};          // devices; marked when done, as two threads may come here at once
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 1;
+  const unsigned long long bit = dev < 64 ? 1ULL << dev : 0;
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (hipFuncSetAttribute((const void*)ortho_small<T, RT, XT>, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS) != hipSuccess) return 1;
+    ready.fetch_or(bit, std::memory_order_release);
+  }
   int bytes = 0;
   for (int i = 0; i < p.ngroups; ++i) { const int b = small_dim(p.g[i].m, p.g[i].n).bytes; if (b > bytes) bytes = b; }
   ortho_small<T, RT, XT><<<dim3(p.matrices), 512, bytes, st>>>(p, co);

@@ -31,12 +31,12 @@ template <typename T> struct VecOf<T, 1> { struct type { T v; __device__ T& oper
 // INTER: V neighbouring channels (V / 2 pairs, V even) a thread; else V first and the V second channels of V pairs.  V = 1
 // takes any layout.  Threads of channels that pass through move one (INTER) or two vectors in the same loop.
 template <typename T, int V, bool INTER>
-__global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const int units, const int hchunk) {
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryP p, const long long row0, const int units, const int hchunk) {
   constexpr int NPAIR = INTER ? V / 2 : V;
   typedef typename VecOf<T, V>::type vec;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / units;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = row0 + id / units;
   if (row >= p.rows) return;
-  const int u = (int)(id - row * units);
+  const int u = (int)(id % units);
   const int h0 = blockIdx.y * hchunk, h1 = min(p.heads, h0 + hchunk);
   const int turning = p.pairs / NPAIR;
   const bool turns = u < turning;
@@ -108,8 +108,13 @@ template <typename T, int V, bool INTER> int go(const RotaryP& p, hipStream_t st
   int split = 1;
   while (split < p.heads && blocks * split < 1024) split *= 2;
   const int hchunk = (p.heads + split - 1) / split;
-  rotary_kernel<T, V, INTER><<<dim3((unsigned)blocks, (unsigned)((p.heads + hchunk - 1) / hchunk)), 256, 0, st>>>(p, units, hchunk);
-  return hipGetLastError() != hipSuccess;
+  const long long per = ((1LL << 32) - 256) / units;        // rows of a launch, which has fewer than 2^32 threads along x
+  for (long long row0 = 0; row0 < p.rows; row0 += per) {
+    const long long rows = p.rows - row0 < per ? p.rows - row0 : per;
+    rotary_kernel<T, V, INTER><<<dim3((unsigned)((rows * units + 255) / 256), (unsigned)((p.heads + hchunk - 1) / hchunk)), 256, 0, st>>>(p, row0, units, hchunk);
+    if (hipGetLastError() != hipSuccess) return 1;
+  }
+  return 0;
 }
 // the widest vectors that fit: 16, 8 or 4 bytes
 template <typename T> int run(const RotaryP& p, hipStream_t st) {

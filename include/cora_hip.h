@@ -269,7 +269,7 @@ enum { CORA_F32 = 0, CORA_BF16 = 1, CORA_F16 = 2 };
  * head; its pair i turns by the angle pos_a * theta^(-2 i / axes_dim[a]): (u, v) -> (u cos - v sin, u sin + v cos), with
  * u, v neighbouring channels (interleaved) or axes_dim[a] / 2 apart.  Channels behind the last axis are copied.
  * backward != 0 turns the other way: the gradient with respect to x of a gradient given for y.
- * x [rows, heads, head_dim] -> y, which may be x itself (same strides).  Row r takes positions pos[r % pos_rows]. */
+ * x [rows, heads, head_dim] -> y, which may be x itself (same strides) and else must not overlap it.  Row r takes positions pos[r % pos_rows]. */
 typedef struct cora_rotary_args {
   int32_t dtype, heads, head_dim, n_axes;
   int32_t axes_dim[4];          /* positive, even, together at most head_dim and at most 128 */
@@ -292,6 +292,8 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream);
  * head_dim: up to 128, a multiple of 8 (float32: 4); pointers 16-byte aligned, strides multiples of 16 bytes,
  * row strides below 2^24 elements.  Sums and
  * softmax statistics are float32; the probabilities are rounded to a 16-bit dtype before they meet v.
+ * What the mask hides does not count even if it is not finite; a row that sees a value that is not finite may come out as
+ * NaN in all its channels.  Outputs must not overlap inputs or each other (rows of one packed buffer may interleave).
  * Backward: dout and the forward's out and lse -> dq, dk, dv (sums over the query heads of a key head).  workspace:
  * cora_attention_workspace(a) bytes, 16-byte aligned, not shared by calls that may overlap.  Results repeat bit for bit. */
 typedef struct cora_attention_args {
@@ -312,7 +314,8 @@ size_t cora_attention_workspace(const cora_attention_args* a);
 
 /* Orthogonalise weight updates by Newton-Schulz products: X = G / (|G|_F + eps), then per step, with coefficients
  * (a, b, c) of coef [steps, 3] (host), X <- a X + (b A + c A^2) X with A = X X^T (tall matrices: of the transpose).
- * All stacks (each `count` equal matrices) are worked on together; y may be x (same strides).  Products are float32-grade
+ * All stacks (each `count` equal matrices) are worked on together; a stack's y may be its x (same strides) and else must
+ * not overlap any x or y.  Products are float32-grade
  * (bfloat16: of an error below the result's rounding).  Refused: coefficients under which a singular value of [0, 1]
  * leaves [0, 8] or |a + b s^2 + c s^4| exceeds 1000.
  * workspace: cora_orthogonalize_workspace(..) bytes, 256-byte aligned, not shared by calls that may overlap. */

@@ -100,6 +100,20 @@ def test_rotary_offsets_past_32_bits():
     within(x, ref, bound, "past 2^32")
 
 
+def test_rotary_more_rows_than_a_launch_has_threads():
+    rows = 2 ** 32 + 512
+    x = torch.zeros(rows, 1, 2, dtype=F16, device="cuda")
+    ends = [slice(0, 512), slice(2 ** 32 - 512, 2 ** 32), slice(2 ** 32, rows)]
+    for i, e in enumerate(ends):
+        x[e].copy_(randn(512, 1, 2, dtype=F16, seed=i))
+    before = [x[e].cpu() for e in ends]
+    pos = positions(512, 1, 7, 50)
+    assert ca.rotary(x, pos.cuda(), [2], out=x) is x
+    for e, b in zip(ends, before):
+        ref, bound = rotary_ref(b, pos, [2], 1e4, True)
+        within(x[e], ref, bound, e)
+
+
 def test_rotary_no_rows():
     assert ca.rotary(torch.empty(0, 2, 16, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda"), [16]).shape == (0, 2, 16)
 

@@ -77,6 +77,29 @@ def test_attention_backward_refuses(kw, word):
     assert _lib.load().cora_attention_backward(C.byref(attn_args(**kw)), 0, None) == -1 and word in _err()
 
 
+def test_attention_refuses_outputs_that_are_inputs_and_launches_too_large():
+    lib = _lib.load()
+    apart = {n: FAKE * (i + 1) for i, n in enumerate(("q", "k", "v", "out", "dout", "dq", "dk", "dv", "workspace", "lse"))}
+    for name, other in (("out", "q"), ("out", "k"), ("out", "v")):
+        assert lib.cora_attention(C.byref(attn_args(**{**apart, name: apart[other]})), 0, None) == -1 and f"{name} is {other}" in _err()
+    for name, other in (("dq", "q"), ("dk", "dout"), ("dv", "dk"), ("dk", "dv"), ("dq", "out")):
+        a = attn_args(**{**apart, name: apart[other]})
+        assert lib.cora_attention_backward(C.byref(a), 0, None) == -1 and " is " in _err()
+    for kw in (dict(rows=1 << 30), dict(n_seq=1 << 22), dict(cu_seqlens=None, n_seq=1 << 22, seq_len=1, rows=1 << 22)):
+        assert lib.cora_attention(C.byref(attn_args(**{**apart, **kw})), 0, None) == -1 and "too many tiles" in _err()
+
+
+def test_orthogonalize_refuses_stacks_that_share_memory():
+    lib = _lib.load()
+    row = dict(x_mat=64, x_row=8, y_mat=64, y_row=8, count=1, rows=8, cols=8)
+    for y0, y1 in ((3, 3), (2, 4), (4, 1), (3, 1)):
+        s = (_lib.CoraMatrices * 2)(_lib.CoraMatrices(x=FAKE, y=y0 * FAKE, **row), _lib.CoraMatrices(x=2 * FAKE, y=y1 * FAKE, **row))
+        assert lib.cora_orthogonalize(0, s, 2, 5, coef(), 1e-7, FAKE, 1 << 20, 0, None) == -1 and "is x or y of stack" in _err()
+    big = (_lib.CoraMatrices * 1)(_lib.CoraMatrices(x=FAKE, y=FAKE, **{**row, "rows": 32768, "cols": 32768, "count": 16, "x_row": 32768, "y_row": 32768,
+                                                                       "x_mat": 1 << 30, "y_mat": 1 << 30}))
+    assert lib.cora_orthogonalize(0, big, 1, 5, coef(), 1e-7, FAKE, 1 << 20, 0, None) == -1 and "too many tiles" in _err()
+
+
 def coef(*c):
     c = c or (3.4445, -4.775, 2.0315) * 5
     return (C.c_float * len(c))(*c)
