@@ -69,6 +69,50 @@ __device__ __forceinline__ bool locate(const AttnP& p, int slot, int TR, long lo
   return n > 0 && tile >= 0 && (long long)tile * TR < n;
 }
 
+// The same for causal walks, the longest first over all sequences: a long tile that starts last would keep the chip waiting.
+// Work item i in the order of falling `tile`, where a sequence of T tiles has 0 .. T - 1: N(t) = sum over the sequences of
+// max(0, T - t) items have tile t or more, so t is found by bisection and the sequence by its rank among those with T > t.
+// One sequence a lane, so up to 64 of them; more keep their own order.  Worth its 1 to 2 us a workgroup where not all
+// workgroups run at once (longest_first; LDS: bytes of a workgroup).  Forward, us, own order / longest first: fp32, 16 x 1024
+// tokens, 1 head 54 / 40; packed clips, bf16, 12 heads of 64 102 / 94; all at once, bf16, 9 sequences, 2 heads 17.9 / 20.3.
+template <int LDS> __device__ __forceinline__ bool longest_first(const AttnP& p) {
+  return p.block && gridDim.x > (LDS <= 80 * 1024 ? 512 : 256);
+}
+__device__ __forceinline__ bool locate_longest(const AttnP& p, int i, int TR, long long& b, int& n, int& tile) {
+  if (!p.cu || p.nseq > 64) {
+    if (!locate(p, i, TR, b, n, tile)) return false;
+    const int T = (n + TR - 1) / TR;
+    if (!p.cu) { tile = T - 1 - i / p.nseq; b = (long long)(i % p.nseq) * n; }
+    else tile = T - 1 - tile;
+    return true;
+  }
+  const int rows = (int)p.rows, lane = threadIdx.x & 63;
+  auto first = [&](int s) { int c = p.cu[s]; return c < 0 ? 0 : (c > rows ? rows : c); };
+  int c0 = 0, len = 0;
+  if (lane < p.nseq) { c0 = first(lane); len = max(0, first(lane + 1) - c0); }
+  const int T = (len + TR - 1) / TR;
+  auto sum = [](int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  int hi = T;                                     // the largest T
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) hi = max(hi, __shfl_xor(hi, o, 64));
+  if (i >= sum(T)) return false;
+  int lo = 0, above = 0;                          // N(lo) > i >= N(hi) = above
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, c = sum(max(0, T - mid));
+    if (c > i) lo = mid; else { hi = mid; above = c; }
+  }
+  const unsigned long long in = __ballot(T > lo);
+  const int rank = __popcll(in & ((1ULL << lane) - 1));
+  const int s = max(0, __ffsll((long long)__ballot(T > lo && rank == i - above)) - 1);
+  b = __builtin_amdgcn_readlane(c0, s); n = __builtin_amdgcn_readlane(len, s); tile = lo;
+  return (long long)tile * TR < n;                // a broken table may give no such tile
+}
+
 constexpr float NO_EXP = -1e30f;   // exponent of a row of zeros, or with an infinity (attn_bwd_q)
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 __device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
@@ -182,6 +226,11 @@ __device__ __forceinline__ void join_own(f32x16 (&acc)[D / 32], float* lds, int 
 }
 
 // ---- forward -------------------------------------------------------------------------------------
+// Bound by the matrix units and, as close behind, by LDS: every matrix instruction (32 cycles of a SIMD in 16 bits) takes 1 KB
+// from LDS, which four SIMDs reading at once is all that LDS gives (128 bytes a cycle).  One workgroup per 128 queries, two to
+// a compute unit; or, for few rows, four waves that share 32 queries (the rule and its figures are at run below).  Measured, causal
+// bf16: 16384 tokens x 16 heads of 128 1.05 ms, 1050 TFLOP/s (a large library product: 1133); fp32 64 images of 196 tokens x 8 heads of 48
+// 88 us, of which a quarter is padding (48 channels to 64, 196 keys to 224).
 // The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
 // Each row goes by its own scores, so its result does not depend on which other rows share its tile.
@@ -195,8 +244,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   __shared__ __attribute__((aligned(16))) T ks1[W::BUF];
   __shared__ __attribute__((aligned(16))) T vs1[W::BUF];
   long long b; int n, tile;
-  if (!locate(p, blockIdx.x / p.heads, QT, b, n, tile)) return;
-  tile = (n + QT - 1) / QT - 1 - tile;                      // causal: the tiles with most keys start first
+  if (!(longest_first<4 * W::BUF * sizeof(T)>(p) ? locate_longest(p, blockIdx.x / p.heads, QT, b, n, tile) : locate(p, blockIdx.x / p.heads, QT, b, n, tile))) return;
   const int head = head_of(blockIdx.x % p.heads, p.heads, p.kv_heads), kv = head / (p.heads / p.kv_heads);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int qw = tile * QT + (SPLIT ? 0 : 32 * w), qi = qw + (lane & 31);  // the wave's first query, the lane's
@@ -333,8 +381,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   __shared__ __attribute__((aligned(16))) T ks1[W::BUF];
   __shared__ __attribute__((aligned(16))) T vs1[W::BUF];
   long long b; int n, tile;
-  if (!locate(p, blockIdx.x / p.heads, QT, b, n, tile)) return;
-  tile = (n + QT - 1) / QT - 1 - tile;
+  if (!(longest_first<4 * W::BUF * sizeof(T)>(p) ? locate_longest(p, blockIdx.x / p.heads, QT, b, n, tile) : locate(p, blockIdx.x / p.heads, QT, b, n, tile))) return;
   const int head = head_of(blockIdx.x % p.heads, p.heads, p.kv_heads), kv = head / (p.heads / p.kv_heads);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int qw = tile * QT + (SPLIT ? 0 : 32 * w), qi = qw + (lane & 31);
@@ -478,7 +525,10 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   __shared__ __attribute__((aligned(16))) float cs0[3][64];   // per staged query: -delta, -lse (log2), exponent of its do scale
   __shared__ __attribute__((aligned(16))) float cs1[3][64];
   long long b; int n, tile;
-  if (!locate(p, blockIdx.x / p.kv_heads, KB, b, n, tile)) return;
+  // here already with more than one workgroup a compute unit, which two then share: 16 x 1024 as above 178 / 141 us the whole pass
+  const bool longest = p.block && gridDim.x * gridDim.y > 256;
+  if (!(longest ? locate_longest(p, blockIdx.x / p.kv_heads, KB, b, n, tile) : locate(p, blockIdx.x / p.kv_heads, KB, b, n, tile))) return;
+  if (longest) tile = (n + KB - 1) / KB - 1 - tile;         // the first keys have the longest walks
   const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int k0 = tile * KB, kw = k0 + 32 * w, ki = kw + (lane & 31);
