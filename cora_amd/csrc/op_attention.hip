@@ -230,15 +230,15 @@ __device__ __forceinline__ void join_own(f32x16 (&acc)[D / 32], float* lds, int 
 // from LDS, which four SIMDs reading at once is all that LDS gives (128 bytes a cycle).  One workgroup per 128 queries, two to
 // a compute unit; or, for few rows, four waves that share 32 queries (the rule and its figures are at run below).  Measured, causal
 // bf16: 16384 tokens x 16 heads of 128 1.05 ms, 1050 TFLOP/s (a large library product: 1133); fp32 64 images of 196 tokens x 8 heads of 48
-// 88 us, of which a quarter is padding (48 channels to 64, 196 keys to 224).
+// 77 us, much of it padding (196 queries to 256, 196 keys to 224, in the second product 48 channels to 64).
 // The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
 // Each row goes by its own scores, so its result does not depend on which other rows share its tile.
-template <typename T, int D, int NW, bool SPLIT>
+template <typename T, int D, int DK, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_fwd(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   typedef Walk<T, D, NW, SPLIT> W;
-  constexpr int KT = W::KT, QT = W::QT, NC = D / O::CH, NS = KT / O::CH;
+  constexpr int KT = W::KT, QT = W::QT, NC = DK / O::CH, NS = KT / O::CH;
   __shared__ __attribute__((aligned(16))) T ks0[W::BUF];
   __shared__ __attribute__((aligned(16))) T vs0[W::BUF];
   __shared__ __attribute__((aligned(16))) T ks1[W::BUF];
@@ -372,12 +372,12 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // enters with a power of two 2^-e that brings its largest element to [1, 2); e is kept for the other kernel, beside
 // -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves nothing and
 // triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
-template <typename T, int D, int NW, bool SPLIT>
+template <typename T, int D, int DK, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
   typedef Walk<T, D, NW, SPLIT> W;
-  constexpr int KT = W::KT, QT = W::QT, NC = D / O::CH;
+  constexpr int KT = W::KT, QT = W::QT, NC = DK / O::CH;
   __shared__ __attribute__((aligned(16))) T ks0[W::BUF];
   __shared__ __attribute__((aligned(16))) T vs0[W::BUF];
   __shared__ __attribute__((aligned(16))) T ks1[W::BUF];
@@ -517,11 +517,11 @@ template <int READS, int PER, int N, int GROUP> __device__ __forceinline__ void 
 // Four products.  The two accumulators and the own keys and values fill the registers: at 128 channels one wave per SIMD, and
 // vector work (exp, masks, packing) is not hidden behind another wave's matrix instructions: 2.7 ms, 810 TFLOP/s at the size above.
 // Staged rows behind the sequence are zeros, and so are their constants: their p is 1, but do and ds are zero.
-template <typename T, int D, int NW>
+template <typename T, int D, int DK, int NW>
 __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1 : 2) void attn_bwd_kv(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
-  constexpr int QT = sizeof(T) == 4 ? 32 : 64, KB = 32 * NW, NC = D / O::CH;
+  constexpr int QT = sizeof(T) == 4 ? 32 : 64, KB = 32 * NW, NC = DK / O::CH;
   __shared__ __attribute__((aligned(16))) T qs0[QT * D];
   __shared__ __attribute__((aligned(16))) T ds0[QT * D];
   __shared__ __attribute__((aligned(16))) T qs1[QT * D];
@@ -678,14 +678,14 @@ __global__ __launch_bounds__(256) void attn_bwd_sum(const AttnP p) {
 long long slots(const AttnP& p, int tr) {
   return p.cu ? p.rows / tr + p.nseq : (long long)p.nseq * ((p.seqlen + tr - 1) / tr);
 }
-template <typename T, int D, int NW, bool SPLIT> int fwd(const AttnP& p, hipStream_t st) {
-  attn_fwd<T, D, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
+template <typename T, int D, int DK, int NW, bool SPLIT> int fwd(const AttnP& p, hipStream_t st) {
+  attn_fwd<T, D, DK, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
-template <typename T, int D, int NW, bool SPLIT> int bwd(const AttnP& p, hipStream_t st) {
-  attn_bwd_q<T, D, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
+template <typename T, int D, int DK, int NW, bool SPLIT> int bwd(const AttnP& p, hipStream_t st) {
+  attn_bwd_q<T, D, DK, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return 1;
-  attn_bwd_kv<T, D, 4><<<dim3((unsigned)(slots(p, 128) * p.kv_heads), (unsigned)p.parts), 256, 0, st>>>(p);
+  attn_bwd_kv<T, D, DK, 4><<<dim3((unsigned)(slots(p, 128) * p.kv_heads), (unsigned)p.parts), 256, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return 1;
   if (p.parts == 1) return 0;
   attn_bwd_sum<T><<<dim3((unsigned)((p.rows * p.kv_heads * p.d / 4 + 255) / 256), 2), 256, 0, st>>>(p);
@@ -696,14 +696,19 @@ template <typename T, int D, int NW, bool SPLIT> int bwd(const AttnP& p, hipStre
 // for causal walks over long sequences, whose last tiles keep the rest waiting.  Forward, us, split / not:
 //   fp32 D 64:  16 x 1024 tokens x 1 head (W 512) 55 / 77;  4 x 1024 x 8 (W 1024) 107 / 86;  1 x 4096 x 8 causal 193 / 285
 //   bf16 D 128: 1 x 4096 x 2 (W 256) 43 / 77;  16 x 1024 x 1 (W 512) 32 / 26;  1 x 16384 x 1 causal (W 512) 171 / 291
-template <typename T, int D, bool BWD> int run(const AttnP& p, hipStream_t st) {
+template <typename T, int D, int DK, bool BWD> int run(const AttnP& p, hipStream_t st) {
   constexpr int NS = sizeof(T) == 4 && D > 64 ? 2 : 4;      // waves whose buffers fit LDS
   const long long w = p.rows * p.heads / 32, most = (D <= 64 ? 512 : 256) * (p.block && p.rows / p.nseq >= 2048 ? 2 : 1);
-  if (w <= most) { if constexpr (BWD) return bwd<T, D, NS, true>(p, st); else return fwd<T, D, NS, true>(p, st); }
-  if constexpr (BWD) return bwd<T, D, 4, false>(p, st); else return fwd<T, D, 4, false>(p, st);
+  if (w <= most) { if constexpr (BWD) return bwd<T, D, DK, NS, true>(p, st); else return fwd<T, D, DK, NS, true>(p, st); }
+  if constexpr (BWD) return bwd<T, D, DK, 4, false>(p, st); else return fwd<T, D, DK, 4, false>(p, st);
 }
+// D: channels of the tiles and of the results, 32 at a time; DK: channels of the score products.  In fp32, which the matrix unit
+// bounds, 16 of padding are left out there: 64 images of 196 tokens, 8 heads of 48, forward / dq / dk and dv 77 / 107 / 146 us,
+// with all 64 channels 88 / 125 / 159.  In 16 bits it gives nothing (fp16, heads of 80 as 80 or 96 channels: 80 / 101 / 144, 78 / 104 / 143).
 template <typename T, bool BWD> int run_d(const AttnP& p, hipStream_t st) {
-  return p.d <= 32 ? run<T, 32, BWD>(p, st) : p.d <= 64 ? run<T, 64, BWD>(p, st) : p.d <= 96 ? run<T, 96, BWD>(p, st) : run<T, 128, BWD>(p, st);
+  if constexpr (sizeof(T) == 4)
+    if (p.d > 32 && p.d <= 48) return run<T, 64, 48, BWD>(p, st);
+  return p.d <= 32 ? run<T, 32, 32, BWD>(p, st) : p.d <= 64 ? run<T, 64, 64, BWD>(p, st) : p.d <= 96 ? run<T, 96, 96, BWD>(p, st) : run<T, 128, 128, BWD>(p, st);
 }
 template <bool BWD> int run_t(const AttnP& p, int dtype, hipStream_t st) {
   return dtype == OP_F32 ? run_d<float, BWD>(p, st) : dtype == OP_BF16 ? run_d<__bf16, BWD>(p, st) : run_d<_Float16, BWD>(p, st);
