@@ -225,12 +225,22 @@ __device__ __forceinline__ void join_own(f32x16 (&acc)[D / 32], float* lds, int 
   }
 }
 
+// Issue order of the block it stands in: READS reads of LDS first, then N times M matrix instructions followed by PER more reads.
+// Left alone the compiler reads an operand right before its use, and where few waves share a SIMD nothing else hides
+// the way from LDS: dk/dv of 16-bit types at 128 channels 2.9 ms, so 2.7; q k of the fp32 forward pass 77 us, so 73 (sizes as below).
+// The 16-bit forward pass and dq, whose tiles are longer, gain nothing or lose.
+template <int READS, int PER, int N, int GROUP, int M = 1> __device__ __forceinline__ void feed() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, GROUP);
+#pragma unroll
+  for (int c = 0; c < N; ++c) { __builtin_amdgcn_sched_group_barrier(0x8, M, GROUP); __builtin_amdgcn_sched_group_barrier(0x100, PER, GROUP); }
+}
+
 // ---- forward -------------------------------------------------------------------------------------
 // Bound by the matrix units and, as close behind, by LDS: every matrix instruction (32 cycles of a SIMD in 16 bits) takes 1 KB
 // from LDS, which four SIMDs reading at once is all that LDS gives (128 bytes a cycle).  One workgroup per 128 queries, two to
 // a compute unit; or, for few rows, four waves that share 32 queries (the rule and its figures are at run below).  Measured, causal
 // bf16: 16384 tokens x 16 heads of 128 1.05 ms, 1050 TFLOP/s (a large library product: 1133); fp32 64 images of 196 tokens x 8 heads of 48
-// 77 us, much of it padding (196 queries to 256, 196 keys to 224, in the second product 48 channels to 64).
+// 73 us, much of it padding (196 queries to 256, 196 keys to 224, in the second product 48 channels to 64).
 // The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
 // Each row goes by its own scores, so its result does not depend on which other rows share its tile.
@@ -294,6 +304,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 #pragma unroll
       for (int c = 0; c < NC; ++c) s[t] = O::mma(L::row_frag(k, 32 * t, c, lane), qf[c], s[t]);
     }
+    if (sizeof(T) == 4) feed<3, 1, NC, 0, 4>();
     if (j0 + KT > wave_min) {
 #pragma unroll
       for (int t = 0; t < KT / 32; ++t)
@@ -499,15 +510,6 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     if (w) return;
   }
   if (own) store_own<T, D>((T*)p.dq + row * p.dqr + (long long)head * p.dqh, acc, back, p.d, h);
-}
-
-// Issue order of the block it stands in: READS reads of LDS first, then N matrix instructions, each followed by PER more reads.
-// Left alone the compiler reads an operand right before its use, and with one wave per SIMD (128 channels) nothing else hides
-// the way from LDS.
-template <int READS, int PER, int N, int GROUP> __device__ __forceinline__ void feed() {
-  __builtin_amdgcn_sched_group_barrier(0x100, READS, GROUP);
-#pragma unroll
-  for (int c = 0; c < N; ++c) { __builtin_amdgcn_sched_group_barrier(0x8, 1, GROUP); __builtin_amdgcn_sched_group_barrier(0x100, PER, GROUP); }
 }
 
 // ---- backward: dk and dv -------------------------------------------------------------------------
