@@ -329,14 +329,15 @@ __global__ __launch_bounds__(512) void ortho_small(const OrthoP p, const OrthoCo
   }
 }
 
-// One product for all matrices.  STEP 0: A = X X^T; 1: P = a I + b A + c A A; 2: X' = P X (last: to the caller's matrix).
-// Tile TS x TS: 64 with four waves of 32 x 32, for matrices that give few tiles; 128 with four waves of 64 x 64, two
-// workgroups a compute unit (the symmetric products of few wide matrices); or 256 with eight waves of 128 x 64, which halves what a flop reads from L2 (the 128 tile's 43
-// bytes a cycle and compute unit exceed it).  The first operand gives
-// the output's columns, the second its rows (op_tile.h), so a lane holds four neighbouring columns of one output row.  Slabs go from global memory straight into one
-// of two LDS buffers while the other is worked on; a lane fetches the 16-byte piece that belongs at its place of the
-// swizzled tile.  Rows outside a matrix arrive as zeros, columns behind it as whatever follows (the columns up to ldn and ldm
-// are stored as zeros, what lies behind gives nothing that is stored).
+// One product for all matrices.  STEP 0: A = X X^T; 1: P = a I + b A + c A A; 2: X' = P X (last: to the caller's
+// matrix). Tile TS x TS: 64 with four waves of 32 x 32, for matrices that give few tiles; 128 with four waves of 64 x
+// 64, two workgroups a compute unit (the symmetric products of few wide matrices); or 256 with eight waves of 128 x 64,
+// which halves what a flop reads from L2 (the 128 tile's 43 bytes a cycle and compute unit exceed it).  The first
+// operand gives the output's columns, the second its rows (op_tile.h), so a lane holds four neighbouring columns of one
+// output row.  Slabs go from global memory straight into one of two LDS buffers while the other is worked on; a lane
+// fetches the 16-byte piece that belongs at its place of the swizzled tile.  Rows outside a matrix arrive as zeros,
+// columns behind it as whatever follows (the columns up to ldn and ldm are stored as zeros, what lies behind gives
+// nothing that is stored).
 constexpr int threads_of(int ts) { return ts == 256 ? 512 : 256; }
 template <typename T, int STEP, bool FULL, int TS>
 __global__ __launch_bounds__(threads_of(TS), 2) void ortho_product(const OrthoP p, const int cuts, const int cur, const int last, const float ca, const float cb, const float cc) {
@@ -651,8 +652,9 @@ template <typename T, int RT, int XT> int run_small(const OrthoP& p, const Ortho
   return hipGetLastError() != hipSuccess;
 }
 
-// How a stack is worked on: in one workgroup with 1 to 4 row tiles of 32 (+ 8: more than 16 tiles of X), or with tiles: 64, or 256 for m >= 1024, and for
-// bf16 results (+ 1) of m >= 256 with fewer instructions a product (below that it costs precision and saves nothing)
+// How a stack is worked on: in one workgroup with 1 to 4 row tiles of 32 (+ 8: more than 16 tiles of X), or with tiles:
+// 64, or 256 for m >= 1024, and for bf16 results (+ 1) of m >= 256 with fewer instructions a product (below that it
+// costs precision and saves nothing)
 int class_of(const OrthoG& g, bool bf16) {
   if (ortho_is_small(g)) return (g.m + 31) / 32 + ((g.m + 31) / 32 * ((g.n + 31) / 32) > 16 ? 8 : 0);
   return (g.m >= 1024 ? 256 : 64) + (bf16 && g.m >= 256);
