@@ -295,6 +295,34 @@ def test_attention_what_the_mask_hides_does_not_count(lens, heads, kv, d, block,
             assert torch.isnan(got[2][~first.cuda()][:, -1]).any(-1).all(), name
 
 
+@pytest.mark.parametrize("n,seqs,heads,d,block,dtype", [(1024, 16, 1, 64, 64, F32), (700, 40, 2, 96, 1, BF16), (129, 130, 4, 32, 1, F16)])
+def test_attention_many_causal_tiles_with_and_without_a_table(n, seqs, heads, d, block, dtype):
+    """Enough tiles that the longest start first: where a tile runs changes no result."""
+    cu, qkv, dout = packed([n] * seqs, 0, heads, heads, d, dtype)
+    q, k, v = split(qkv.cuda(), heads, heads)
+    results = []
+    for kw in (dict(seq_len=n), dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"))):
+        out, lse = ca.attention(q, k, v, causal_block=block, **kw)
+        results.append((out, lse) + ca.attention_backward(dout.cuda(), q, k, v, out, lse, causal_block=block, **kw))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    ref, bound = attention_ref(*split(qkv[:n], heads, heads), [0, n], block, d ** -0.5, dout[:n])
+    for name, t in zip(("out", "dq", "dk", "dv"), (results[0][0],) + results[0][2:]):
+        within(t[:n], ref[name], bound[name], name)
+
+
+def test_attention_many_causal_tiles_with_empty_sequences():
+    lens = [0, 1000, 0, 1, 700, 33, 2100, 0, 900, 1300, 31, 1024, 0]
+    cu, qkv, dout = packed(lens, 40, 12, 4, 32, BF16)
+    ref, bound = attention_ref(*split(qkv, 12, 4), cu, 16, 32 ** -0.5, dout)
+    q, k, v = split(qkv.cuda(), 12, 4)
+    kw = dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), causal_block=16)
+    out, lse = ca.attention(q, k, v, **kw)
+    within(out[:cu[-1]], ref["out"][:cu[-1]], bound["out"][:cu[-1]], "out")
+    for n, t in zip(("dq", "dk", "dv"), ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)):
+        within(t[:cu[-1]], ref[n][:cu[-1]], bound[n][:cu[-1]], n)
+
+
 def test_attention_broken_tables_stay_in_bounds():
     """Descending and out-of-range bounds: rows outside [0, rows) are never touched and the call ends."""
     q = randn(50, 2, 32, dtype=BF16).cuda()
