@@ -518,7 +518,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // fp32 and are added in order by attn_bwd_sum: few workgroups with long walks would leave most of the chip idle.
 // Four products.  The two accumulators and the own keys and values fill the registers: at 128 channels one wave per SIMD, and
 // vector work (exp, masks, packing) is not hidden behind another wave's matrix instructions: 2.7 ms, 810 TFLOP/s at the size above.
-// Staged rows behind the sequence are zeros, and so are their constants: their p is 1, but do and ds are zero.
+// Staged rows behind the sequence are zeros, or pieces of its last rows where rows repeat or overlap (a stride below the
+// row's length); their -lse is set to -infinity, so their p and ds are zero whatever is there.
 template <typename T, int D, int DK, int NW>
 __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1 : 2) void attn_bwd_kv(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
@@ -576,12 +577,14 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   auto work = [&](int, T* qt, T* dt_, float (&cs)[3][64]) {
     const int q0 = qbeg + wq * QT;
     if (++wq == ntile) wq = 0;
-    if (q0 < all_max) {
+    const bool edge = q0 < all_max, tail = q0 + QT > n;
+    if (tail && w == 0 && lane >= n - q0) cs[1][lane] = -INFINITY;
+    if (edge) {
       auto mark = [&](int id) { cs[1][id / (D / O::E)] = NAN; };
       quarantine<T, D, QT, NW>(qt, w, lane, mark);
       quarantine<T, D, QT, NW>(dt_, w, lane, mark);
-      lds_barrier();
     }
+    if (edge || tail) lds_barrier();
     if (kw >= n) return;
     if (F16) {
       float e = q0 + lane < n ? cs[2][lane] : NO_EXP;
