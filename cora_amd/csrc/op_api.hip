@@ -181,7 +181,7 @@ void ortho_place(OrthoP& p, void* ws) {
   p.ws = (unsigned short*)((char*)ws + ((size_t)p.matrices * ORTHO_PARTS * sizeof(double) + 255) / 256 * 256);
 }
 
-static size_t constants_bytes(long long rows, int heads) { return ((size_t)rows * heads * 3 * sizeof(float) + 15) / 16 * 16; }
+static size_t constants_bytes(long long rows, int heads) { return ((size_t)rows * heads * 2 * sizeof(float) + 15) / 16 * 16; }
 size_t attention_ws_bytes(int dtype, long long rows, int nseq, int heads, int kv_heads, int d, int block) {
   const int parts = attention_parts(dtype, rows, nseq, heads, kv_heads, block);
   return constants_bytes(rows, heads) + (parts > 1 ? (size_t)parts * 2 * sizeof(float) * (size_t)rows * (size_t)kv_heads * (size_t)d : 0);

@@ -113,7 +113,6 @@ __device__ __forceinline__ bool locate_longest(const AttnP& p, int i, int TR, lo
   return (long long)tile * TR < n;                // a broken table may give no such tile
 }
 
-constexpr float NO_EXP = -1e30f;   // exponent of a row of zeros, or with an infinity (attn_bwd_q)
 __device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 __device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 // row of accumulator register r of lane half h in a 32 x 32 tile
@@ -233,6 +232,35 @@ template <int READS, int PER, int N, int GROUP, int M = 1> __device__ __forceinl
   __builtin_amdgcn_sched_group_barrier(0x100, READS, GROUP);
 #pragma unroll
   for (int c = 0; c < N; ++c) { __builtin_amdgcn_sched_group_barrier(0x8, M, GROUP); __builtin_amdgcn_sched_group_barrier(0x100, PER, GROUP); }
+}
+
+// fp16 holds 2^-24 .. 2^16, and ds ~ p do / sqrt(n) of an unscaled loss lies below.  A tile of ds, whose column is the lane's own
+// row, therefore enters its product times mul = 2^-e, and so do the sums acc.  Every lane has an e of its own: small values of a
+// row keep their bits whatever the other rows hold.  Kept while the column's largest value comes out in 2^-8 .. 2^15 (what fp16 then
+// rounds by 2^-25 is 2^-17 of it), else set so that it is in 2^4 .. 2^5: e is hardly ever changed, and costs a search of the tile.
+constexpr int LEAST_EXP = -30;     // ds below 2^-38 gives nothing in fp16 results; the sums times 2^30 stay finite
+template <int N> __device__ __forceinline__ void fit_half(f32x16& ds, f32x16 (&acc)[N], int& e, float& mul) {
+  float big = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(ds[r]));
+  // a lane pair shares a column: it is too small if both halves are, and not both empty
+  unsigned long long small = __ballot(big * mul < 0x1p-8f && e > LEAST_EXP), none = __ballot(big == 0.f);
+  small &= small >> 32; none &= none >> 32;
+  if ((unsigned)(small & ~none) || __any(big * mul > 0x1p15f)) {
+    big = half_max(big);
+    int to = e;
+    if (big < INFINITY && (big * mul > 0x1p15f || (big > 0.f && big * mul < 0x1p-8f)))
+      to = min(max(__builtin_amdgcn_frexp_expf(big) - 5, LEAST_EXP), 90);
+    const float f = __builtin_amdgcn_ldexpf(1.f, e - to);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+    e = to;
+    mul = __builtin_amdgcn_ldexpf(1.f, -to);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ds[r] *= mul;
 }
 
 // ---- forward -------------------------------------------------------------------------------------
@@ -379,10 +407,9 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // ---- backward: dq (and the row constants the dk/dv kernel reads) ---------------------------------
 // Three products where the forward pass has two, bound like it: 16384 tokens x 16 heads of 128, causal bf16, 1.55 ms, 1060 TFLOP/s.
 // q k and do v are computed here and in the dk/dv kernel: seven products instead of five, but no atomics and no ds in memory.
-// fp16 holds nothing below 2^-24, and ds ~ p do / sqrt(n) of an unscaled loss lies there.  Every query row of do therefore
-// enters with a power of two 2^-e that brings its largest element to [1, 2); e is kept for the other kernel, beside
-// -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves nothing and
-// triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
+// In fp16 every query row of do enters with a power of two 2^-e that brings its largest element to [1, 2).
+// The row constants are -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves
+// nothing and triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
 template <typename T, int D, int DK, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
@@ -425,7 +452,6 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     big = half_max(big);
     const int e = big > 0.f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
     dscale = __builtin_amdgcn_ldexpf(1.f, -e); back = __builtin_amdgcn_ldexpf(p.scale, e);
-    if (own && h == 0 && (!SPLIT || w == 0)) p.delta[2 * plane + at] = big > 0.f && big < INFINITY ? (float)e : NO_EXP;
   }
   const float lse2 = own ? p.lse[at] * CORA_LOG2E : 0.f, sl2 = p.scale * CORA_LOG2E;
   // Where a wave sees one key tile only, delta is taken from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
@@ -529,8 +555,8 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   __shared__ __attribute__((aligned(16))) T ds0[QT * D];
   __shared__ __attribute__((aligned(16))) T qs1[QT * D];
   __shared__ __attribute__((aligned(16))) T ds1[QT * D];
-  __shared__ __attribute__((aligned(16))) float cs0[3][64];   // per staged query: -delta, -lse (log2), exponent of its do scale
-  __shared__ __attribute__((aligned(16))) float cs1[3][64];
+  __shared__ __attribute__((aligned(16))) float cs0[2][64];   // per staged query: -delta, -lse (log2)
+  __shared__ __attribute__((aligned(16))) float cs1[2][64];
   long long b; int n, tile;
   // here already with more than one workgroup a compute unit, which two then share: 16 x 1024 as above 178 / 141 us the whole pass
   const bool longest = p.block && gridDim.x * gridDim.y > 256;
@@ -560,21 +586,22 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
 #pragma unroll
     for (int r = 0; r < 16; ++r) { ak[i][r] = 0.f; av[i][r] = 0.f; }
   const float sl2 = p.scale * CORA_LOG2E;
-  float ecur = NO_EXP;                                  // F16: exponent ak is scaled by
+  [[maybe_unused]] int ex = 0;                          // F16: ak and ds are scaled by mul = 2^-ex
+  [[maybe_unused]] float mul = 1.f;
   [[maybe_unused]] const long long plane = (long long)p.heads * p.rows;
 
   int fhead = kv * group + it0 / ntile, fq = it0 % ntile, wq = fq;       // the next tile to fetch and to work on (counted: a division per tile is 6 % of the time)
-  auto fetch = [&](int, T* q, T* d, float (&cs)[3][64]) {
+  auto fetch = [&](int, T* q, T* d, float (&cs)[2][64]) {
     const int q0 = qbeg + fq * QT, head = fhead;
     if (++fq == ntile) { fq = 0; ++fhead; }
     into_q((const T*)p.q + (b + q0) * p.qr + (long long)head * p.qh, n - q0, q, w);
     into_d((const T*)p.dout + (b + q0) * p.dor + (long long)head * p.doh, n - q0, d, w);
     // constants: one request of 64 floats each (fp32 stages 32 queries and asks for 32 more than it needs)
 #pragma unroll
-    for (int k = 0; k < (F16 ? 3 : 2); ++k)
+    for (int k = 0; k < 2; ++k)
       if (w == k % NW) REQUEST(p.delta + k * plane + (long long)head * p.rows + b + q0, 4 * min(n - q0, 64), cs[k], 4, 4 * lane);
   };
-  auto work = [&](int, T* qt, T* dt_, float (&cs)[3][64]) {
+  auto work = [&](int, T* qt, T* dt_, float (&cs)[2][64]) {
     const int q0 = qbeg + wq * QT;
     if (++wq == ntile) wq = 0;
     const bool edge = q0 < all_max, tail = q0 + QT > n;
@@ -586,20 +613,6 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
     }
     if (edge || tail) lds_barrier();
     if (kw >= n) return;
-    if (F16) {
-      float e = q0 + lane < n ? cs[2][lane] : NO_EXP;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) e = fmaxf(e, __shfl_xor(e, o, 64));
-      if (e > ecur) {                                   // larger gradients than before: bring the sum to their scale
-        const float f = ecur == NO_EXP ? 0.f : __builtin_amdgcn_exp2f(ecur - e);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) ak[i][r] *= f;
-        ecur = e;
-      }
-    }
-    const float dscale = F16 && ecur != NO_EXP ? __builtin_amdgcn_exp2f(-ecur) : 1.f;
 #pragma unroll D == 128 ? 1 : 2
     for (int t = 0; t < QT / 32; ++t) {
       f32x16 s, dp;
@@ -627,10 +640,8 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
           if (q0 + 32 * t + acc_row(r, h) < qmin) { s[r] = 0.f; dp[r] = 0.f; }       // p = 0 does not hide an infinite do v
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        dp[r] *= s[r];
-        if (F16) dp[r] *= dscale;
-      }
+      for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+      if constexpr (F16) fit_half(dp, ak, ex, mul);
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
         const frag pf = O::pack(s, c), gf = O::pack(dp, c);
@@ -649,7 +660,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
 #undef FETCH
 #undef WORK
   if (own) {
-    const float f = F16 && ecur != NO_EXP ? p.scale * __builtin_amdgcn_exp2f(ecur) : p.scale;
+    const float f = F16 ? __builtin_amdgcn_ldexpf(p.scale, ex) : p.scale;
     if (p.parts > 1) {
       const long long half = p.rows * p.kv_heads * p.d;
       float* dst = p.partial + 2 * half * blockIdx.y + ((b + ki) * p.kv_heads + kv) * p.d;

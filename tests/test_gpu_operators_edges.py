@@ -1,5 +1,7 @@
 """Calls of the stand-alone operators that their documentation allows at its edges: repeated and overlapping rows, gradients of
 very different sizes, values that are not finite, long sequences, launches of every tile size."""
+import math
+
 import pytest
 import torch
 
@@ -42,3 +44,44 @@ def test_attention_rows_that_repeat_or_overlap(lens, step, block, dtype):
         within(lse, ref["lse"], bound["lse"], (names, "lse"))
         for n, t in zip(("dq", "dk", "dv"), ca.attention_backward(gpu["dout"], gpu["q"], gpu["k"], gpu["v"], out, lse, **kw)):
             within(t, ref[n], bound[n], (names, n))
+
+
+def by_key(q, k, v, cu, block, scale, dout):
+    """attention_ref with the part of the fp16 gradients' bounds that belongs to small ds taken from what a key (dk) or a query (dq)
+    itself sees, instead of the sequence's largest gradient: ds enters its products times a power of two that keeps the largest one
+    of 32 at 2^-8 at least, where fp16 is off by 2^-25 absolutely: 2^-17 of the largest ds of the key or query."""
+    ref, bound = attention_ref(q, k, v, cu, block, scale, dout)
+    heads = q.shape[1]
+    g, flat = heads // k.shape[1], 2.0 ** -24
+    for b, e in zip(cu[:-1], cu[1:]):
+        i = torch.arange(e - b)
+        vis = i[None, :] // block <= i[:, None] // block if block else torch.ones(e - b, e - b, dtype=torch.bool)
+        for h in range(heads):
+            Q, K, V, G = q[b:e, h].double(), k[b:e, h // g].double(), v[b:e, h // g].double(), dout[b:e, h].double()
+            p = torch.softmax(((Q @ K.T) * scale).masked_fill(~vis, -math.inf), 1)
+            ds = (p * (G @ V.T - (G * (p @ V)).sum(1, keepdim=True))).abs()
+            old = flat * G.abs().amax() * vis
+            bound["dk"][b:e, h // g] += scale * (2.0 ** -17 * ds.amax(0)[:, None] * vis.T - old.T) @ Q.abs()
+            bound["dq"][b:e, h] += scale * (2.0 ** -17 * ds.amax(1)[:, None] * vis - old) @ K.abs()
+    return ref, bound
+
+
+@pytest.mark.parametrize("lens,heads,kv,d,block", [([512], 2, 1, 64, 1), ([300, 97], 4, 2, 128, 1), ([700], 1, 1, 32, 50), ([200] * 40, 4, 4, 80, 1)])
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 20])
+def test_attention_fp16_dk_of_keys_that_large_gradients_do_not_see(lens, heads, kv, d, block, ratio):
+    """The first token's gradient is far larger than the others'; keys that it does not see keep their precision."""
+    cu, qkv, dout = packed(lens, 0, heads, kv, d, F16)
+    dout = dout.float().clamp(-3, 3) * 8 / ratio
+    dout[cu[:-1]] *= ratio
+    dout = dout.to(F16)
+    ref, bound = by_key(*split(qkv, heads, kv), cu, block, d ** -0.5, dout)
+    q, k, v = split(qkv.cuda(), heads, kv)
+    kw = dict(cu_seqlens=table(cu), causal_block=block)
+    out, lse = ca.attention(q, k, v, **kw)
+    dk = ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)[1]
+    hidden = torch.ones(cu[-1], dtype=torch.bool)
+    for b in cu[:-1]:
+        hidden[b:b + block] = False                       # the first token sees its own block
+    within(dk[hidden.cuda()], ref["dk"][hidden], bound["dk"][hidden], "dk")
+    assert bound["dk"][hidden].norm() < 0.1 * ref["dk"][hidden].norm()     # the bound would not let them be lost: reference values only
+    within(dk, ref["dk"], bound["dk"], "all dk")
