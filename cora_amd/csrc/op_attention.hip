@@ -407,7 +407,6 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // ---- backward: dq (and the row constants the dk/dv kernel reads) ---------------------------------
 // Three products where the forward pass has two, bound like it: 16384 tokens x 16 heads of 128, causal bf16, 1.55 ms, 1060 TFLOP/s.
 // q k and do v are computed here and in the dk/dv kernel: seven products instead of five, but no atomics and no ds in memory.
-// In fp16 every query row of do enters with a power of two 2^-e that brings its largest element to [1, 2).
 // The row constants are -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves
 // nothing and triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
 template <typename T, int D, int DK, int NW, bool SPLIT>
@@ -437,22 +436,18 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   const Fetch<T, D, KT, W::FW> fk(p.kr, p.d, fw, lane), fv(p.vr, p.d, fw, lane);
   const long long row = b + qi, at = (long long)head * p.rows + row, plane = (long long)p.heads * p.rows;
   frag qf[NC], df[NC];
-  float delta = 0.f, big = 0.f;
+  float delta = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     qf[c] = L::own_frag((const T*)p.q + row * p.qr + (long long)head * p.qh, own, c, p.d, lane);
     df[c] = L::own_frag((const T*)p.dout + row * p.dor + (long long)head * p.doh, own, c, p.d, lane);
     const frag of = L::own_frag((const T*)p.o + row * p.orow + (long long)head * p.oh, own, c, p.d, lane);
 #pragma unroll
-    for (int i = 0; i < O::E; ++i) { delta = __builtin_fmaf((float)df[c][i], (float)of[i], delta); big = fmaxf(big, fabsf((float)df[c][i])); }
+    for (int i = 0; i < O::E; ++i) delta = __builtin_fmaf((float)df[c][i], (float)of[i], delta);
   }
   delta = half_sum(delta);
-  float dscale = 1.f, back = p.scale;
-  if (F16) {
-    big = half_max(big);
-    const int e = big > 0.f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
-    dscale = __builtin_amdgcn_ldexpf(1.f, -e); back = __builtin_amdgcn_ldexpf(p.scale, e);
-  }
+  [[maybe_unused]] int ex = 0;                              // F16: acc and ds are scaled by mul = 2^-ex
+  [[maybe_unused]] float mul = 1.f;
   const float lse2 = own ? p.lse[at] * CORA_LOG2E : 0.f, sl2 = p.scale * CORA_LOG2E;
   // Where a wave sees one key tile only, delta is taken from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
   // 16 bits, which delta otherwise inherits, counts most in rows that see few keys.
@@ -508,16 +503,13 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
         dp = O::mma(L::row_frag(v, 32 * t, c, lane), df[c], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)) * dp[r];
-        if (F16) pr *= dscale;
-        s[r] = pr;
-      }
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)) * dp[r];
       if (j0 + 32 * t + 32 > wave_min) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (j0 + 32 * t + acc_row(r, h) >= lim) s[r] = 0.f;
       }
+      if constexpr (F16) fit_half(s, acc, ex, mul);
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
         const frag pf = O::pack(s, c);
@@ -531,11 +523,19 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   WALK(SPLIT ? (end + NW * KT - 1) / (NW * KT) : (end + KT - 1) / KT, FETCH, WORK)
 #undef FETCH
 #undef WORK
-  if constexpr (SPLIT) {
+  float f = F16 ? __builtin_amdgcn_ldexpf(p.scale, ex) : p.scale;
+  if constexpr (SPLIT) {                                    // the waves' exponents differ
+    if constexpr (F16) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+      f = 1.f;
+    }
     join_own<D, NW>(acc, reinterpret_cast<float*>(ks0), w, lane);
     if (w) return;
   }
-  if (own) store_own<T, D>((T*)p.dq + row * p.dqr + (long long)head * p.dqh, acc, back, p.d, h);
+  if (own) store_own<T, D>((T*)p.dq + row * p.dqr + (long long)head * p.dqh, acc, f, p.d, h);
 }
 
 // ---- backward: dk and dv -------------------------------------------------------------------------

@@ -85,3 +85,19 @@ def test_attention_fp16_dk_of_keys_that_large_gradients_do_not_see(lens, heads, 
     within(dk[hidden.cuda()], ref["dk"][hidden], bound["dk"][hidden], "dk")
     assert bound["dk"][hidden].norm() < 0.1 * ref["dk"][hidden].norm()     # the bound would not let them be lost: reference values only
     within(dk, ref["dk"], bound["dk"], "all dk")
+
+
+@pytest.mark.parametrize("lens,block", [([2] * 50, 0), ([2, 3, 200], 1), ([3000], 0)])
+def test_attention_fp16_gradients_of_large_values(lens, block):
+    """Large values, small gradients: their products fit fp16, the products with a gradient brought to 1 would not."""
+    d = 128
+    cu, qkv, dout = packed(lens, 0, 2, 2, d, F16)
+    qkv[:, 4:] = (qkv[:, 4:].float() * 1.5e4).clamp(-6e4, 6e4).to(F16)
+    dout = (dout.float() * 1e-3).to(F16)
+    ref, bound = by_key(*split(qkv, 2, 2), cu, block, d ** -0.5, dout)
+    q, k, v = split(qkv.cuda(), 2, 2)
+    kw = dict(cu_seqlens=table(cu), causal_block=block)
+    out, lse = ca.attention(q, k, v, **kw)
+    for n, t in zip(("dq", "dk", "dv"), ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)):
+        assert ref[n].abs().max() < 6e4, n
+        within(t, ref[n], bound[n], n)
