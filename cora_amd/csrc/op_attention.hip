@@ -387,8 +387,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     l = 0.f;
 #pragma unroll
     for (int o = 0; o < NW; ++o) {
-      const float mo = ml[0][o][lane & 31];
-      if (mo != -INFINITY) l += ml[1][o][lane & 31] * __builtin_amdgcn_exp2f(mo - mt);
+      const float mo = ml[0][o][lane & 31];                 // -infinity: nothing seen (l = 0), or nothing but NaN (l = NaN)
+      l += ml[1][o][lane & 31] * (mo == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mo - mt));
     }
     const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
 #pragma unroll

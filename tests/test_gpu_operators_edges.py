@@ -101,3 +101,16 @@ def test_attention_fp16_gradients_of_large_values(lens, block):
     for n, t in zip(("dq", "dk", "dv"), ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)):
         assert ref[n].abs().max() < 6e4, n
         within(t, ref[n], bound[n], n)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,heads", [(33, 1), (97, 2), (1025, 1), (600, 64)])
+def test_attention_lse_of_rows_that_see_nan(n, heads, dtype):
+    """The last key alone in its tile is NaN: so are the results and the softmax' denominators of all rows, and every gradient of a
+    key that they see."""
+    cu, qkv, dout = packed([n], 0, heads, heads, 32, dtype)
+    q, k, v = (t.contiguous() for t in split(qkv.cuda(), heads, heads))
+    k[-1] = float("nan")
+    out, lse = ca.attention(q, k, v)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    assert all(torch.isnan(t).all() for t in ca.attention_backward(dout.cuda(), q, k, v, out, lse))
