@@ -238,6 +238,8 @@ template <int READS, int PER, int N, int GROUP, int M = 1> __device__ __forceinl
 // row, therefore enters its product times mul = 2^-e, and so do the sums acc.  Every lane has an e of its own: small values of a
 // row keep their bits whatever the other rows hold.  Kept while the column's largest value comes out in 2^-8 .. 2^15 (what fp16 then
 // rounds by 2^-25 is 2^-17 of it), else set so that it is in 2^4 .. 2^5: e is hardly ever changed, and costs a search of the tile.
+// The probabilities of dk/dv, 1 / n where all keys are alike, enter times 2^14: fp16 then holds them with 11 bits down to 2^-28.
+constexpr int P_EXP = 14;
 constexpr int LEAST_EXP = -30;     // ds below 2^-38 gives nothing in fp16 results; the sums times 2^30 stay finite
 template <int N> __device__ __forceinline__ void fit_half(f32x16& ds, f32x16 (&acc)[N], int& e, float& mul) {
   float big = 0.f;
@@ -452,7 +454,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   // Where a wave sees one key tile only, delta is taken from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
   // 16 bits, which delta otherwise inherits, counts most in rows that see few keys.
   const bool whole = sizeof(T) == 2 && wave_end <= KT;
-  if (own && h == 0 && (!SPLIT || w == 0)) { if (!whole) p.delta[at] = -delta; p.delta[plane + at] = -lse2; }
+  if (own && h == 0 && (!SPLIT || w == 0)) { if (!whole) p.delta[at] = -delta; p.delta[plane + at] = (F16 ? P_EXP : 0) - lse2; }
 
   f32x16 acc[D / 32];
 #pragma unroll
@@ -555,7 +557,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
   __shared__ __attribute__((aligned(16))) T ds0[QT * D];
   __shared__ __attribute__((aligned(16))) T qs1[QT * D];
   __shared__ __attribute__((aligned(16))) T ds1[QT * D];
-  __shared__ __attribute__((aligned(16))) float cs0[2][64];   // per staged query: -delta, -lse (log2)
+  __shared__ __attribute__((aligned(16))) float cs0[2][64];   // per staged query: -delta, -lse (log2; fp16: 14 more)
   __shared__ __attribute__((aligned(16))) float cs1[2][64];
   long long b; int n, tile;
   // here already with more than one workgroup a compute unit, which two then share: 16 x 1024 as above 178 / 141 us the whole pass
@@ -660,16 +662,16 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
 #undef FETCH
 #undef WORK
   if (own) {
-    const float f = F16 ? __builtin_amdgcn_ldexpf(p.scale, ex) : p.scale;
+    const float f = F16 ? __builtin_amdgcn_ldexpf(p.scale, ex - P_EXP) : p.scale, fv = F16 ? __builtin_amdgcn_ldexpf(1.f, -P_EXP) : 1.f;
     if (p.parts > 1) {
       const long long half = p.rows * p.kv_heads * p.d;
       float* dst = p.partial + 2 * half * blockIdx.y + ((b + ki) * p.kv_heads + kv) * p.d;
       store_own<float, D>(dst, ak, f, p.d, h);
-      store_own<float, D>(dst + half, av, 1.f, p.d, h);
+      store_own<float, D>(dst + half, av, fv, p.d, h);
       return;
     }
     store_own<T, D>((T*)p.dk + (b + ki) * p.dkr + (long long)kv * p.dkh, ak, f, p.d, h);
-    store_own<T, D>((T*)p.dv + (b + ki) * p.dvr + (long long)kv * p.dvh, av, 1.f, p.d, h);
+    store_own<T, D>((T*)p.dv + (b + ki) * p.dvr + (long long)kv * p.dvh, av, fv, p.d, h);
   }
 }
 

@@ -25,7 +25,7 @@ struct AttnP {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
   float* lse;                   // [heads, rows]
-  float* delta;                 // backward workspace [2, heads, rows]: -rowsum(dout out), -lse (log2)
+  float* delta;                 // backward workspace [2, heads, rows]: -rowsum(dout out), -lse (log2; fp16: 14 more)
   float* partial;               // [parts, 2, rows, kv_heads, d]: dk and dv of each part, if parts > 1
   int parts;                    // ranges the queries of a key tile are cut into (attention_parts)
   const int* cu;                // [nseq + 1] first rows, or null: nseq sequences of seqlen rows each

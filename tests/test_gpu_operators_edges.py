@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import cora_amd as ca
-from tests.operator_bounds import attention_ref
+from tests.operator_bounds import attention_ref, half_eps
 from tests.test_gpu_operators import BF16, F16, F32, packed, randn, split, within
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +114,18 @@ def test_attention_lse_of_rows_that_see_nan(n, heads, dtype):
     out, lse = ca.attention(q, k, v)
     assert torch.isnan(out).all() and torch.isnan(lse).all()
     assert all(torch.isnan(t).all() for t in ca.attention_backward(dout.cuda(), q, k, v, out, lse))
+
+
+@pytest.mark.parametrize("n,block", [(98304, 0), (3000, 0), (98304, 49152)])
+def test_attention_fp16_dv_of_long_sequences(n, block):
+    """Queries of zero see all keys alike: p = 1 / n, which fp16 holds with 8 bits only at this length.  64 rows of dout are 1:
+    dv = 64 p for every key (a key of the second block: from the rows of that block).  p and dv are rounded once each (2^-11), the sum's
+    64 terms in fp32 (64 2^-24), exp2 of the logarithm of n is off by less than 1e-5."""
+    d = 16
+    q = torch.zeros(n, 1, d, dtype=F16, device="cuda")
+    k, v = (randn(n, 1, d, dtype=F16, seed=i).cuda() for i in (1, 2))
+    dout = torch.zeros_like(q)
+    dout[-64:] = 1
+    out, lse = ca.attention(q, k, v, causal_block=block)
+    dv = ca.attention_backward(dout, q, k, v, out, lse, causal_block=block)[2].double().cpu()
+    assert ((dv - 64 / n).abs() <= 64 / n * (2 * half_eps(F16) + 64 * 2.0 ** -24 + 1e-5)).all(), float((dv * n / 64 - 1).abs().max())
