@@ -158,6 +158,7 @@ __device__ __forceinline__ int limit(int i, int n, int block) {
     if (it_ + 1 < (COUNT)) WORK(it_ + 1, 1);                                       \
   }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // What a mask hides must not count, even if it is not finite: hidden scores are replaced, but in the product behind them 0 times
 // infinity would.  A tile of which some rows of the workgroup do not see all is therefore searched first (each lane its own
 // 16-byte pieces, as it requested them): elements that are not finite become zeros, and mark(piece) makes the score
@@ -167,25 +168,24 @@ template <typename T, int D, int R, int NW, typename M> __device__ __forceinline
 #pragma unroll 1
   for (int i = 0; i < R * D / Op<T>::E / 64 / NW; ++i) {
     const int id = (i * NW + w) * 64 + lane;
-    uint4& at = reinterpret_cast<uint4*>(t)[id];
-    uint4 v = at;
-    unsigned* u = &v.x;
+    u32x4& at = reinterpret_cast<u32x4*>(t)[id];          // a vector type, which may alias the elements that others read
+    u32x4 v = at;
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       unsigned keep = ~0u;
-      if ((u[e] & INF) == INF) keep = sizeof(T) == 4 ? 0u : 0xffff0000u;
-      if (sizeof(T) == 2 && (u[e] >> 16 & INF) == INF) keep &= 0xffffu;
+      if ((v[e] & INF) == INF) keep = sizeof(T) == 4 ? 0u : 0xffff0000u;
+      if (sizeof(T) == 2 && (v[e] >> 16 & INF) == INF) keep &= 0xffffu;
       bad |= keep != ~0u;
-      u[e] &= keep;
+      v[e] &= keep;
     }
     if (bad) { at = v; mark(id); }
   }
 }
-// the waves' LDS writes are done; requests under way stay under way
-__device__ __forceinline__ void lds_barrier() {
+// the waves' LDS writes are done; requests under way stay under way.  WAVE: only the wave's own, whose buffer no other wave reads
+template <bool WAVE = false> __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+  if (!WAVE) __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     k += mine; v += mine;
     if (j0 + KT > all_min && j0 < end && p.block) {
       quarantine<T, D, KT, W::FW>(v, fw, lane, [&](int id) { k[id * Op<T>::E] = (T)NAN; });
-      if (!SPLIT) lds_barrier();
+      lds_barrier<SPLIT>();
     }
     if (j0 >= wave_end) return;
     f32x16 s[KT / 32];
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
     k += mine; v += mine;
     if (j0 + KT > all_min && j0 < end && p.block) {
       quarantine<T, D, KT, W::FW>(k, fw, lane, [&](int id) { v[id * Op<T>::E] = (T)NAN; });
-      if (!SPLIT) lds_barrier();
+      lds_barrier<SPLIT>();
     }
     if (j0 >= wave_end) return;
     if (whole) {
