@@ -109,6 +109,7 @@ struct cora_ctx {
   float *W = nullptr, *dW = nullptr, *amu = nullptr, *anu = nullptr;
   bool dW_owned = true;
   int64_t adam_count = 0;
+  bool stepped = false;      // the moments hold steps of the current recipe (not zeros, nor a state that was set)
   size_t oLn1g, oLn1b, oLn2g, oLn2b, oWqkv, oWo, oW1, ob1, oW2, ob2, oWp, obp, oWout, obout;
   // use_vode_state_layernorm: gamma / beta of the L+1 vode LayerNorms ([L+1, D] each), the normalised
   // vodes x' the blocks read, their row statistics, and the cotangents dE/dx' of vodes 1..L+1
@@ -274,6 +275,7 @@ int settle_pending(cora_ctx* c) {
 float* vode_ptr(cora_ctx* c, float* base, int l) { return l == 0 ? base : base + c->n0 + (long long)(l - 1) * c->nl; }
 float* err_ptr(cora_ctx* c, int l) { return c->Es + (long long)(l - 1) * c->nl; }  // l = 1..L+1 ; L+2 = e_img
 
+void count_step(cora_ctx* c) { c->adam_count += 1; c->stepped = true; }
 void drop_learn_graphs(cora_ctx* c) {
   if (c->learn_graph || c->wgrad_graph || c->apply_graph || c->dist_learn_graph) hipStreamSynchronize(c->st);
   if (c->dist_learn_graph) { hipGraphExecDestroy(c->dist_learn_graph); c->dist_learn_graph = nullptr; }
@@ -1364,6 +1366,7 @@ int cora_set_adam_state(cora_ctx* c, const float* mu, const float* nu, int64_t c
   rc = copy_in(c, c->anu, nu, c->nW, c->nW);
   if (rc) return rc;
   c->adam_count = count;
+  c->stepped = false;
   return 0;
 }
 int cora_get_adam_state(cora_ctx* c, float* mu, float* nu, int64_t* count) {
@@ -1421,6 +1424,13 @@ int cora_set_muon(cora_ctx* c, int enabled, float beta, int nesterov, float wd, 
     if (int rc = dalloc(c, &w, (long long)(ortho_ws_bytes(p) / sizeof(float) + 64))) return rc;
     c->mws = w;
     HCHECK(hipStreamSynchronize(c->st));
+  }
+  // the moments of one recipe mean nothing to the other: AdamW would divide Muon's momentum by a second moment that never saw it
+  if (on != c->muon && c->stepped) {
+    launch_zero(c->amu, sizeof(float) * c->nW, c->st);
+    launch_zero(c->anu, sizeof(float) * c->nW, c->st);
+    HCHECK(hipStreamSynchronize(c->st));
+    c->adam_count = 0; c->stepped = false;
   }
   c->muon = on;
   if (on) {
@@ -1729,7 +1739,7 @@ int cora_apply_wgrad(cora_ctx* c, float eta_w, float scale_by, cora_step_out* ou
   HCHECK(hipEventRecord(c->ev0, c->st));
   if (graphed) HCHECK(hipGraphLaunch(c->apply_graph, c->st));
   else if ((rc = enqueue_apply(c, scale_by))) return rc;
-  c->adam_count += 1;
+  count_step(c);
   HCHECK(hipEventRecord(c->ev1, c->st));
   HCHECK(hipStreamSynchronize(c->st));
   c->learn_warm = true;
@@ -1816,7 +1826,7 @@ int cora_step(cora_ctx* c, const float* x, int x_on_device, int T, const float* 
   HCHECK(hipGraphLaunch(gi, c->st));
   HCHECK(hipEventRecord(c->ev1, c->st));
   HCHECK(hipGraphLaunch(c->learn_graph, c->st));
-  c->adam_count += 1;
+  count_step(c);
   HCHECK(hipEventRecord(c->ev2, c->st));
   // scalars back through pinned memory: [energy row of step T-1 (slots or plain)] [w-energy row] [mse sum]
   double* ho = c->host_out;
@@ -1951,7 +1961,7 @@ static int step_ipc_impl(cora_ctx* c, const float* x, int x_on_device, int T, co
     if (!rc) rc = enqueue_wgrad(c);                                            // :426-427
     if (!rc && dist) NCHECK(g_rccl.AllReduce(c->dW, c->dW, c->nW, ncclFloat, ncclSum, c->comm, c->st));
     if (!rc) rc = enqueue_adamw(c, scale_by, c->hyp_dev + 4 + 4 * t);          // :428
-    if (!rc) c->adam_count += 1;
+    if (!rc) count_step(c);
   }
   if (rc) return rc;
   HCHECK(hipEventRecord(c->ev1, c->st));
@@ -2144,7 +2154,7 @@ int cora_step_dist(cora_ctx* c, const float* x, int x_on_device, int T, const fl
     HCHECK(hipGraphLaunch(c->dist_learn_graph, c->st));
   }
   c->dist_last_mode = graphed ? 2 : 1;
-  c->adam_count += 1;
+  count_step(c);
   HCHECK(hipEventRecord(c->ev2, c->st));
   double* ho = c->host_out;
   const size_t nslot = (size_t)(L + 3) * 8;
@@ -2349,7 +2359,7 @@ static int unmask_impl(cora_ctx* c, const float* x_true, const float* x_init, co
     if (eta_w) {                                             // :967-979
       if ((rc = enqueue_wgrad(c))) break;
       if ((rc = enqueue_adamw(c, scale_by, c->hyp_dev + 4 + 4 * t))) break;
-      c->adam_count += 1;
+      count_step(c);
     }
     if (use_corruption) launch_sens_clamp(c->xp, c->xt, c->mk, alpha, c->n0, c->st);   // :982-994
   }

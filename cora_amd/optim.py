@@ -47,7 +47,8 @@ class muon:
     """Weight steps by orthogonalised momentum for the blocks' matrices (query, key, value and output projections, both MLP
     matrices); every other parameter takes the AdamW step of the adam_* values with the same learning rate.
     m <- beta m + g;  u = g + beta m (nesterov) or m;  O = Newton-Schulz(u), ns_steps products with ns_coeffs, (a, b, c) or a
-    triple for every step (`cora_amd.orthogonalize`);  W <- W - lr (sqrt(max(1, rows / cols)) O + weight_decay W)."""
+    triple for every step (`cora_amd.orthogonalize`);  W <- W - lr (sqrt(max(1, rows / cols)) O + weight_decay W).
+    A model that changes between this recipe and `adamw` starts with zero moments of every parameter, as with a new `Optim`."""
     learning_rate: Schedule
     beta: float = 0.95
     nesterov: bool = True

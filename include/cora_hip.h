@@ -130,7 +130,8 @@ int cora_set_optim(cora_ctx* ctx, float clip_h, float momentum, float clip_w, fl
  * projections and the two MLP matrices.  With g the scaled, clipped gradient: m <- beta m + g, u = g + beta m (nesterov) or m,
  * O = Newton-Schulz(u) as cora_orthogonalize (steps, coef [steps, 3], eps), W <- W - eta_w (sqrt(max(1, rows / cols)) O + wd W).
  * Every other parameter keeps the AdamW step of cora_set_optim with the same eta_w.  m lives in the first AdamW moment.
- * enabled 0 goes back to AdamW for all.  The reference has AdamW only (examples/debug_transformer_wandb.py:1154-1159). */
+ * enabled 0 goes back to AdamW for all.  A change between the two starts the optimiser afresh -- both moments of every parameter and
+ * the count are zeroed -- unless no step was taken since cora_set_adam_state: that state is the next step's.  The reference has AdamW only (examples/debug_transformer_wandb.py:1154-1159). */
 int cora_set_muon(cora_ctx* ctx, int enabled, float beta, int nesterov, float wd, int steps, const float* coef, float eps);
 
 /* --- the step ------------------------------------------------------------------------------- */
