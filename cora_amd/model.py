@@ -241,6 +241,7 @@ class TransformerDecoder:
         if self._ctx is not None:
             _lib.load().cora_destroy(self._ctx)
             self._ctx = None
+            self._optim_sig = self._muon_sig = None      # what the next ctx was told: nothing yet
 
     def __del__(self):
         try:

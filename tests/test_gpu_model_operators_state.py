@@ -68,3 +68,22 @@ def test_a_state_that_was_set_is_kept_by_the_recipe_that_steps_next(monkeypatch)
     for k in want:
         assert np.array_equal(want[k], got[k]), k
     model.close()
+
+
+@pytest.mark.parametrize("name", ["images_rotary", "clips_causal"])
+def test_a_closed_model_steps_by_its_recipe_again(name, monkeypatch):
+    """close() drops the device state; the next batch sets the recipe up again -- Muon's numbers, the clips, AdamW's numbers -- and
+    steps as a new model does."""
+    import cora_amd as ca
+    for recipe in (ca.muon(0.02), ca.adamw(1e-3, weight_decay=0.5)):
+        ca, case, model, optim, oh = setup(name, monkeypatch, optim_w=recipe)
+        weights = model.get_weights()
+        want = step_of(ca, model, case, optim, oh)
+        model.close()
+        model.set_weights(weights)
+        for l, t in enumerate(case["h"]):
+            model.vodes[l].h.set(t)
+        got = step_of(ca, model, case, optim, oh)
+        for k in want:
+            assert np.array_equal(want[k], got[k]), k
+        model.close()
