@@ -5,8 +5,8 @@ They run the kernels a `TransformerDecoder` uses for `pos_encoding="rotary"`, `c
 optimiser, on the caller's own tensors.  The C entry points are `cora_rotary`, `cora_attention`, `cora_attention_backward`
 and `cora_orthogonalize` of include/cora_hip.h, which states the formulas.  Types: float32, bfloat16, float16.  Launches go
 to torch's current stream of the tensors' device and nothing is synchronised, so the calls can be captured into a graph.
-There is no autograd: gradients come from the `*_backward` calls, and tensors that require one are refused while torch
-records it.  The reference has none of these operators.
+There is no autograd: gradients come from the `*_backward` calls, and tensors that require one while torch records it, or that
+carry a forward-mode tangent, are refused.  The reference has none of these operators.
 
 Small calls last some 5 us on the GPU, so the checks below are kept to a few lookups per tensor."""
 from __future__ import annotations
@@ -19,14 +19,17 @@ from . import _lib
 _torch = None        # imported by the first call: the rest of the package works without torch
 _codes = {}
 _stream = None
+_duals = None
 
 
 def _load():
-    global _torch, _stream
+    global _torch, _stream, _duals
     import torch
+    from torch.autograd import forward_ad
     _codes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
     _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
         (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _duals = forward_ad
     _torch = torch
     return torch
 
@@ -49,6 +52,8 @@ def _no_grad(t, name: str) -> None:
     if t.requires_grad and _torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: these operators are not recorded by autograd; use the *_backward "
                          "calls under torch.no_grad(), or detach it")
+    if getattr(_duals, "_current_level", 0) >= 0 and _duals.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent: these operators have no forward-mode derivative; take its primal")
 
 
 def _like(t, name: str, lead, shape) -> None:
@@ -159,6 +164,7 @@ def _attention_inputs(q, k, v, cu_seqlens, seq_len, causal_block, scale):
 
 def _check_lse(lse, q) -> None:
     _table(lse, "lse", q, _torch.float32, 2, f"float32 tensor {(q.shape[1], q.shape[0])}")
+    _no_grad(lse, "lse")
     if lse.shape[0] != q.shape[1] or lse.shape[1] != q.shape[0]:
         raise ValueError(f"lse must be a contiguous float32 tensor {(q.shape[1], q.shape[0])}, got {tuple(lse.shape)}")
 

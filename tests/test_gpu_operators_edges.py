@@ -129,3 +129,22 @@ def test_attention_fp16_dv_of_long_sequences(n, block):
     out, lse = ca.attention(q, k, v, causal_block=block)
     dv = ca.attention_backward(dout, q, k, v, out, lse, causal_block=block)[2].double().cpu()
     assert ((dv - 64 / n).abs() <= 64 / n * (2 * half_eps(F16) + 64 * 2.0 ** -24 + 1e-5)).all(), float((dv * n / 64 - 1).abs().max())
+
+
+def test_tensors_with_a_tangent_or_a_gradient_are_refused():
+    from torch.autograd import forward_ad
+    x, pos = randn(8, 2, 32).cuda(), torch.zeros(8, 1, dtype=torch.int32, device="cuda")
+    out, lse = ca.attention(x, x, x)
+    calls = {"x": lambda t: ca.rotary(t, pos, [32]), "dout": lambda t: ca.rotary_backward(t, pos, [32]), "q": lambda t: ca.attention(t, x, x),
+             "k": lambda t: ca.attention(x, t, x), "v": lambda t: ca.attention(x, x, t),
+             "a gradient": lambda t: ca.attention_backward(t, x, x, x, out, lse), "m": lambda t: ca.orthogonalize([x[:, 0], t[:, 0]])}
+    with forward_ad.dual_level():
+        for name, call in calls.items():
+            with pytest.raises(ValueError, match="tangent"):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+            call(x)                                           # others are taken inside a level too
+            call(forward_ad.unpack_dual(forward_ad.make_dual(x, torch.ones_like(x))).primal)
+        with pytest.raises(ValueError, match="tangent"):
+            ca.attention_backward(x, x, x, x, out, forward_ad.make_dual(lse, torch.ones_like(lse)))
+    with pytest.raises(ValueError, match="requires a gradient"):
+        ca.attention_backward(x, x, x, x, out, lse.clone().requires_grad_())
