@@ -20,6 +20,7 @@ _torch = None        # imported by the first call: the rest of the package works
 _codes = {}
 _stream = None
 _duals = None
+_MOST = 2 ** 31 - 1  # of the C structures' 32-bit fields, which ctypes fills with a number's lower bits
 
 
 def _load():
@@ -96,6 +97,11 @@ def _rotary(x, positions, axes_dim, theta, interleaved, out, backward):
         raise ValueError(f"axes_dim must name 1 to 4 axes, got {n_axes}")
     _table(positions, "positions", x, _torch.int32, 2, f"int32 tensor [n, {n_axes}]")
     rows, heads, d = x.shape
+    if heads > _MOST or d > _MOST:
+        raise ValueError(f"x has shape {tuple(x.shape)}: heads and head_dim must be below 2^31")
+    for n in axes_dim:
+        if not -_MOST <= n <= _MOST:
+            raise ValueError(f"axes_dim must be positive, even and at most 128, got {tuple(axes_dim)}")
     n, width = positions.shape
     if width != n_axes:
         raise ValueError(f"positions must be a contiguous int32 tensor [n, {n_axes}], got {tuple(positions.shape)}")
@@ -157,6 +163,10 @@ def _attention_inputs(q, k, v, cu_seqlens, seq_len, causal_block, scale):
         if rows and (n < 1 or rows % n):
             raise ValueError(f"{rows} rows are not a multiple of seq_len {n}")
         n_seq = rows // n if rows else 0
+    if heads > _MOST or kv > _MOST or d > _MOST or n_seq > _MOST:
+        raise ValueError(f"heads {heads}, kv_heads {kv}, head_dim {d} and the number of sequences {n_seq} must be below 2^31")
+    if not -_MOST <= causal_block <= _MOST:
+        raise ValueError(f"causal_block must be 0 or positive and below 2^31, got {causal_block}")
     head = (code, heads, kv, d, n_seq, n, causal_block, d ** -0.5 if scale is None else scale, rows, table,
             q.data_ptr(), k.data_ptr(), v.data_ptr())
     return head, _heads(q, "q") + _heads(k, "k") + _heads(v, "v")
@@ -272,6 +282,8 @@ def orthogonalize(x, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), 
             _like(outs[i], "out", t, t.shape)
         if t.numel():
             count, rows, cols, xm, xr = _matrices(t, "x")
+            if max(count, rows, cols) > _MOST:
+                raise ValueError(f"x[{i}] has shape {tuple(t.shape)}: rows and columns must be at most 32768")
             ym, yr = _matrices(outs[i], "out")[3:]
             stacks.append((t.data_ptr(), outs[i].data_ptr(), xm, xr, ym, yr, count, rows, cols))
     if stacks:

@@ -148,3 +148,22 @@ def test_tensors_with_a_tangent_or_a_gradient_are_refused():
             ca.attention_backward(x, x, x, x, out, forward_ad.make_dual(lse, torch.ones_like(lse)))
     with pytest.raises(ValueError, match="requires a gradient"):
         ca.attention_backward(x, x, x, x, out, lse.clone().requires_grad_())
+
+
+def test_numbers_past_32_bits_are_refused():
+    """None of them may be taken for its lower 32 bits."""
+    x, pos = randn(8, 2, 32, dtype=BF16).cuda(), torch.zeros(8, 1, dtype=torch.int32, device="cuda")
+    for block in (2 ** 31, 2 ** 32, 2 ** 32 + 1, -2 ** 32 + 1):
+        with pytest.raises(ValueError, match="causal_block"):
+            ca.attention(x, x, x, causal_block=block)
+    for axis in (2 ** 32 + 32, -2 ** 32 + 32):
+        with pytest.raises(ValueError, match="axes_dim"):
+            ca.rotary(x, pos, [axis])
+    wide = x[:, :1].expand(8, 2 ** 32 + 2, 32)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ca.rotary(wide, pos, [32], out=wide)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ca.attention(wide, x, x, out=wide)
+    one = torch.zeros(1, device="cuda")
+    with pytest.raises(ValueError, match="32768"):
+        ca.orthogonalize(one.expand(2 ** 32 + 8, 1), out=one.expand(2 ** 32 + 8, 1))
