@@ -76,7 +76,7 @@ int check_attention(const cora_attention_args* a, AttnP* p, const char* who, boo
   if (!a->lse || (uintptr_t)a->lse % 4 || (a->cu_seqlens && (uintptr_t)a->cu_seqlens % 4))
     return refuse("%s: lse is NULL, or lse or cu_seqlens is not 4-byte aligned", who);
   // workgroups of up to 256 threads, fewer than 2^32 threads: one per 128 rows of a sequence and head (32 where there are few rows)
-  const long long tiles = a->cu_seqlens ? a->rows / 128 + a->n_seq : (long long)a->n_seq * ((a->seq_len + 127) / 128);
+  const long long tiles = a->cu_seqlens ? a->rows / 128 + a->n_seq : a->n_seq * (((long long)a->seq_len + 127) / 128);
   if ((tiles + 1024) * a->heads >= (1LL << 24)) return refuse("%s: too many tiles for one launch", who);
   if (backward) {
     if (!a->workspace || (uintptr_t)a->workspace % 16 || a->workspace_bytes < cora_attention_workspace(a))
