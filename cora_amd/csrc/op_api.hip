@@ -42,6 +42,48 @@ bool disjoint(long long rows, long long heads, long long d, long long sr, long l
   if (heads <= 1) return sr >= d;
   return (sh >= d && sr >= (heads - 1) * sh + d) || (sr >= d && sh >= (rows - 1) * sr + d);
 }
+// n0 x n1 pieces of w bytes, s0 and s1 bytes apart
+struct Span {
+  long long at, n0, s0, n1, s1, w;
+  long long end() const { return at + (n0 - 1) * s0 + (n1 - 1) * s1 + w; }
+  bool gapless() const {
+    const bool swap = n1 <= 1 || (n0 > 1 && s0 < s1);
+    const long long a = swap ? s0 : s1, na = swap ? n0 : n1, b = swap ? s1 : s0, nb = swap ? n1 : n0;
+    const long long inner = (na - 1) * a + w;
+    return (na <= 1 || a <= w) && (nb <= 1 || b <= inner);
+  }
+};
+Span bytes(const void* p, long long n) { return Span{(long long)(uintptr_t)p, 1, 0, 1, 0, n}; }
+// Do they share memory?  Decided where one of the two strides agrees, as views of one buffer do, and where neither has gaps; what
+// this leaves open (interleaved pieces of different strides) is the caller's to know.
+bool meet(Span a, Span b) {
+  if (a.at >= b.end() || b.at >= a.end()) return false;
+  if (a.gapless() && b.gapless()) return true;
+  auto same = [](long long na, long long sa, long long nb, long long sb) { return na <= 1 || nb <= 1 || sa == sb; };
+  const bool one = same(a.n0, a.s0, b.n0, b.s0), two = same(a.n1, a.s1, b.n1, b.s1);
+  if (!one && !two) return false;
+  if (!one || (two && a.n0 + b.n0 < a.n1 + b.n1))             // dimension 0 is solved for, dimension 1 tried out
+    for (Span* s : {&a, &b}) { const long long n = s->n0, st = s->s0; s->n0 = s->n1; s->s0 = s->s1; s->n1 = n; s->s1 = st; }
+  const long long r = a.n0 > 1 ? a.s0 : b.s0;
+  auto hit = [&](long long o) {                               // is there a d with -a.w < o + d r < b.w?
+    long long lo = -(b.n0 - 1), hi = a.n0 - 1;
+    if (r == 0) return -a.w < o && o < b.w;
+    auto floor_div = [](long long x, long long y) { return x / y - (x % y < 0); };
+    const long long first = floor_div(-a.w - o, r) + 1, last = -floor_div(o - b.w, r) - 1;
+    if (first > lo) lo = first;
+    if (last < hi) hi = last;
+    return lo <= hi;
+  };
+  if (same(a.n1, a.s1, b.n1, b.s1)) {
+    const long long st = a.n1 > 1 ? a.s1 : b.s1;
+    for (long long k = -(b.n1 - 1); k < a.n1; ++k)
+      if (hit(a.at - b.at + k * st)) return true;
+  } else if (a.n1 * b.n1 <= 4096)
+    for (long long i = 0; i < a.n1; ++i)
+      for (long long j = 0; j < b.n1; ++j)
+        if (hit(a.at + i * a.s1 - b.at - j * b.s1)) return true;
+  return false;
+}
 bool bad_dtype(int dtype) { return dtype < CORA_F32 || dtype > CORA_F16; }
 
 int check_attention(const cora_attention_args* a, AttnP* p, const char* who, bool backward) {
@@ -86,6 +128,22 @@ int check_attention(const cora_attention_args* a, AttnP* p, const char* who, boo
   for (const Ref& r : refs)
     for (const Ref& s : refs)
       if (r.out && &r != &s && (backward || !s.bwd) && r.ptr == s.ptr) return refuse("%s: %s is %s", who, r.name, s.name);
+  const long long eb = op_bytes(a->dtype);
+  auto span = [&](const Ref& r) { return Span{(long long)(uintptr_t)r.ptr, a->rows, r.row * eb, r.heads, r.head * eb, a->head_dim * eb}; };
+  struct Flat { const char* name; Span s; bool out; } flat[] = {
+    {"lse", bytes(a->lse, 4LL * a->heads * a->rows), !backward}, {"cu_seqlens", bytes(a->cu_seqlens, a->cu_seqlens ? 4LL * (a->n_seq + 1) : 0), false},
+    {"workspace", bytes(a->workspace, backward ? (long long)cora_attention_workspace(a) : 0), backward}};
+  for (const Ref& r : refs) {
+    if (r.bwd && !backward) continue;
+    if (r.out)
+      for (const Ref& s : refs)
+        if (&r != &s && (backward || !s.bwd) && meet(span(r), span(s))) return refuse("%s: %s overlaps %s", who, r.name, s.name);
+    for (const Flat& f : flat)
+      if (f.s.w && (r.out || f.out) && meet(span(r), f.s)) return refuse("%s: %s overlaps %s", who, r.name, f.name);
+  }
+  for (const Flat& f : flat)
+    for (const Flat& g : flat)
+      if (&f != &g && f.out && f.s.w && g.s.w && meet(f.s, g.s)) return refuse("%s: %s overlaps %s", who, f.name, g.name);
   memset(p, 0, sizeof *p);
   p->q = a->q; p->k = a->k; p->v = a->v; p->out = a->out; p->o = a->out; p->lse = a->lse;
   p->dout = a->dout; p->dq = a->dq; p->dk = a->dk; p->dv = a->dv; p->cu = a->cu_seqlens;
@@ -217,6 +275,9 @@ int cora_rotary(const cora_rotary_args* a, int device, void* hip_stream) {
   if (a->x == a->y && ((a->rows > 1 && a->x_row != a->y_row) || (a->heads > 1 && a->x_head != a->y_head)))
     return refuse("%s: in place, x and y need the same strides", who);
   if (a->rows > (1LL << 39) / a->head_dim) return refuse("%s: too many rows for one launch", who);
+  const Span y{(long long)(uintptr_t)a->y, a->rows, a->y_row * eb, a->heads, a->y_head * eb, (long long)a->head_dim * eb};
+  if (a->x != a->y && meet(y, Span{(long long)(uintptr_t)a->x, a->rows, a->x_row * eb, a->heads, a->x_head * eb, y.w})) return refuse("%s: y overlaps x", who);
+  if (meet(y, bytes(a->pos, a->pos_rows * a->n_axes * 4))) return refuse("%s: y overlaps pos", who);
   RotaryP p;
   memset(&p, 0, sizeof p);
   p.x = a->x; p.y = a->y; p.pos = a->pos; p.rows = a->rows; p.pos_rows = a->pos_rows;
@@ -291,9 +352,24 @@ int cora_orthogonalize(int dtype, const cora_matrices* stacks, int n_stacks, int
       if (i != j && stacks[i].count && stacks[j].count && (stacks[i].y == stacks[j].y || stacks[i].y == stacks[j].x))
         return refuse("%s: y of stack %d is x or y of stack %d", who, i, j);
   if (!any) return 0;
+  const long long eb = op_bytes(dtype);
+  auto x_of = [&](const cora_matrices& s) { return Span{(long long)(uintptr_t)s.x, s.count, s.x_mat * eb, s.rows, s.x_row * eb, s.cols * eb}; };
+  auto y_of = [&](const cora_matrices& s) { return Span{(long long)(uintptr_t)s.y, s.count, s.y_mat * eb, s.rows, s.y_row * eb, s.cols * eb}; };
+  for (int i = 0; i < n_stacks; ++i) {
+    if (!stacks[i].count) continue;
+    const Span y = y_of(stacks[i]);
+    for (int j = 0; j < n_stacks; ++j) {
+      if (!stacks[j].count) continue;
+      if ((i != j || stacks[i].x != stacks[i].y) && meet(y, x_of(stacks[j]))) return refuse("%s: y of stack %d overlaps x of stack %d", who, i, j);
+      if (i < j && meet(y, y_of(stacks[j]))) return refuse("%s: y of stack %d overlaps y of stack %d", who, i, j);
+    }
+  }
   const size_t need = cora_orthogonalize_workspace(dtype, stacks, n_stacks);
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < need)
     return refuse("%s: workspace is NULL, not 256-byte aligned or smaller than %zu bytes", who, need);
+  for (int i = 0; i < n_stacks; ++i)
+    if (stacks[i].count && (meet(bytes(workspace, (long long)need), x_of(stacks[i])) || meet(bytes(workspace, (long long)need), y_of(stacks[i]))))
+      return refuse("%s: the workspace overlaps stack %d", who, i);
   OnDevice dev(device);
   if (!dev.ok) return refuse("%s: device %d is not available", who, device);
   for (int i = 0; i < n_stacks;) {

@@ -262,6 +262,8 @@ int cora_forward_static(const cora_config* cfg, int device, const float* W_dev, 
  * allocation, no copy, no synchronisation, so they may be called under stream capture.  The caller's current device is
  * left as it was.  Thread-safe; errors: cora_last_error(NULL).  Strides count elements; the innermost dimension is
  * contiguous.  Inputs may have any strides >= 0 (0 repeats a row or head); rows and heads of an output must not overlap.
+ * An output that overlaps an input, another output or the workspace is refused where the two have a stride in common or no gaps, as
+ * views of one buffer do; other overlaps are the caller's to avoid.
  * No counterpart in the reference, whose blocks have additive positions and bidirectional attention
  * (pcx/nn/_layer.py:405-447) and whose weights are stepped by AdamW. */
 enum { CORA_F32 = 0, CORA_BF16 = 1, CORA_F16 = 2 };
