@@ -7,7 +7,7 @@ import torch
 
 import cora_amd as ca
 from tests.operator_bounds import attention_ref, half_eps
-from tests.test_gpu_operators import BF16, F16, F32, packed, randn, split, within
+from tests.test_gpu_operators import BF16, F16, F32, ortho_close, packed, randn, split, within
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +167,24 @@ def test_numbers_past_32_bits_are_refused():
     one = torch.zeros(1, device="cuda")
     with pytest.raises(ValueError, match="32768"):
         ca.orthogonalize(one.expand(2 ** 32 + 8, 1), out=one.expand(2 ** 32 + 8, 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("count,rows,cols", [
+    (6, 1030, 1300),        # P X on tiles of 256 (180 of them), the symmetric products on 128
+    (5, 1300, 1030),        # the same, tall: the result is written transposed
+    (11, 2309, 2051),       # the symmetric products on 256 too, tall, odd sizes
+    (40, 390, 1030),        # the symmetric products on 64, P X on 128
+    (40, 1031, 390),        # the same, tall
+])
+def test_orthogonalize_every_tile_size(count, rows, cols, dtype):
+    """Stacks that are large enough for the wide tiles; the first and the last matrix against 64 bits."""
+    G = torch.empty(count, rows, cols, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(rows + cols)
+    G.normal_(generator=gen)
+    G += torch.randn(count, rows, 4, device="cuda", generator=gen) @ torch.randn(count, 4, cols, device="cuda", generator=gen)
+    G = (1e-3 * G).to(dtype)
+    got = ca.orthogonalize(G, steps=3)
+    assert torch.isfinite(got).all()
+    for i in (0, count - 1):
+        ortho_close(got[i], G[i].cpu(), steps=3)
