@@ -121,8 +121,8 @@ __global__ __launch_bounds__(256) void ortho_load(const OrthoP p) {
 // transposing read 80 apart) or, where that does not fit, to 16 mod 256.
 constexpr int SMALL_LDS = 160 * 1024 - 256;
 struct SmallDim { int mp, np, sx, sa, bytes; };           // padded sizes, row strides in halves, LDS bytes
-__host__ __device__ inline SmallDim small_dim(int m, int n) {
-  SmallDim d;
+__host__ __device__ constexpr SmallDim small_dim(int m, int n) {
+  SmallDim d = {};
   d.mp = (m + 31) / 32 * 32; d.np = (n + 31) / 32 * 32;
   for (int want = 80; want >= 16; want -= 64) {
     d.sx = d.np + ((want - 2 * d.np) & 255) / 2; d.sa = d.mp + ((want - 2 * d.mp) & 255) / 2;
@@ -131,6 +131,7 @@ __host__ __device__ inline SmallDim small_dim(int m, int n) {
   }
   return d;
 }
+static_assert(small_dim(97, 128).bytes <= SMALL_LDS && small_dim(97, 129).bytes > SMALL_LDS, "4 row tiles: never more than 16 tiles of X");
 
 // the steps, for matrices of RT row tiles and X of at most 8 XT tiles
 template <int RT, int XT>
@@ -652,7 +653,7 @@ template <typename T, int RT, int XT> int run_small(const OrthoP& p, const Ortho
   return hipGetLastError() != hipSuccess;
 }
 
-// How a stack is worked on: in one workgroup with 1 to 4 row tiles of 32 (+ 8: more than 16 tiles of X), or with tiles:
+// How a stack is worked on: in one workgroup with 1 to 4 row tiles of 32 (+ 8, up to 3 of them: more than 16 tiles of X), or with tiles:
 // 64, or 256 for m >= 1024, and for bf16 results (+ 1) of m >= 256 with fewer instructions a product (below that it
 // costs precision and saves nothing)
 int class_of(const OrthoG& g, bool bf16) {
@@ -676,7 +677,7 @@ template <typename T> int run(const OrthoP& p, int steps, const float* coef, hip
   OrthoCoef co;
   co.steps = steps;
   for (int i = 0; i < 3 * steps; ++i) co.c[i] = coef[i];
-  for (int cls : {256 + BF16, 64 + 1, 64, 8 + 4, 8 + 3, 8 + 2, 8 + 1, 4, 3, 2, 1}) {
+  for (int cls : {256 + BF16, 64 + 1, 64, 8 + 3, 8 + 2, 8 + 1, 4, 3, 2, 1}) {
     const OrthoP q = only(p, BF16, cls);
     if (!q.ngroups) continue;
     // 256 tiles need half the compute units to have one: 5 steps of 2 x 2048 x 8192 fp32 in 5.0 ms with 64, 4.2 with 128, 4.0
@@ -685,7 +686,7 @@ template <typename T> int run(const OrthoP& p, int steps, const float* coef, hip
     for (int i = 0; i < q.ngroups; ++i) wide += (long long)q.g[i].count * ((q.g[i].m + 255) / 256) * ((q.g[i].n + 255) / 256);
     const int rc = cls >= 256 ? (wide >= 128 ? run_tiled<T, !BF16, 256>(q, steps, coef, st) : run_tiled<T, !BF16, 64>(q, steps, coef, st)) :
                    cls == 64 + 1 ? run_tiled<T, !BF16, 64>(q, steps, coef, st) : cls == 64 ? run_tiled<T, true, 64>(q, steps, coef, st) :
-                   cls == 12 ? run_small<T, 4, 5>(q, co, st) : cls == 11 ? run_small<T, 3, 5>(q, co, st) :
+                   cls == 11 ? run_small<T, 3, 5>(q, co, st) :
                    cls == 10 ? run_small<T, 2, 5>(q, co, st) : cls == 9 ? run_small<T, 1, 5>(q, co, st) :
                    cls == 4 ? run_small<T, 4, 2>(q, co, st) : cls == 3 ? run_small<T, 3, 2>(q, co, st) :
                    cls == 2 ? run_small<T, 2, 2>(q, co, st) : run_small<T, 1, 2>(q, co, st);
