@@ -207,9 +207,9 @@ int ortho_bad_step(int steps, const float* coef) {
   for (int i = 0; i <= 256; ++i) sv[i] = i / 256.f;
   for (int s = 0; s < steps; ++s)
     for (float& x : sv) {
-      const float l = x * x, f = coef[3 * s] + coef[3 * s + 1] * l + coef[3 * s + 2] * l * l;
+      const float l = x * x, g = coef[3 * s + 1] * l + coef[3 * s + 2] * l * l, f = coef[3 * s] + g;   // g: of b A + c A^2 alone
       x = fabsf(x * f);
-      if (!(fabsf(f) <= 1000.f) || !(x <= 8.f) || !(fabsf(coef[3 * s]) <= 1000.f)) return s;
+      if (!(fabsf(f) <= 1000.f) || !(fabsf(g) <= 1000.f) || !(x <= 8.f) || !(fabsf(coef[3 * s]) <= 1000.f)) return s;
     }
   return -1;
 }

@@ -320,7 +320,7 @@ size_t cora_attention_workspace(const cora_attention_args* a);
  * All stacks (each `count` equal matrices) are worked on together; a stack's y may be its x (same strides) and else must
  * not overlap any x or y.  Products are float32-grade
  * (bfloat16: of an error below the result's rounding).  Refused: coefficients under which a singular value of [0, 1]
- * leaves [0, 8] or |a + b s^2 + c s^4| exceeds 1000.
+ * leaves [0, 8] or |a + b s^2 + c s^4|, |b s^2 + c s^4| or |a| exceeds 1000.
  * workspace: cora_orthogonalize_workspace(..) bytes, 256-byte aligned, not shared by calls that may overlap. */
 typedef struct cora_matrices {
   const void* x; void* y;

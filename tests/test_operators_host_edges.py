@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 from cora_amd import _lib
-from tests.test_operators_host import FAKE, attn_args, coef, rotary_args
+from tests.test_operators_host import FAKE, attn_args, coef, rotary_args, stack
 
 
 def refused(call, word):
@@ -96,3 +96,10 @@ def test_orthogonalize_refuses_overlapping_outputs():
     if not torch.cuda.is_available():
         refused(call(two(dict(x=BASE, y=BASE + 512), far)), "not available")                                 # the other half of every row
         refused(call(two(dict(x=BASE, y=BASE), far)), "not available")
+
+
+def test_orthogonalize_refuses_coefficients_whose_products_leave_fp16():
+    """b A + c A^2 is kept apart from a I for bfloat16 results and may be larger than their sum: 2000 in the second step here, where
+    the planes, 64 times the value, hold 1023."""
+    s = stack()
+    refused(_lib.load().cora_orthogonalize(1, s, 1, 2, coef(0.001, 0.0, 0.0, 999.0, -1.99e9, 0.0), 1e-7, FAKE * 100, 1 << 40, 0, None), "out of range")
