@@ -84,7 +84,7 @@ def _heads(t, name: str):
     if heads == 1:
         head = d
     if rows == 1:
-        row = heads * head
+        row = d
     return row, head
 
 

@@ -188,3 +188,22 @@ def test_orthogonalize_every_tile_size(count, rows, cols, dtype):
     assert torch.isfinite(got).all()
     for i in (0, count - 1):
         ortho_close(got[i], G[i].cpu(), steps=3)
+
+
+def test_one_row_of_a_long_head_major_cache():
+    """A dimension of size one has no stride that counts, however far its heads lie apart."""
+    base = randn(16, 1, 128, dtype=BF16, seed=3)
+    cache = torch.zeros(16, 2 ** 13 + 8, 128, dtype=BF16, device="cuda")
+    cache[:, 5:6] = base.cuda()
+    row = cache[:, 5:6].transpose(0, 1)                      # [1, 16, 128], heads 2^20 elements and more apart
+    q = randn(1, 16, 128, dtype=BF16, seed=4)
+    out, lse = ca.attention(q.cuda(), row, row)
+    assert torch.equal(out, row) and out.shape == q.shape    # one key: its value
+    ref, bound = attention_ref(q, base.transpose(0, 1), base.transpose(0, 1), [0, 1], 0, 128 ** -0.5, q)
+    within(lse, ref["lse"], bound["lse"], "lse")
+    for n, t in zip(("dq", "dk", "dv"), ca.attention_backward(q.cuda(), q.cuda(), row, row, out, lse)):
+        within(t, ref[n], bound[n], n)
+    turned = ca.rotary(row, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), [128], out=row)
+    assert torch.equal(turned, row)
+    same = q.cuda()[:, :1].expand(1, 16, 128)                # one row of one head, repeated
+    assert torch.equal(ca.attention(same, row, row)[0], row)
