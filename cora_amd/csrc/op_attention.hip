@@ -451,9 +451,9 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
   [[maybe_unused]] int ex = 0;                              // F16: acc and ds are scaled by mul = 2^-ex
   [[maybe_unused]] float mul = 1.f;
   const float lse2 = own ? p.lse[at] * CORA_LOG2E : 0.f, sl2 = p.scale * CORA_LOG2E;
-  // Where a wave sees one key tile only, delta is taken from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
+  // A row that sees the first key tile only takes delta from the tile itself, sum_j p_ij (do_i v_j): the rounding of out to
   // 16 bits, which delta otherwise inherits, counts most in rows that see few keys.
-  const bool whole = sizeof(T) == 2 && wave_end <= KT;
+  const bool whole = sizeof(T) == 2 && lim <= KT;
   if (own && h == 0 && (!SPLIT || w == 0)) { if (!whole) p.delta[at] = -delta; p.delta[plane + at] = (F16 ? P_EXP : 0) - lse2; }
 
   f32x16 acc[D / 32];
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
       lds_barrier<SPLIT>();
     }
     if (j0 >= wave_end) return;
-    if (whole) {
+    if (sizeof(T) == 2 && j0 == 0 && wave_min <= KT) {
       float sum = 0.f;
 #pragma unroll 1
       for (int t = 0; t < KT / 32; ++t) {
@@ -491,8 +491,11 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
         for (int r = 0; r < 16; ++r)
           if (32 * t + acc_row(r, h) < lim) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)), dp[r], sum);
       }
-      delta = half_sum(sum);
-      if (own && h == 0) p.delta[at] = -delta;
+      sum = half_sum(sum);
+      if (whole) {
+        delta = sum;
+        if (own && h == 0) p.delta[at] = -delta;
+      }
     }
 #pragma unroll
     for (int t = 0; t < KT / 32; ++t) {

@@ -207,3 +207,24 @@ def test_one_row_of_a_long_head_major_cache():
     assert torch.equal(turned, row)
     same = q.cuda()[:, :1].expand(1, 16, 128)                # one row of one head, repeated
     assert torch.equal(ca.attention(same, row, row)[0], row)
+
+
+def rounding_ratio(got, exact):
+    """error of a 16-bit result in units of what rounding the exact one would give"""
+    exact = exact.double()
+    rel = lambda t: float((t.double().cpu() - exact).norm() / exact.norm())
+    return rel(got) / rel(exact.to(got.dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,heads,d,block", [(155, 8, 80, 5), (155, 16, 32, 3), (300, 16, 64, 7)])
+def test_attention_dq_of_rows_that_see_few_keys(n, heads, d, block, dtype):
+    """The rounding of ds and of dq are each as large as the result's own: 1.41 of it together.  The rounding of out, through delta,
+    would make it 1.6 and more in rows of 25 keys and less, so it must stay out of these.  1.52 leaves 7 % to the sample's spread
+    (7000 elements and more; five seeds of the exact arithmetic gave 1.37 .. 1.50 with delta exact, 1.54 .. 1.82 without)."""
+    cu, qkv, dout = packed([n], 0, heads, heads, d, dtype, seed=3)
+    ref, _ = attention_ref(*split(qkv, heads, heads), cu, block, d ** -0.5, dout)
+    q, k, v = split(qkv.cuda(), heads, heads)
+    out, lse = ca.attention(q, k, v, causal_block=block)
+    dq = ca.attention_backward(dout.cuda(), q, k, v, out, lse, causal_block=block)[0]
+    assert rounding_ratio(dq[:25], ref["dq"][:25]) <= 1.52
