@@ -411,7 +411,8 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // q k and do v are computed here and in the dk/dv kernel: seven products instead of five, but no atomics and no ds in memory.
 // The row constants are -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves
 // nothing and triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
-template <typename T, int D, int DK, int NW, bool SPLIT>
+// FINE: ds enters its product in two pieces of the 16-bit type, so that its rounding does not count (the rule is at bwd).
+template <typename T, int D, int DK, int NW, bool SPLIT, bool FINE>
 __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
@@ -518,8 +519,14 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
         const frag pf = O::pack(s, c);
+        [[maybe_unused]] frag rf;
+        if constexpr (FINE) rf = O::rest(s, c, pf);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] = O::mma(L::col_frag(k, t * (32 / O::CH) + c, i, lane), pf, acc[i]);
+        for (int i = 0; i < D / 32; ++i) {
+          const frag kf = L::col_frag(k, t * (32 / O::CH) + c, i, lane);
+          acc[i] = O::mma(kf, pf, acc[i]);
+          if constexpr (FINE) acc[i] = O::mma(kf, rf, acc[i]);
+        }
       }
     }
   };
@@ -551,7 +558,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // vector work (exp, masks, packing) is not hidden behind another wave's matrix instructions: 2.7 ms, 810 TFLOP/s at the size above.
 // Staged rows behind the sequence are zeros, or pieces of its last rows where rows repeat or overlap (a stride below the
 // row's length); their -lse is set to -infinity, so their p and ds are zero whatever is there.
-template <typename T, int D, int DK, int NW>
+template <typename T, int D, int DK, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1 : 2) void attn_bwd_kv(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
@@ -650,13 +657,17 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
         const frag pf = O::pack(s, c), gf = O::pack(dp, c);
+        [[maybe_unused]] frag pr, gr;
+        if constexpr (FINE) { pr = O::rest(s, c, pf); gr = O::rest(dp, c, gf); }
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-          av[i] = O::mma(L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), pf, av[i]);
-          ak[i] = O::mma(L::col_frag(qt, t * (32 / O::CH) + c, i, lane), gf, ak[i]);
+          const frag df = L::col_frag(dt_, t * (32 / O::CH) + c, i, lane), qf = L::col_frag(qt, t * (32 / O::CH) + c, i, lane);
+          av[i] = O::mma(df, pf, av[i]);
+          ak[i] = O::mma(qf, gf, ak[i]);
+          if constexpr (FINE) { av[i] = O::mma(df, pr, av[i]); ak[i] = O::mma(qf, gr, ak[i]); }
         }
       }
-      if (sizeof(T) == 2) feed<8, 2, D / 8, 1>();
+      if (sizeof(T) == 2 && !FINE) feed<8, 2, D / 8, 1>();
     }
   };
 #define FETCH(it, buf) fetch(it, buf ? qs1 : qs0, buf ? ds1 : ds0, buf ? cs1 : cs0)
@@ -703,11 +714,27 @@ template <typename T, int D, int DK, int NW, bool SPLIT> int fwd(const AttnP& p,
   attn_fwd<T, D, DK, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
 }
+// FINE: the rounding of ds and p to 16 bits is as large as the results' own; both together are 1.41 times that, 1.48 with the
+// rounding of out in delta.  Small calls (all gradients), where few terms make up a result, and narrow heads (dq), where delta counts
+// more, come to 1.5 .. 1.8 times; there ds and p enter the products in two pieces.  dq, dk, dv against 64 bits, in errors of the
+// plain form, one piece / two, bf16: 46 tokens, 2 heads of 16, causal, 1.67 1.48 1.29 / 1.03 1.02 1.00; 2258 + 257 tokens, 4 heads of 16, dq
+// 1.53 / 1.08; 600 random calls with this rule: 1.48 at most.  Backward pass, us: 10 x 100 tokens, 4 heads of 16, 10.6 / 11.6; 8 x 512, 8
+// heads of 24 (dq alone), causal, 28.6 / 31.2.  For heads of 32 too dq would take 426 for 352 (8 x 2048 tokens, 16 heads, fp16).
+template <typename T, int D, int DK, int NW, bool SPLIT, bool FINE> int bwd_q(const AttnP& p, hipStream_t st) {
+  attn_bwd_q<T, D, DK, NW, SPLIT, FINE><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
+  return hipGetLastError() != hipSuccess;
+}
+template <typename T, int D, int DK, bool FINE> int bwd_kv(const AttnP& p, hipStream_t st) {
+  attn_bwd_kv<T, D, DK, 4, FINE><<<dim3((unsigned)(slots(p, 128) * p.kv_heads), (unsigned)p.parts), 256, 0, st>>>(p);
+  return hipGetLastError() != hipSuccess;
+}
 template <typename T, int D, int DK, int NW, bool SPLIT> int bwd(const AttnP& p, hipStream_t st) {
-  attn_bwd_q<T, D, DK, NW, SPLIT><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
-  if (hipGetLastError() != hipSuccess) return 1;
-  attn_bwd_kv<T, D, DK, 4><<<dim3((unsigned)(slots(p, 128) * p.kv_heads), (unsigned)p.parts), 256, 0, st>>>(p);
-  if (hipGetLastError() != hipSuccess) return 1;
+  constexpr bool HALF = sizeof(T) == 2;
+  const bool small = HALF && p.rows * p.heads <= 4096;
+  if constexpr (HALF && (SPLIT || D == 32)) {                // small calls are split
+    if (small || p.d <= 24 ? bwd_q<T, D, DK, NW, SPLIT, true>(p, st) : bwd_q<T, D, DK, NW, SPLIT, false>(p, st)) return 1;
+  } else if (bwd_q<T, D, DK, NW, SPLIT, false>(p, st)) return 1;
+  if (small ? bwd_kv<T, D, DK, HALF>(p, st) : bwd_kv<T, D, DK, false>(p, st)) return 1;
   if (p.parts == 1) return 0;
   attn_bwd_sum<T><<<dim3((unsigned)((p.rows * p.kv_heads * p.d / 4 + 255) / 256), 2), 256, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;

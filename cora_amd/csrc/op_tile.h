@@ -46,6 +46,13 @@ template <> struct Op<__bf16> {
     for (int t = 0; t < 8; ++t) f[t] = (__bf16)c[8 * s + t];
     return f;
   }
+  // what pack left of the values, in the same type
+  static __device__ __forceinline__ frag rest(const f32x16& c, int s, const frag& p) {
+    frag f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) f[t] = (__bf16)(c[8 * s + t] - (float)p[t]);
+    return f;
+  }
 };
 template <> struct Op<_Float16> {
   typedef h16x8 frag;
@@ -57,6 +64,12 @@ template <> struct Op<_Float16> {
     frag f;
 #pragma unroll
     for (int t = 0; t < 8; ++t) f[t] = (_Float16)c[8 * s + t];
+    return f;
+  }
+  static __device__ __forceinline__ frag rest(const f32x16& c, int s, const frag& p) {
+    frag f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) f[t] = (_Float16)(c[8 * s + t] - (float)p[t]);
     return f;
   }
 };

@@ -228,3 +228,29 @@ def test_attention_dq_of_rows_that_see_few_keys(n, heads, d, block, dtype):
     out, lse = ca.attention(q, k, v, causal_block=block)
     dq = ca.attention_backward(dout.cuda(), q, k, v, out, lse, causal_block=block)[0]
     assert rounding_ratio(dq[:25], ref["dq"][:25]) <= 1.52
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens,heads,kv,d,block", [([46], 2, 2, 16, 1), ([2, 3, 0, 2, 2, 3, 4], 3, 3, 48, 196), ([5, 17], 2, 2, 64, 64), ([7] * 9, 8, 2, 128, 0),
+                                                   ([338], 8, 8, 16, 5), ([100] * 10, 4, 4, 16, 0), ([300, 96], 4, 4, 80, 1)])
+def test_attention_gradients_of_small_calls(lens, heads, kv, d, block, dtype):
+    """ds and p enter in two pieces, 2^-17 off and less, which leaves the results' own rounding (1) and that of out through delta (up to
+    half as much, 1.12 together).  In one piece each would add 1 more: 1.41 .. 1.8.  Up to 4096 rows and heads."""
+    cu, qkv, dout = packed(lens, 0, heads, kv, d, dtype, seed=11)
+    ref, _ = attention_ref(*split(qkv, heads, kv), cu, block, d ** -0.5, dout)
+    q, k, v = split(qkv.cuda(), heads, kv)
+    kw = dict(cu_seqlens=table(cu), causal_block=block)
+    out, lse = ca.attention(q, k, v, **kw)
+    for n, t in zip(("dq", "dk", "dv"), ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)):
+        assert rounding_ratio(t, ref[n]) <= 1.25, n
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens,heads,d,block", [([2258, 257], 4, 16, 196), ([512] * 8, 8, 24, 1)])
+def test_attention_dq_of_narrow_heads(lens, heads, d, block, dtype):
+    cu, qkv, dout = packed(lens, 0, heads, heads, d, dtype, seed=12)
+    ref, _ = attention_ref(*split(qkv, heads, heads), cu, block, d ** -0.5, dout)
+    q, k, v = split(qkv.cuda(), heads, heads)
+    kw = dict(cu_seqlens=table(cu), causal_block=block)
+    out, lse = ca.attention(q, k, v, **kw)
+    assert rounding_ratio(ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)[0], ref["dq"]) <= 1.25
