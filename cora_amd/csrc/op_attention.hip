@@ -234,6 +234,21 @@ template <int READS, int PER, int N, int GROUP, int M = 1> __device__ __forceinl
   for (int c = 0; c < N; ++c) { __builtin_amdgcn_sched_group_barrier(0x8, M, GROUP); __builtin_amdgcn_sched_group_barrier(0x100, PER, GROUP); }
 }
 
+// acc += (tile of rows)^T w with a sum of its own for the 32 rows.  For fp32: added one after the other, two products an instruction, the
+// terms of a long walk leave thousands of roundings in one growing sum.  Taken by dk and dv, and by out and dq of heads up to 64
+// (wider heads have as large errors in their scores).  Against 64 bits, one sum / sums apart: 8 x 2048 tokens, 8 of 2 heads of 64,
+// causal, dk 1.1e-6 / 4.8e-7, dq 5.7e-7 / 4.5e-7, out 4.0e-7 / 2.6e-7.  Time, us: forward 310 / 311, backward 1190 / 1155 (fewer registers
+// are held); 64 x 196 tokens, 8 heads of 48, 73 / 75 and 246 / 244; backward of heads of 80 and 128 3 and 2 % longer.
+template <typename T, int D> __device__ __forceinline__ void sum_apart(const T* tile, const f32x16& w, int t, int i, int lane, f32x16& acc) {
+  f32x16 part;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) part[r] = 0.f;
+#pragma unroll
+  for (int c = 0; c < 32 / Op<T>::CH; ++c) part = Op<T>::mma(Tile<T, D>::col_frag(tile, t * (32 / Op<T>::CH) + c, i, lane), Op<T>::pack(w, c), part);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] += part[r];
+}
+
 // fp16 holds 2^-24 .. 2^16, and ds ~ p do / sqrt(n) of an unscaled loss lies below.  A tile of ds, whose column is the lane's own
 // row, therefore enters its product times mul = 2^-e, and so do the sums acc.  Every lane has an e of its own: small values of a
 // row keep their bits whatever the other rows hold.  Kept while the column's largest value comes out in 2^-8 .. 2^15 (what fp16 then
@@ -275,7 +290,7 @@ template <int N> __device__ __forceinline__ void fit_half(f32x16& ds, f32x16 (&a
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
 // Each row goes by its own scores, so its result does not depend on which other rows share its tile.
 template <typename T, int D, int DK, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_fwd(const AttnP p) {
+__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : DK == 48 ? 3 : 2) void attn_fwd(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   typedef Walk<T, D, NW, SPLIT> W;
   constexpr int KT = W::KT, QT = W::QT, NC = DK / O::CH, NS = KT / O::CH;
@@ -366,6 +381,10 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
         sum += s[t][r];
       }
     l += sum;
+    if constexpr (sizeof(T) == 4 && D <= 64) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) sum_apart<T, D>(v, s[0], 0, i, lane, acc[i]);
+    } else
 #pragma unroll
     for (int c = 0; c < NS; ++c) {
       const frag pf = O::pack(s[c * O::CH / 32], c % (32 / O::CH));
@@ -516,6 +535,10 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
           if (j0 + 32 * t + acc_row(r, h) >= lim) s[r] = 0.f;
       }
       if constexpr (F16) fit_half(s, acc, ex, mul);
+      if constexpr (sizeof(T) == 4 && D <= 64) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) sum_apart<T, D>(k, s, t, i, lane, acc[i]);
+      } else
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
         const frag pf = O::pack(s, c);
@@ -654,6 +677,13 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] *= s[r];
       if constexpr (F16) fit_half(dp, ak, ex, mul);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          sum_apart<T, D>(dt_, s, t, i, lane, av[i]);
+          sum_apart<T, D>(qt, dp, t, i, lane, ak[i]);
+        }
+      } else
 #pragma unroll
       for (int c = 0; c < 32 / O::CH; ++c) {
         const frag pf = O::pack(s, c), gf = O::pack(dp, c);

@@ -254,3 +254,34 @@ def test_attention_dq_of_narrow_heads(lens, heads, d, block, dtype):
     kw = dict(cu_seqlens=table(cu), causal_block=block)
     out, lse = ca.attention(q, k, v, **kw)
     assert rounding_ratio(ca.attention_backward(dout.cuda(), q, k, v, out, lse, **kw)[0], ref["dq"]) <= 1.25
+
+
+def rel(got, want):
+    return float((got.double().cpu() - want).norm() / want.norm())
+
+
+def test_attention_fp32_sums_of_long_walks():
+    """A sum of N random terms whose every addition rounds by U / sqrt(3) (rms) of the sum so far is off by sqrt(N / 2) U / sqrt(3) of the
+    result.  dk and dv of 4 heads' 2048 queries, out and dq of 8192 keys: in one chain, two products an instruction, 4096 roundings
+    make 1.6e-6; sums apart for 32 rows leave 256 and 16: 4e-7.  p adds 5e-7: lse and the exponent's argument, 8 .. 16, are held to
+    half of 2^-20 three times.  Together 6.5e-7, and half as much again for the sample, scores and exp: 1e-6."""
+    heads, kv, d, n = 16, 4, 64, 2048
+    cu, qkv, dout = packed([n] * 8, 0, heads, kv, d, F32)
+    q, k, v = split(qkv.cuda(), heads, kv)
+    out, lse = ca.attention(q, k, v, seq_len=n)
+    _, dk, dv = ca.attention_backward(dout.cuda(), q, k, v, out, lse, seq_len=n)
+    ref, _ = attention_ref(qkv[:n, :4], qkv[:n, heads:heads + 1], qkv[:n, heads + kv:heads + kv + 1], [0, n], 0, d ** -0.5, dout[:n, :4])
+    for name, t in (("dk", dk), ("dv", dv)):
+        assert rel(t[:n, :1], ref[name]) <= 1e-6, name
+    n, d = 8192, 16
+    cu, qkv, dout = packed([n], 0, 3, 3, d, F32)
+    q, k, v = split(qkv.cuda(), 3, 3)
+    out, lse = ca.attention(q, k, v)
+    dq = ca.attention_backward(dout.cuda(), q, k, v, out, lse)[0]
+    # the reference's first 256 rows
+    Q, K, V, G = (t.double().transpose(0, 1) for t in (qkv[:256, :3], qkv[:, 3:6], qkv[:, 6:], dout[:256]))
+    p = torch.softmax(Q @ K.transpose(1, 2) / 4, 2)
+    O = p @ V
+    ds = p * (G @ V.transpose(1, 2) - (G * O).sum(2, keepdim=True))
+    assert rel(out[:256].transpose(0, 1), O) <= 1e-6
+    assert rel(dq[:256].transpose(0, 1), ds @ K / 4) <= 1e-6
