@@ -250,34 +250,39 @@ template <typename T, int D> __device__ __forceinline__ void sum_apart(const T* 
 }
 
 // fp16 holds 2^-24 .. 2^16, and ds ~ p do / sqrt(n) of an unscaled loss lies below.  A tile of ds, whose column is the lane's own
-// row, therefore enters its product times mul = 2^-e, and so do the sums acc.  Every lane has an e of its own: small values of a
+// row, therefore enters its product times 2^-e, and so do the sums acc: times mul here, or (IN) it comes so.  Every lane has an e of its own: small values of a
 // row keep their bits whatever the other rows hold.  Kept while the column's largest value comes out in 2^-8 .. 2^15 (what fp16 then
 // rounds by 2^-25 is 2^-17 of it), else set so that it is in 2^4 .. 2^5: e is hardly ever changed, and costs a search of the tile.
 // The probabilities of dk/dv, 1 / n where all keys are alike, enter times 2^14: fp16 then holds them with 11 bits down to 2^-28.
 constexpr int P_EXP = 14;
 constexpr int LEAST_EXP = -30;     // ds below 2^-38 gives nothing in fp16 results; the sums times 2^30 stay finite
-template <int N> __device__ __forceinline__ void fit_half(f32x16& ds, f32x16 (&acc)[N], int& e, float& mul) {
+template <bool IN, int N> __device__ __forceinline__ void fit_half(f32x16& ds, f32x16 (&acc)[N], int& e, float& mul) {
   float big = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(ds[r]));
+  if (!IN) big *= mul;
   // a lane pair shares a column: it is too small if both halves are, and not both empty
-  unsigned long long small = __ballot(big * mul < 0x1p-8f && e > LEAST_EXP), none = __ballot(big == 0.f);
+  unsigned long long small = __ballot(big < 0x1p-8f && e > LEAST_EXP), none = __ballot(big == 0.f);
   small &= small >> 32; none &= none >> 32;
-  if ((unsigned)(small & ~none) || __any(big * mul > 0x1p15f)) {
+  if ((unsigned)(small & ~none) || __any(big > 0x1p15f)) {
     big = half_max(big);
     int to = e;
-    if (big < INFINITY && (big * mul > 0x1p15f || (big > 0.f && big * mul < 0x1p-8f)))
-      to = min(max(__builtin_amdgcn_frexp_expf(big) - 5, LEAST_EXP), 90);
+    if (big < INFINITY && (big > 0x1p15f || (big > 0.f && big < 0x1p-8f)))
+      to = min(max(__builtin_amdgcn_frexp_expf(big) - 5 + e, LEAST_EXP), 90);
     const float f = __builtin_amdgcn_ldexpf(1.f, e - to);
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+    if (IN)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] *= f;
     e = to;
     mul = __builtin_amdgcn_ldexpf(1.f, -to);
   }
+  if (!IN)
 #pragma unroll
-  for (int r = 0; r < 16; ++r) ds[r] *= mul;
+    for (int r = 0; r < 16; ++r) ds[r] *= mul;
 }
 
 // ---- forward -------------------------------------------------------------------------------------
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // nothing and triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
 // FINE: ds enters its product in two pieces of the 16-bit type, so that its rounding does not count (the rule is at bwd).
 template <typename T, int D, int DK, int NW, bool SPLIT, bool FINE>
-__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 2) void attn_bwd_q(const AttnP p) {
+__global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : sizeof(T) == 2 && D == 64 ? 3 : 2) void attn_bwd_q(const AttnP p) {
   typedef Op<T> O; typedef Tile<T, D> L; typedef typename O::frag frag;
   constexpr bool F16 = __is_same(T, _Float16);
   typedef Walk<T, D, NW, SPLIT> W;
@@ -528,13 +533,13 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
         dp = O::mma(L::row_frag(v, 32 * t, c, lane), df[c], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -lse2)) * dp[r];
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, F16 ? -lse2 - (float)ex : -lse2)) * dp[r];
       if (j0 + 32 * t + 32 > wave_min) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (j0 + 32 * t + acc_row(r, h) >= lim) s[r] = 0.f;
       }
-      if constexpr (F16) fit_half(s, acc, ex, mul);
+      if constexpr (F16) fit_half<true>(s, acc, ex, mul);
       if constexpr (sizeof(T) == 4 && D <= 64) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) sum_apart<T, D>(k, s, t, i, lane, acc[i]);
@@ -676,7 +681,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 4 && D > 64) || D == 128 ? 1
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-      if constexpr (F16) fit_half(dp, ak, ex, mul);
+      if constexpr (F16) fit_half<false>(dp, ak, ex, mul);
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
