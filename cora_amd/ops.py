@@ -167,7 +167,7 @@ def _attention_inputs(q, k, v, cu_seqlens, seq_len, causal_block, scale):
         raise ValueError(f"heads {heads}, kv_heads {kv}, head_dim {d} and the number of sequences {n_seq} must be below 2^31")
     if not -_MOST <= causal_block <= _MOST:
         raise ValueError(f"causal_block must be 0 or positive and below 2^31, got {causal_block}")
-    head = (code, heads, kv, d, n_seq, n, causal_block, d ** -0.5 if scale is None else scale, rows, table,
+    head = (code, heads, kv, d, n_seq, n, causal_block, (d or 1) ** -0.5 if scale is None else scale, rows, table,
             q.data_ptr(), k.data_ptr(), v.data_ptr())
     return head, _heads(q, "q") + _heads(k, "k") + _heads(v, "v")
 
@@ -273,7 +273,7 @@ def orthogonalize(x, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), 
     code, first = _lead(xs[0], "x"), xs[0]
     stacks = []
     for i, t in enumerate(xs):
-        _like(t, f"x[{i}]", first, t.shape)
+        _like(t, f"x[{i}]", first, getattr(t, "shape", None))
         if t.dim() not in (2, 3):
             raise ValueError(f"matrices must be [rows, cols] or [count, rows, cols], got shape {tuple(t.shape)}")
         if outs[i] is None:

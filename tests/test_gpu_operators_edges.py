@@ -285,3 +285,11 @@ def test_attention_fp32_sums_of_long_walks():
     ds = p * (G @ V.transpose(1, 2) - (G * O).sum(2, keepdim=True))
     assert rel(out[:256].transpose(0, 1), O) <= 1e-6
     assert rel(dq[:256].transpose(0, 1), ds @ K / 4) <= 1e-6
+
+
+def test_refusals_name_what_is_wrong():
+    x = torch.zeros(8, 2, 0, dtype=BF16, device="cuda")
+    with pytest.raises(ca._lib.CoraError, match="head_dim"):
+        ca.attention(x, x, x)
+    with pytest.raises(TypeError, match="torch tensor"):
+        ca.orthogonalize([torch.zeros(4, 4, device="cuda"), [[1.0]]])
