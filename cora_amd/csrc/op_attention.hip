@@ -14,8 +14,9 @@
 // product is fetched in the same order and the probabilities never pass through LDS.
 // fp32 operands use v_mfma_f32_32x32x2_f32, 16-bit ones v_mfma_f32_32x32x16_*; a "chunk" is what one 16-byte register
 // piece per lane covers of the contraction: 8 channels in fp32, 16 in 16 bits.
-// All sums, statistics and accumulators are fp32.  The probabilities (and ds) of 16-bit operands are rounded to the
-// operands' type before their product, as the matrix unit takes them; their row sum is taken before that rounding (lse is exact to fp32).
+// All sums, statistics and accumulators are fp32; fp32's are taken 32 rows at a time (sum_apart).  The probabilities (and ds) of 16-bit
+// operands are rounded to the operands' type before their product, as the matrix unit takes them, or given in two pieces (FINE, at
+// bwd); their row sum is taken before that rounding (lse is exact to fp32).  fp16's enter times powers of two (fit_half).
 //
 // No atomics: every output element is summed by one wave in a fixed order, so results repeat bit for bit.
 #include "op_tile.h"
@@ -226,7 +227,8 @@ __device__ __forceinline__ void join_own(f32x16 (&acc)[D / 32], float* lds, int 
 
 // Issue order of the block it stands in: READS reads of LDS first, then N times M matrix instructions followed by PER more reads.
 // Left alone the compiler reads an operand right before its use, and where few waves share a SIMD nothing else hides
-// the way from LDS: dk/dv of 16-bit types at 128 channels 2.9 ms, so 2.7; q k of the fp32 forward pass 77 us, so 73 (sizes as below).
+// the way from LDS: dk/dv of 16-bit types at 128 channels 2.9 ms, so 2.7; the fp32 forward pass 77 us, so 73 (sizes as below; without a
+// profiler, which adds 2 to 4 us).
 // The 16-bit forward pass and dq, whose tiles are longer, gain nothing or lose.
 template <int READS, int PER, int N, int GROUP, int M = 1> __device__ __forceinline__ void feed() {
   __builtin_amdgcn_sched_group_barrier(0x100, READS, GROUP);
@@ -290,7 +292,8 @@ template <bool IN, int N> __device__ __forceinline__ void fit_half(f32x16& ds, f
 // from LDS, which four SIMDs reading at once is all that LDS gives (128 bytes a cycle).  One workgroup per 128 queries, two to
 // a compute unit; or, for few rows, four waves that share 32 queries (the rule and its figures are at run below).  Measured, causal
 // bf16: 16384 tokens x 16 heads of 128 1.05 ms, 1050 TFLOP/s (a large library product: 1133); fp32 64 images of 196 tokens x 8 heads of 48
-// 73 us, much of it padding (196 queries to 256, 196 keys to 224, in the second product 48 channels to 64).
+// 75 us: padding (196 queries to 256, 196 keys to 224, in the second product 48 channels to 64), two rounds of workgroups, and matrix
+// units that are busy 64 % of the cycles in which their compute unit has waves (dq 66 %, dk/dv 68 %).
 // The running maximum m only has to keep exp2 in range, so it is raised (and the sums
 // scaled) when a score exceeds it by 8 in log2 units, not at every new maximum: the sums then carry factors up to 2^8.
 // Each row goes by its own scores, so its result does not depend on which other rows share its tile.
@@ -431,7 +434,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 }
 
 // ---- backward: dq (and the row constants the dk/dv kernel reads) ---------------------------------
-// Three products where the forward pass has two, bound like it: 16384 tokens x 16 heads of 128, causal bf16, 1.55 ms, 1060 TFLOP/s.
+// Three products where the forward pass has two, bound like it: 16384 tokens x 16 heads of 128, causal bf16, 1.5 ms, 1100 TFLOP/s.
 // q k and do v are computed here and in the dk/dv kernel: seven products instead of five, but no atomics and no ds in memory.
 // The row constants are -delta, from which the product do v starts, and -lse (log2 units).  (Starting q k from -lse / scale saves
 // nothing and triples the error of fp32 gradients: the sum is then rounded at the size of lse / scale.)
@@ -583,7 +586,7 @@ __global__ __launch_bounds__(64 * NW, SPLIT || (sizeof(T) == 4 && D > 64) ? 1 : 
 // With p.parts > 1 that walk is cut into as many ranges, one per workgroup (blockIdx.y), whose sums go to the workspace in
 // fp32 and are added in order by attn_bwd_sum: few workgroups with long walks would leave most of the chip idle.
 // Four products.  The two accumulators and the own keys and values fill the registers: at 128 channels one wave per SIMD, and
-// vector work (exp, masks, packing) is not hidden behind another wave's matrix instructions: 2.7 ms, 810 TFLOP/s at the size above.
+// vector work (exp, masks, packing) is not hidden behind another wave's matrix instructions: 2.65 ms, 830 TFLOP/s at the size above.
 // Staged rows behind the sequence are zeros, or pieces of its last rows where rows repeat or overlap (a stride below the
 // row's length); their -lse is set to -infinity, so their p and ds are zero whatever is there.
 template <typename T, int D, int DK, int NW, bool FINE>
@@ -777,8 +780,8 @@ template <typename T, int D, int DK, int NW, bool SPLIT> int bwd(const AttnP& p,
 // Forward and dq, few rows: with W = rows * heads / 32 waves of queries and 1024 SIMDs, splitting the keys over the waves of
 // a workgroup pays up to W = 512 where two such workgroups fit a compute unit (D <= 64), to 256 above, and to twice that
 // for causal walks over long sequences, whose last tiles keep the rest waiting.  Forward, us, split / not:
-//   fp32 D 64:  16 x 1024 tokens x 1 head (W 512) 55 / 77;  4 x 1024 x 8 (W 1024) 107 / 86;  1 x 4096 x 8 causal 193 / 285
-//   bf16 D 128: 1 x 4096 x 2 (W 256) 43 / 77;  16 x 1024 x 1 (W 512) 32 / 26;  1 x 16384 x 1 causal (W 512) 171 / 291
+//   fp32 D 64:  16 x 1024 tokens x 1 head (W 512) 60 / 82;  4 x 1024 x 8 (W 1024) 102 / 81;  1 x 4096 x 8 causal 199 / 292
+//   bf16 D 128: 1 x 4096 x 2 (W 256) 46 / 80;  16 x 1024 x 1 (W 512) 33 / 26;  1 x 16384 x 1 causal (W 512) 176 / 288
 template <typename T, int D, int DK, bool BWD> int run(const AttnP& p, hipStream_t st) {
   constexpr int NS = sizeof(T) == 4 && D > 64 ? 2 : 4;      // waves whose buffers fit LDS
   const long long w = p.rows * p.heads / 32, most = (D <= 64 ? 512 : 256) * (p.block && p.rows / p.nseq >= 2048 ? 2 : 1);
@@ -786,7 +789,7 @@ template <typename T, int D, int DK, bool BWD> int run(const AttnP& p, hipStream
   if constexpr (BWD) return bwd<T, D, DK, 4, false>(p, st); else return fwd<T, D, DK, 4, false>(p, st);
 }
 // D: channels of the tiles and of the results, 32 at a time; DK: channels of the score products.  In fp32, which the matrix unit
-// bounds, 16 of padding are left out there: 64 images of 196 tokens, 8 heads of 48, forward / dq / dk and dv 77 / 107 / 146 us,
+// bounds, 16 of padding are left out there: 64 images of 196 tokens, 8 heads of 48, forward / dq / dk and dv 77 / 108 / 144 us under a profiler,
 // with all 64 channels 88 / 125 / 159.  In 16 bits it gives nothing (fp16, heads of 80 as 80 or 96 channels: 80 / 101 / 144, 78 / 104 / 143).
 template <typename T, bool BWD> int run_d(const AttnP& p, hipStream_t st) {
   if constexpr (sizeof(T) == 4)
@@ -801,8 +804,9 @@ template <bool BWD> int run_t(const AttnP& p, int dtype, hipStream_t st) {
 
 // dk/dv: parts until there is a workgroup per compute unit, and four where the walks are causal and long; a part keeps at
 // least 256 queries (fp32 128).  Whole backward pass, us, 1 / 2 / 4 parts:
-//   fp32 D 64: 16 x 1024 tokens x 1 head 251 / 197 / 197;  4 x 1024 x 8: 264 / 264 / 275;  1 x 4096 x 8 causal 912 / 888 / 775
-//   bf16 D 64: 1 x 4096 x 2: 140 / 108 / 95;  16 x 1024 x 4: 76 / 100 / 127;  the packed clips' dk/dv (12 of 4 heads) 300 / 203
+//   fp32 D 64: 16 x 1024 tokens x 1 head 212 / 159 / 161;  4 x 1024 x 8: 250 / 253 / 263;  1 x 4096 x 8 causal 810 / 772 / 644
+//   bf16 D 64: 1 x 4096 x 2: 108 / 79 / 66;  16 x 1024 x 4: 78 / 100 / 120;  12 packed clips of very different lengths, 12 of 4 heads,
+//   causal, with the forward pass 450 / 397 / 406
 int attention_parts(int dtype, long long rows, int nseq, int heads, int kv_heads, int block) {
   if (nseq < 1) return 1;
   const long long blocks = (rows / 128 + nseq) * kv_heads, walk = rows / nseq * (heads / kv_heads);
