@@ -2,10 +2,12 @@
 #include "../../include/cora_hip.h"
 #include "ops.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <vector>
 
 void cora_note_error(const char* msg) noexcept;   // ctx.hip
 
@@ -347,23 +349,28 @@ int cora_orthogonalize(int dtype, const cora_matrices* stacks, int n_stacks, int
     if (s.x == s.y && ((s.rows > 1 && s.x_row != s.y_row) || (s.count > 1 && s.x_mat != s.y_mat)))
       return refuse("%s: stack %d: in place, x and y need the same strides", who, i);
   }
-  for (int i = 0; i < n_stacks; ++i)
-    for (int j = 0; j < n_stacks; ++j)
-      if (i != j && stacks[i].count && stacks[j].count && (stacks[i].y == stacks[j].y || stacks[i].y == stacks[j].x))
-        return refuse("%s: y of stack %d is x or y of stack %d", who, i, j);
   if (!any) return 0;
   const long long eb = op_bytes(dtype);
   auto x_of = [&](const cora_matrices& s) { return Span{(long long)(uintptr_t)s.x, s.count, s.x_mat * eb, s.rows, s.x_row * eb, s.cols * eb}; };
   auto y_of = [&](const cora_matrices& s) { return Span{(long long)(uintptr_t)s.y, s.count, s.y_mat * eb, s.rows, s.y_row * eb, s.cols * eb}; };
-  for (int i = 0; i < n_stacks; ++i) {
-    if (!stacks[i].count) continue;
-    const Span y = y_of(stacks[i]);
-    for (int j = 0; j < n_stacks; ++j) {
-      if (!stacks[j].count) continue;
-      if ((i != j || stacks[i].x != stacks[i].y) && meet(y, x_of(stacks[j]))) return refuse("%s: y of stack %d overlaps x of stack %d", who, i, j);
-      if (i < j && meet(y, y_of(stacks[j]))) return refuse("%s: y of stack %d overlaps y of stack %d", who, i, j);
+  // in the order of their addresses only neighbours need to be compared
+  struct Item { Span s; int stack; bool y; };
+  std::vector<Item> all;
+  try {
+    all.reserve(2 * (size_t)n_stacks);
+  } catch (...) { return refuse("%s: out of host memory", who); }
+  for (int i = 0; i < n_stacks; ++i)
+    if (stacks[i].count) { all.push_back({x_of(stacks[i]), i, false}); all.push_back({y_of(stacks[i]), i, true}); }
+  std::sort(all.begin(), all.end(), [](const Item& a, const Item& b) { return a.s.at < b.s.at; });
+  for (size_t k = 0; k < all.size(); ++k)
+    for (size_t l = k + 1; l < all.size() && all[l].s.at < all[k].s.end(); ++l) {
+      if (!all[k].y && !all[l].y) continue;
+      const bool first = all[k].y && (!all[l].y || all[k].stack < all[l].stack);
+      const Item &y = first ? all[k] : all[l], &o = first ? all[l] : all[k];
+      if (y.s.at == o.s.at) {
+        if (y.stack != o.stack) return refuse("%s: y of stack %d is x or y of stack %d", who, y.stack, o.stack);
+      } else if (meet(y.s, o.s)) return refuse("%s: y of stack %d overlaps %c of stack %d", who, y.stack, o.y ? 'y' : 'x', o.stack);
     }
-  }
   const size_t need = cora_orthogonalize_workspace(dtype, stacks, n_stacks);
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < need)
     return refuse("%s: workspace is NULL, not 256-byte aligned or smaller than %zu bytes", who, need);
