@@ -53,7 +53,7 @@ def _no_grad(t, name: str) -> None:
     if t.requires_grad and _torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: these operators are not recorded by autograd; use the *_backward "
                          "calls under torch.no_grad(), or detach it")
-    if getattr(_duals, "_current_level", 0) >= 0 and _duals.unpack_dual(t).tangent is not None:
+    if _duals._current_level >= 0 and _duals.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} carries a tangent: these operators have no forward-mode derivative; take its primal")
 
 
@@ -88,20 +88,29 @@ def _heads(t, name: str):
     return row, head
 
 
+_axes = {}           # axes_dim -> its C array
+
+
+def _axes_array(axes_dim):
+    if not 1 <= len(axes_dim) <= 4:
+        raise ValueError(f"axes_dim must name 1 to 4 axes, got {len(axes_dim)}")
+    if not all(-_MOST <= n <= _MOST for n in axes_dim):
+        raise ValueError(f"axes_dim must be positive, even and at most 128, got {axes_dim}")
+    if len(_axes) >= 256:
+        _axes.clear()
+    return _axes.setdefault(axes_dim, (C.c_int32 * 4)(*axes_dim))
+
+
 def _rotary(x, positions, axes_dim, theta, interleaved, out, backward):
     code = _lead(x, "x")
     if x.dim() != 3:
         raise ValueError(f"x must be [rows, heads, head_dim], got shape {tuple(x.shape)}")
     n_axes = len(axes_dim)
-    if not 1 <= n_axes <= 4:
-        raise ValueError(f"axes_dim must name 1 to 4 axes, got {n_axes}")
+    axes = _axes.get(axes_dim := tuple(axes_dim)) or _axes_array(axes_dim)
     _table(positions, "positions", x, _torch.int32, 2, f"int32 tensor [n, {n_axes}]")
     rows, heads, d = x.shape
     if heads > _MOST or d > _MOST:
         raise ValueError(f"x has shape {tuple(x.shape)}: heads and head_dim must be below 2^31")
-    for n in axes_dim:
-        if not -_MOST <= n <= _MOST:
-            raise ValueError(f"axes_dim must be positive, even and at most 128, got {tuple(axes_dim)}")
     n, width = positions.shape
     if width != n_axes:
         raise ValueError(f"positions must be a contiguous int32 tensor [n, {n_axes}], got {tuple(positions.shape)}")
@@ -115,7 +124,7 @@ def _rotary(x, positions, axes_dim, theta, interleaved, out, backward):
         return out
     xr, xh = _heads(x, "x")
     yr, yh = _heads(out, "out")
-    a = _lib.CoraRotaryArgs(code, heads, d, n_axes, tuple(axes_dim), 1 if interleaved else 0, backward, theta, rows, n,
+    a = _lib.CoraRotaryArgs(code, heads, d, n_axes, axes, 1 if interleaved else 0, backward, theta, rows, n,
                             positions.data_ptr(), x.data_ptr(), out.data_ptr(), xr, xh, yr, yh)
     index = x.get_device()
     _lib.check(_lib.load().cora_rotary(a, index, _stream(index)))
@@ -282,7 +291,7 @@ def orthogonalize(x, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), 
             _like(outs[i], "out", t, t.shape)
         if t.numel():
             count, rows, cols, xm, xr = _matrices(t, "x")
-            if max(count, rows, cols) > _MOST:
+            if count > _MOST or rows > _MOST or cols > _MOST:
                 raise ValueError(f"x[{i}] has shape {tuple(t.shape)}: rows and columns must be at most 32768")
             ym, yr = _matrices(outs[i], "out")[3:]
             stacks.append((t.data_ptr(), outs[i].data_ptr(), xm, xr, ym, yr, count, rows, cols))

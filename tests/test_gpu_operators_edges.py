@@ -232,10 +232,10 @@ def test_attention_dq_of_rows_that_see_few_keys(n, heads, d, block, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("lens,heads,kv,d,block", [([46], 2, 2, 16, 1), ([2, 3, 0, 2, 2, 3, 4], 3, 3, 48, 196), ([5, 17], 2, 2, 64, 64), ([7] * 9, 8, 2, 128, 0),
-                                                   ([338], 8, 8, 16, 5), ([100] * 10, 4, 4, 16, 0), ([300, 96], 4, 4, 80, 1)])
+                                                   ([338], 8, 8, 16, 5), ([100] * 10, 4, 4, 16, 0), ([200, 50], 4, 4, 80, 1)])
 def test_attention_gradients_of_small_calls(lens, heads, kv, d, block, dtype):
     """ds and p enter in two pieces, 2^-17 off and less, which leaves the results' own rounding (1) and that of out through delta (up to
-    half as much, 1.12 together).  In one piece each would add 1 more: 1.41 .. 1.8.  Up to 4096 rows and heads."""
+    half as much, 1.12 together).  In one piece each would add 1 more: 1.41 .. 1.8.  Up to 1024 rows x heads, 4096 of heads up to 24."""
     cu, qkv, dout = packed(lens, 0, heads, kv, d, dtype, seed=11)
     ref, _ = attention_ref(*split(qkv, heads, kv), cu, block, d ** -0.5, dout)
     q, k, v = split(qkv.cuda(), heads, kv)
