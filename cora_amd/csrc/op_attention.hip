@@ -758,7 +758,7 @@ template <typename T, int D, int DK, int NW, bool SPLIT> int fwd(const AttnP& p,
 // plain form, one piece / two, bf16: 46 tokens, 2 heads of 16, causal, 1.67 1.48 1.29 / 1.03 1.02 1.00; 2258 + 257 tokens, 4 heads of 16, dq
 // 1.53 / 1.08; 906 random calls with this rule: 1.50 at most.  Backward pass, us: 10 x 100 tokens, 4 heads of 16, 10.6 / 11.6; 8 x 512, 8
 // heads of 24 (dq alone), causal, 28.6 / 31.2.  With no need for it: dq of heads of 32 426 for 352 (8 x 2048 tokens, 16 heads, fp16); 702 + 223
-// tokens, 2 heads of 80, causal, 44 for 36.
+// tokens, 2 heads of 80, causal, with the forward pass 59 for 51.
 template <typename T, int D, int DK, int NW, bool SPLIT, bool FINE> int bwd_q(const AttnP& p, hipStream_t st) {
   attn_bwd_q<T, D, DK, NW, SPLIT, FINE><<<dim3((unsigned)(slots(p, Walk<T, D, NW, SPLIT>::QT) * p.heads)), 64 * NW, 0, st>>>(p);
   return hipGetLastError() != hipSuccess;
